@@ -357,6 +357,83 @@ SCMIAC_API int scmiac_ntxent2_backward(const float *zi, const float *zj, int64_t
                                        float *dzi, float *dzj, void *workspace, size_t workspace_bytes,
                                        void *stream);
 
+/*
+ * Element types of the entry points below, whose arrays are `void *`.
+ */
+#define SCMIAC_F32 0
+#define SCMIAC_F16 1
+#define SCMIAC_BF16 2
+
+/*
+ * Dense layer with its epilogue (the encoder layers of the training loop, and scores of cells against
+ * a table of reference cells; no entry point of the reference's own):
+ *     z = x w^T + bias,   y = act(z) + residual
+ *   x [m, k] (rows ldx elements apart), w [n, k] (ldw), bias [n] or NULL, residual [m, n] (ldr) or NULL;
+ *   y [m, n] out; z [m, n] out: the pre-activation as backward reads it, or NULL.  All of one `dtype`;
+ *   sums in float32 (float32 products are exact to float32's own rounding).  m >= 0; n, k >= 1.
+ * backward: dy [m, n]; z as forward left it (may be NULL for SCMIAC_ACT_NONE);
+ *   dx [m, k], dw [n, k], dbias [n] out, each may be NULL.  The gradient of `residual` is dy itself.
+ *   Sums over rows are taken in an order that depends on the shape alone: results repeat bit for bit.
+ * Both take scmiac_linear_workspace_size(m, n, k, dtype, act, backward) bytes of device scratch.
+ */
+#define SCMIAC_ACT_NONE 0
+#define SCMIAC_ACT_RELU 1
+#define SCMIAC_ACT_GELU 2 /* z Phi(z), with the error function */
+#define SCMIAC_ACT_SILU 3 /* z / (1 + exp(-z)) */
+SCMIAC_API int scmiac_linear_workspace_size(int64_t m, int64_t n, int64_t k, int dtype, int act, int backward,
+                                            size_t *bytes);
+SCMIAC_API int scmiac_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
+                                     const void *residual, int64_t ldr, int64_t m, int64_t n, int64_t k, int dtype,
+                                     int act, void *y, void *z, void *workspace, size_t workspace_bytes, void *stream);
+SCMIAC_API int scmiac_linear_backward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *z,
+                                      const void *dy, int64_t m, int64_t n, int64_t k, int dtype, int act, void *dx,
+                                      void *dw, void *dbias, void *workspace, size_t workspace_bytes, void *stream);
+
+/*
+ * The k largest entries of each row, by (value descending, index ascending), and the row's
+ * log-sum-exp: a teacher's side of scmiac_distill_forward.  No counterpart in the reference.
+ *   x [n, v] of `dtype`, rows ld elements apart; 1 <= k <= SCMIAC_TOP_MAX_K; temperature > 0
+ *   values [n, k] of `dtype`, idx [n, k] int32: past the end of a row of fewer than k classes -inf and -1
+ *   (the padding of the k-NN tables).  lse [n] float32 = log sum_j exp(x_j / temperature).
+ * A row that holds a NaN has lse NaN; its entries are then unspecified (indices stay within the row).
+ */
+#define SCMIAC_TOP_MAX_K 64
+SCMIAC_API int scmiac_top_logits_workspace_size(int64_t n, int64_t v, int k, int dtype, size_t *bytes);
+SCMIAC_API int scmiac_top_logits(const void *x, int64_t ld, int64_t n, int64_t v, int dtype, int k, float temperature,
+                                 void *values, int32_t *idx, float *lse, void *workspace, size_t workspace_bytes,
+                                 void *stream);
+
+/*
+ * Distillation from a teacher's top logits (no counterpart in the reference; beside
+ * scmiac_ntxent2_forward as the loss of soft targets).  Per row, with student logits x [v], the teacher's
+ * logits a_i of the classes idx_i, i < k, temperatures T (student) and Ta (teacher):
+ *     t_i = exp(a_i / Ta - c),   c = log sum_i exp(a_i / Ta), or teacher_lse where given
+ *     L   = sum_i t_i (log t_i - log softmax(x / T)[idx_i])
+ *   idx [n, k] int32, top [n, k] float32, teacher_lse [n] float32 or NULL, x of `dtype`, rows ld apart.
+ *   idx -1 is padding, and a weight t_i of 0 contributes nothing.  A class may be listed more than once.  A row
+ *   without a teacher (all padding, or all a_i -inf) and a row whose classes are all -inf have L = 0 and no
+ *   gradient.  An idx below -1 or from v on, or a listed a_i that is NaN, makes the row's L and gradient NaN.
+ * forward: reduction SCMIAC_REDUCE_NONE: loss [n]; _MEAN: loss [1] over the rows that count (those not
+ *   described above as L = 0), 0 if there are none; _SUM: loss [1].  row_stats [4 n] and scale [1]
+ *   (MEAN, SUM) float32 are what backward reads.
+ * backward: dx [n, v] of `dtype` (rows ldd apart): d L / d x, times grad[i * grad_stride] (float32, device) and
+ *   *scale (or 1 where scale is NULL).  Deterministic.
+ *   1 <= k <= SCMIAC_DISTILL_MAX_K, 1 <= v < 2^31, 0 <= n < 2^24.
+ */
+#define SCMIAC_DISTILL_MAX_K 1024
+#define SCMIAC_REDUCE_NONE 0
+#define SCMIAC_REDUCE_MEAN 1
+#define SCMIAC_REDUCE_SUM 2
+SCMIAC_API int scmiac_distill_workspace_size(int64_t n, int64_t v, int dtype, size_t *bytes);
+SCMIAC_API int scmiac_distill_forward(const void *x, int64_t ld, int64_t n, int64_t v, int dtype, const int32_t *idx,
+                                      const float *top, int k, const float *teacher_lse, float temperature,
+                                      float teacher_temperature, int reduction, float *loss, float *row_stats,
+                                      float *scale, void *workspace, size_t workspace_bytes, void *stream);
+SCMIAC_API int scmiac_distill_backward(const void *x, int64_t ld, int64_t n, int64_t v, int dtype, const int32_t *idx,
+                                       const float *top, int k, float temperature, float teacher_temperature,
+                                       const float *row_stats, const float *grad, int64_t grad_stride,
+                                       const float *scale, void *dx, int64_t ldd, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

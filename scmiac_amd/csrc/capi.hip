@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "../../include/scmiac_hip.h"
+#include "api_error.h"
 #include "kernels.h"
 
 using namespace scmiac;
@@ -20,6 +21,7 @@ static int fail(int code, const char* fmt, ...) {
     va_end(ap);
     return code;
 }
+int scmiac::api_fail(int code, const char* message) { return fail(code, "%s", message); }
 static int hip_fail(hipError_t e, const char* what) {
     return fail(SCMIAC_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }

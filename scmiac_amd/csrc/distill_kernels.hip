@@ -1,0 +1,823 @@
+// A teacher's top logits and the loss of learning from them.
+//
+//   top_logits       values, idx = the k largest of each row, by (value descending, index ascending);
+//                    lse = log sum_j exp(x_j / T)
+//   distill forward  t_i = exp(a_i / Ta - c)  over the listed classes, c their log-sum-exp or the teacher's own,
+//                    tau = sum t_i,   L = sum_i t_i (log t_i - x[idx_i] / T) + tau lse(x / T)
+//   distill backward dL/dx_j = (tau p_j - sum_{i: idx_i = j} t_i) / T,   p = softmax(x / T)
+//
+// All of it is bound by reading the rows once (and, backward, writing them once); one pass keeps a
+// running maximum and sum of exponentials per lane, in the exponent's own unit (base 2, so that
+// the scale c = log2(e) / T is one multiply-add in front of v_exp_f32):
+//     s = sum exp2(x c - mc),  mc = the rounded product max * c.
+// Every later use takes the same mc, so its rounding cancels.  A row belongs to one wave (short rows), to the
+// four waves of a block, or to several blocks whose results a second kernel joins (few rows).
+#include <hip/hip_runtime.h>
+
+#include "train_common.h"
+#include "train_kernels.h"
+
+namespace scmiac {
+namespace {
+
+using namespace train;
+
+typedef unsigned long long u64;
+
+constexpr int kThreads = 256;
+constexpr int kWaves = kThreads / 64;
+constexpr int kMaxTop = 64;        // one entry per lane of a wave
+constexpr int kShortRow = 1024;    // up to here a wave takes a whole row: a block's four waves would find less than
+                                   // one 16-byte vector per lane each
+constexpr int kLoads = 4;          // vectors a lane has in flight
+constexpr int kAhead = 2;          // vectors fetched ahead of the one at work, where the k best are kept
+
+// ------------------------------------------------------------------ running log-sum-exp
+
+struct LseAcc {
+    float m, mc, s;   // maximum, its rounded product with c, sum of exp2(x c - mc)
+    __device__ __forceinline__ void init() { m = -INFINITY, mc = 0.f, s = 0.f; }
+    __device__ __forceinline__ void raise(float vm, float c) {
+        if (vm > m) {
+            s *= fast_exp2((m - vm) * c);   // m = -inf: 0
+            m = vm;
+            mc = vm * c;
+        }
+    }
+    __device__ __forceinline__ void add(float x, float c) { s += fast_exp2(fmaf(x, c, -mc)); }
+    // all lanes of the wave
+    __device__ __forceinline__ void join_wave(float c) {
+        const float top = wave_max(m);
+        const float tc = (top == -INFINITY) ? 0.f : top * c;
+        s = wave_sum((m == -INFINITY) ? 0.f : s * fast_exp2(mc - tc));
+        m = top;
+        mc = tc;
+    }
+};
+// joins n (m, s) pairs; the result is the same in whatever lane it is computed
+__device__ __forceinline__ LseAcc join_pairs(const float2* p, int n, float c) {
+    LseAcc a;
+    a.init();
+    for (int i = 0; i < n; ++i) a.m = fmaxf(a.m, p[i].x);
+    a.mc = (a.m == -INFINITY) ? 0.f : a.m * c;
+    for (int i = 0; i < n; ++i)
+        if (p[i].x != -INFINITY) a.s += p[i].y * fast_exp2(p[i].x * c - a.mc);
+    return a;
+}
+__device__ __forceinline__ float lse_value(const LseAcc& a) {
+    if (a.m == -INFINITY || a.m == INFINITY) return a.s != a.s && a.m == -INFINITY ? a.s : a.m;
+    return (a.mc + log2f(a.s)) * kLn2;
+}
+
+// ------------------------------------------------------------------ a row, vector by vector
+
+// Calls body(f, first index) for the 16-byte vectors of columns [lo, hi) of a row and one(x, index, valid)
+// for the elements in front of the first aligned vector and behind the last, ascending in index for
+// every wave.  Wave `w` of `W` takes every W-th kilobyte.
+template <typename T, typename Body, typename One>
+__device__ __forceinline__ void stream_row(const T* __restrict__ row, long long lo, long long hi, int w, int W, Body body,
+                                           One one) {
+    constexpr int N = Vec16<T>::N;
+    const int lane = threadIdx.x & 63;
+    const uintptr_t addr = reinterpret_cast<uintptr_t>(row + lo);
+    long long head = (long long)(((16 - (addr & 15)) & 15) / sizeof(T));
+    if (head > hi - lo) head = hi - lo;
+    const long long nv = (hi - lo - head) / N;
+    const long long tail0 = lo + head + nv * N;
+    if (w == 0 && head > 0) {
+        const bool valid = lane < head;
+        one(valid ? to_f32(row[lo + lane]) : -INFINITY, lo + lane, valid);
+    }
+    const u32x4* __restrict__ vec = reinterpret_cast<const u32x4*>(row + lo + head);
+    const long long step = (long long)W * 64;
+    long long v0 = (long long)w * 64;
+    for (; v0 + step * (kLoads - 1) + 64 <= nv; v0 += step * kLoads) {
+        Vec16<T> buf[kLoads];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) buf[u].raw = vec[v0 + step * u + lane];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) body(buf[u], lo + head + (v0 + step * u + lane) * N, true);
+    }
+    for (; v0 < nv; v0 += step) {
+        const bool valid = v0 + lane < nv;
+        Vec16<T> buf;
+        buf.raw = vec[valid ? v0 + lane : nv - 1];
+        body(buf, lo + head + (v0 + lane) * N, valid);
+    }
+    if (w == 0 && tail0 < hi) {
+        const bool valid = tail0 + lane < hi;
+        one(valid ? to_f32(row[tail0 + lane]) : -INFINITY, tail0 + lane, valid);
+    }
+}
+
+template <typename T>
+__device__ __forceinline__ float unpack(const Vec16<T>& v, float (&f)[Vec16<T>::N]) {
+#pragma unroll
+    for (int i = 0; i < Vec16<T>::N; ++i) f[i] = v.get(i);
+    float m = f[0];
+#pragma unroll
+    for (int i = 1; i < Vec16<T>::N; ++i) m = fmaxf(m, f[i]);
+    return m;
+}
+
+// ------------------------------------------------------------------ top k
+
+// An entry: the value as a whole number of the same order in the upper half, ~index in the lower;
+// larger is better, and no entry is 0.
+__device__ __forceinline__ uint32_t order_key(float x) {
+    const uint32_t b = __float_as_uint(x + 0.f);   // -0 and +0 are the same value
+    return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
+}
+__device__ __forceinline__ float key_value(uint32_t k) {
+    return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
+}
+__device__ __forceinline__ u64 make_entry(float x, long long index) {
+    return ((u64)order_key(x) << 32) | (uint32_t)~(uint32_t)index;
+}
+
+// The smallest entry of a selection of at least k of the wave's entries e[0..R) (0: none): exactly the k
+// best where slack is 0, up to `slack` more otherwise.  Bisection over the values, then over the
+// indices of one value, each step a compare and a population count per 64 entries.
+template <int R>
+__device__ __forceinline__ u64 select_from(const u64 (&e)[R], int k, int slack) {
+    auto count_hi = [&](uint32_t t) {
+        int c = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) c += __popcll(__ballot((uint32_t)(e[r] >> 32) >= t));
+        return c;
+    };
+    if (count_hi(1u) <= k) return 1ull;
+    uint32_t best = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) best = max(best, (uint32_t)(e[r] >> 32));
+#pragma unroll
+    for (int off = 32; off; off >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, off));
+    best = (uint32_t)__builtin_amdgcn_readfirstlane((int)best);
+    uint32_t lo = 1u, hi = best;              // count(lo) >= k;  count(hi + 1) = 0
+    while (lo < hi) {
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        const int c = count_hi(mid);
+        if (c >= k) {
+            lo = mid;
+            if (c <= k + slack) return (u64)lo << 32;
+        } else {
+            hi = mid - 1;
+        }
+    }
+    // more than k + slack entries >= lo, fewer than k above it: the rest by index among those of value lo
+    int above = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) above += __popcll(__ballot((uint32_t)(e[r] >> 32) > lo));
+    const int need = k - above;
+    uint32_t l2 = 0u, h2 = 0xffffffffu;
+    while (l2 < h2) {
+        const uint32_t mid = l2 + (h2 - l2) / 2 + 1;
+        int c = 0;
+#pragma unroll
+        for (int r = 0; r < R; ++r) c += __popcll(__ballot((uint32_t)(e[r] >> 32) == lo && (uint32_t)e[r] >= mid));
+        if (c >= need) {
+            l2 = mid;
+            if (c == need) break;
+        } else {
+            h2 = mid - 1;
+        }
+    }
+    return ((u64)lo << 32) | l2;
+}
+
+// writes the entries >= t of the wave to dst[0..), in any order; returns how many
+template <int R>
+__device__ __forceinline__ int keep_entries(const u64 (&e)[R], u64 t, u64* dst) {
+    int n = 0;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const u64 mask = __ballot(e[r] >= t);
+        if (e[r] >= t) dst[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] = e[r];
+        n += __popcll(mask);
+    }
+    return n;
+}
+
+// the k best (up to `slack` more) of buf[0..cnt) to the front of buf; t: the smallest kept
+template <int R>
+__device__ __forceinline__ int shrink_list(u64* buf, int cnt, int k, int slack, u64& t) {
+    const int lane = threadIdx.x & 63;
+    u64 e[R];
+    wave_lds_fence();
+#pragma unroll
+    for (int r = 0; r < R; ++r) e[r] = (r * 64 + lane < cnt) ? buf[r * 64 + lane] : 0ull;
+    t = select_from<R>(e, k, slack);
+    const int n = keep_entries<R>(e, t, buf);
+    wave_lds_fence();
+    return n;
+}
+
+// The candidates of one wave, in LDS: everything that may still be among the k best of what the wave has seen.
+template <typename T>
+struct WaveList {
+    static constexpr int kTrigger = 256;
+    static constexpr int kCap = kTrigger + 64 * Vec16<T>::N;   // a vector adds up to 64 N entries
+    u64* buf;
+    int cnt, k;
+    float tau;      // k entries of the list are >= tau; all of them came earlier, so a later entry must exceed it
+    bool open;      // fewer than k entries seen: everything is taken
+    __device__ __forceinline__ void init(u64* b, int k_) { buf = b, cnt = 0, k = k_, tau = -INFINITY, open = true; }
+    __device__ __forceinline__ void shrink(int slack) {
+        u64 t;
+        // (registers for as many entries as there are: a step of the selection costs three instructions per 64)
+        if (cnt <= kTrigger) cnt = shrink_list<kTrigger / 64>(buf, cnt, k, slack, t);
+        else if (cnt <= 384) cnt = shrink_list<6>(buf, cnt, k, slack, t);
+        else cnt = shrink_list<kCap / 64>(buf, cnt, k, slack, t);
+        if (cnt >= k) {
+            tau = key_value((uint32_t)(t >> 32));
+            open = false;
+        }
+    }
+    __device__ __forceinline__ void push(float x, long long index, bool valid) {
+        const bool take = valid && (open || x > tau);
+        const u64 mask = __ballot(take);
+        if (mask) {
+            if (take) buf[cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] = make_entry(x, index);
+            cnt += __popcll(mask);
+        }
+    }
+    __device__ __forceinline__ void room() {
+        if (cnt > kTrigger) shrink(k / 4);
+    }
+};
+
+// Rank of each lane's entry among the wave's first n lanes (0: the best).
+__device__ __forceinline__ int rank_of(u64 e, int n) {
+    int rank = 0;
+    for (int j = 0; j < n; ++j) {
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(e >> 32), j), lo = __builtin_amdgcn_readlane((uint32_t)e, j);
+        rank += ((((u64)hi << 32) | lo) > e) ? 1 : 0;
+    }
+    return rank;
+}
+
+template <typename T>
+__device__ __forceinline__ void write_top(u64 e, int found, int k, T* __restrict__ values, int* __restrict__ idx) {
+    const int lane = threadIdx.x & 63;
+    if (lane < found) {
+        const int r = rank_of(e, found);
+        values[r] = from_f32<T>(key_value((uint32_t)(e >> 32)));
+        idx[r] = (int)~(uint32_t)e;
+    } else if (lane < k) {       // fewer classes than k: the tables' padding
+        values[lane] = from_f32<T>(-INFINITY);
+        idx[lane] = -1;
+    }
+}
+
+// Block (row group, split).  WPR: waves per row.
+template <typename T, int WPR>
+__global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restrict__ x, long long ld, long long n, long long v,
+                                                              int k, float c, int splits, long long split_len,
+                                                              T* __restrict__ values, int* __restrict__ idx,
+                                                              float* __restrict__ lse, u64* __restrict__ part,
+                                                              float2* __restrict__ part_ms) {
+    constexpr int N = Vec16<T>::N;
+    __shared__ u64 lists[kWaves][WaveList<T>::kCap];
+    __shared__ float2 ms[kWaves];
+    __shared__ int counts[kWaves];
+    const int wave = wave_id(), lane = threadIdx.x & 63;
+    const int w = wave % WPR;
+    const long long row = (long long)blockIdx.x * (kWaves / WPR) + wave / WPR;
+    const bool live = row < n;
+    const int split = blockIdx.y;
+    const long long lo = split * split_len, hi = min(v, lo + split_len);
+
+    LseAcc acc;
+    acc.init();
+    WaveList<T> list;
+    list.init(lists[wave], k);
+    if (live) {
+        // the elements in front of the first 16-byte vector, the vectors (every WPR-th kilobyte), the
+        // elements behind the last one: one step each of one loop, so that the list's code exists once
+        const T* xr = x + row * ld;
+        long long head = (long long)(((16 - (reinterpret_cast<uintptr_t>(xr + lo) & 15)) & 15) / sizeof(T));
+        if (head > hi - lo) head = hi - lo;
+        const long long nv = (hi - lo - head) / N, body = lo + head, tail = body + nv * N;
+        const u32x4* vecs = reinterpret_cast<const u32x4*>(xr + body);
+        const long long step = (long long)WPR * 64;
+        long long at = (long long)w * 64;
+        bool front = w == 0 && head > 0, back = w == 0 && tail < hi;
+        auto fetch = [&](long long v0) {
+            u32x4 r = {0u, 0u, 0u, 0u};
+            if (v0 + lane < nv) r = vecs[v0 + lane];
+            return r;
+        };
+        u32x4 ahead[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) ahead[u] = fetch(at + u * step);
+        while (true) {
+            float f[N], vm;
+            int valid;              // elements of this lane
+            long long first;
+            if (!front && at < nv) {
+                Vec16<T> cur;
+                cur.raw = ahead[0];
+#pragma unroll
+                for (int u = 0; u + 1 < kAhead; ++u) ahead[u] = ahead[u + 1];
+                ahead[kAhead - 1] = fetch(at + kAhead * step);
+                vm = unpack<T>(cur, f);
+                valid = (at + lane < nv) ? N : 0;
+                first = body + (at + lane) * N;
+                at += step;
+            } else if (front || back) {
+                const long long from = front ? lo : tail, to = front ? body : hi;
+                valid = (from + lane < to) ? 1 : 0;
+                first = from + lane;
+                f[0] = vm = valid ? to_f32(xr[first]) : -INFINITY;
+#pragma unroll
+                for (int i = 1; i < N; ++i) f[i] = -INFINITY;
+                if (front) front = false;
+                else back = false;
+            } else {
+                break;
+            }
+            if (valid) {
+                acc.raise(vm, c);
+#pragma unroll
+                for (int i = 0; i < N; ++i) acc.add(f[i], c);
+            }
+            if (__any(valid && (list.open || vm > list.tau))) {
+                list.room();
+#pragma unroll
+                for (int i = 0; i < N; ++i) list.push(f[i], first + i, i < valid);
+            }
+        }
+        acc.join_wave(c);
+    }
+    // the k best of the wave, then of the row's waves
+    u64 mine = 0;
+    int found = 0;
+    {
+        list.shrink(0);
+        found = list.cnt;
+        if (WPR == 1) mine = (lane < found) ? list.buf[lane] : 0ull;
+    }
+    if (WPR > 1) {
+        if (lane == 0) {
+            ms[wave] = make_float2(acc.m, acc.s);
+            counts[wave] = found;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        u64 e[kWaves];
+#pragma unroll
+        for (int q = 0; q < kWaves; ++q) e[q] = (lane < counts[q]) ? lists[q][lane] : 0ull;
+        acc = join_pairs(ms, kWaves, c);
+        const u64 t = select_from<kWaves>(e, k, 0);
+        found = keep_entries<kWaves>(e, t, lists[0]);
+        wave_lds_fence();
+        mine = (lane < found) ? lists[0][lane] : 0ull;
+    }
+    if (!live) return;
+    if (splits > 1) {
+        if (lane < k) part[(row * splits + split) * k + lane] = mine;
+        if (lane == 0) part_ms[row * splits + split] = make_float2(acc.m, acc.s);
+        return;
+    }
+    write_top<T>(mine, found, k, values + row * k, idx + row * k);
+    if (lane == 0) lse[row] = lse_value(acc);
+}
+
+// Joins the splits of a row: sixteen waves take up to 1024 entries each, the first joins their best.
+constexpr int kJoinWaves = 16;
+constexpr int kJoinR = 16;
+template <typename T>
+__global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k, float c, int splits, const u64* __restrict__ part,
+                                                                          const float2* __restrict__ part_ms,
+                                                                          T* __restrict__ values, int* __restrict__ idx,
+                                                                          float* __restrict__ lse) {
+    __shared__ u64 best[kJoinWaves * kMaxTop];
+    __shared__ int counts[kJoinWaves];
+    const int wave = wave_id(), lane = threadIdx.x & 63;
+    const long long row = blockIdx.x;
+    const int total = splits * k;
+    const u64* src = part + row * total;
+    u64 e[kJoinR];
+#pragma unroll
+    for (int r = 0; r < kJoinR; ++r) {
+        const int at = (r * kJoinWaves + wave) * 64 + lane;
+        e[r] = (at < total) ? src[at] : 0ull;
+    }
+    u64 t = select_from<kJoinR>(e, k, 0);
+    int found = keep_entries<kJoinR>(e, t, best + wave * kMaxTop);
+    if (lane == 0) counts[wave] = found;
+    __syncthreads();
+    if (wave == 1) {
+        LseAcc acc;
+        acc.init();
+        for (int i = lane; i < splits; i += 64) {
+            const float2 p = part_ms[row * splits + i];
+            if (p.x > acc.m) {
+                acc.s *= fast_exp2((acc.m - p.x) * c);
+                acc.m = p.x;
+                acc.mc = p.x * c;
+            }
+            if (p.x != -INFINITY) acc.s += p.y * fast_exp2(p.x * c - acc.mc);
+        }
+        acc.join_wave(c);
+        if (lane == 0) lse[row] = lse_value(acc);
+    }
+    if (wave != 0) return;
+#pragma unroll
+    for (int r = 0; r < kJoinWaves; ++r) e[r] = (lane < counts[r]) ? best[r * kMaxTop + lane] : 0ull;
+    t = select_from<kJoinR>(e, k, 0);
+    found = keep_entries<kJoinR>(e, t, best);
+    wave_lds_fence();
+    const u64 mine = (lane < found) ? best[lane] : 0ull;
+    write_top<T>(mine, found, k, values + row * k, idx + row * k);
+}
+
+// ------------------------------------------------------------------ distillation
+
+// What a row's forward pass leaves for its backward pass, and for the loss.
+//   x = mc, y = log2 of the sum (softmax p = exp2(x c - mc - y)); z = the teacher's normaliser (base 2),
+//   w = tau: 0 for a row without a teacher (or without a class), NaN for a row with an index that is none
+__device__ __forceinline__ float teacher_weight(float a, float ca, float cn) { return fast_exp2(fmaf(a, ca, -cn)); }
+
+// One wave: the teacher's distribution of a row against the student's log-sum-exp.
+template <typename T>
+__device__ __forceinline__ void finish_row(const T* __restrict__ xr, long long v, float c, const LseAcc& acc,
+                                           const int* __restrict__ idx, const float* __restrict__ top, int k,
+                                           const float* __restrict__ teacher_lse, float ca, long long row,
+                                           float* __restrict__ loss, float4* __restrict__ stats) {
+    const int lane = threadIdx.x & 63;
+    const int* ir = idx + row * k;
+    const float* ar = top + row * k;
+    float top_max = -INFINITY;
+    bool bad = false;
+    for (int i = lane; i < k; i += 64) {
+        const int j = ir[i];
+        bad |= j < -1 || j >= v;
+        if (j >= 0 && j < v) {
+            const float a = ar[i];
+            bad |= a != a;
+            top_max = fmaxf(top_max, a);
+        }
+    }
+    top_max = wave_max(top_max);
+    bad = __any(bad);
+    float cn;   // base 2
+    if (teacher_lse) {
+        cn = teacher_lse[row] * kLog2e;
+    } else {
+        const float mc = (top_max == -INFINITY) ? 0.f : top_max * ca;
+        float s = 0.f;
+        for (int i = lane; i < k; i += 64) {
+            const int j = ir[i];
+            if (j >= 0 && j < v) s += fast_exp2(fmaf(ar[i], ca, -mc));
+        }
+        cn = mc + log2f(wave_sum(s));
+    }
+    // sum t (log t - (x - max)) + tau log(sum): differences from the row's maximum, where little cancels
+    float tau = 0.f, part = 0.f;
+    if (top_max != -INFINITY && acc.m != -INFINITY) {
+        for (int i = lane; i < k; i += 64) {
+            const int j = ir[i];
+            if (j >= 0 && j < v) {
+                const float t = teacher_weight(ar[i], ca, cn);
+                if (!(t <= 0.f)) {
+                    const float s = fmaf(to_f32(xr[j]), c, -acc.mc);
+                    part += t * (fmaf(ar[i], ca, -cn) - s);
+                    tau += t;
+                }
+            }
+        }
+        tau = wave_sum(tau);
+        part = wave_sum(part);
+    }
+    const float l2s = log2f(acc.s);
+    if (lane == 0) {
+        const bool empty = top_max == -INFINITY || acc.m == -INFINITY;
+        float value = empty ? 0.f : kLn2 * fmaf(tau, l2s, part);
+        if (bad || acc.s != acc.s) value = tau = NAN;
+        loss[row] = value;
+        stats[row] = make_float4(acc.mc, l2s, cn, tau);
+    }
+}
+
+template <typename T, int WPR>
+__global__ __launch_bounds__(kThreads) void distill_forward_kernel(const T* __restrict__ x, long long ld, long long n,
+                                                                   long long v, float c, int splits, long long split_len,
+                                                                   const int* __restrict__ idx, const float* __restrict__ top,
+                                                                   int k, const float* __restrict__ teacher_lse, float ca,
+                                                                   float* __restrict__ loss, float4* __restrict__ stats,
+                                                                   float2* __restrict__ part_ms) {
+    constexpr int N = Vec16<T>::N;
+    __shared__ float2 ms[kWaves];
+    const int wave = wave_id(), lane = threadIdx.x & 63;
+    const int w = wave % WPR;
+    const long long row = (long long)blockIdx.x * (kWaves / WPR) + wave / WPR;
+    const bool live = row < n;
+    const int split = blockIdx.y;
+    const long long lo = split * split_len, hi = min(v, lo + split_len);
+    const T* xr = x + row * ld;
+    LseAcc acc;
+    acc.init();
+    if (live) {
+        stream_row<T>(
+            xr, lo, hi, w, WPR,
+            [&](const Vec16<T>& vec, long long, bool valid) {
+                float f[N];
+                const float vm = unpack<T>(vec, f);
+                if (valid) {
+                    acc.raise(vm, c);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) acc.add(f[i], c);
+                }
+            },
+            [&](float xv, long long, bool valid) {
+                if (valid) {
+                    acc.raise(xv, c);
+                    acc.add(xv, c);
+                }
+            });
+        acc.join_wave(c);
+    }
+    if (WPR > 1) {
+        if (lane == 0) ms[wave] = make_float2(acc.m, acc.s);
+        __syncthreads();
+        if (wave != 0) return;
+        acc = join_pairs(ms, kWaves, c);
+    }
+    if (!live) return;
+    if (splits > 1) {
+        if (lane == 0) part_ms[row * splits + split] = make_float2(acc.m, acc.s);
+        return;
+    }
+    finish_row<T>(xr, v, c, acc, idx, top, k, teacher_lse, ca, row, loss, stats);
+}
+
+template <typename T>
+__global__ __launch_bounds__(64) void distill_join_kernel(const T* __restrict__ x, long long ld, long long v, float c, int splits,
+                                                          const float2* __restrict__ part_ms, const int* __restrict__ idx,
+                                                          const float* __restrict__ top, int k,
+                                                          const float* __restrict__ teacher_lse, float ca,
+                                                          float* __restrict__ loss, float4* __restrict__ stats) {
+    const long long row = blockIdx.x;
+    LseAcc acc;
+    acc.init();
+    for (int i = threadIdx.x; i < splits; i += 64) {
+        const float2 p = part_ms[row * splits + i];
+        if (p.x > acc.m) {
+            acc.s *= fast_exp2((acc.m - p.x) * c);
+            acc.m = p.x;
+            acc.mc = p.x * c;
+        }
+        if (p.x != -INFINITY) acc.s += p.y * fast_exp2(p.x * c - acc.mc);
+    }
+    acc.join_wave(c);
+    finish_row<T>(x + row * ld, v, c, acc, idx, top, k, teacher_lse, ca, row, loss, stats);
+}
+
+// Sum (mean: over the rows that have a teacher) of the rows' losses, in an order that depends on n alone.
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* __restrict__ row_loss,
+                                                                  const float4* __restrict__ stats, long long n, int mean,
+                                                                  float* __restrict__ loss, float* __restrict__ scale) {
+    __shared__ double sums[kSumThreads / 64];
+    __shared__ int counts[kSumThreads / 64];
+    double sum = 0.0;
+    int count = 0;
+    for (long long i = threadIdx.x; i < n; i += kSumThreads) {
+        sum += (double)row_loss[i];
+        count += !(stats[i].w == 0.f);
+    }
+    for (int off = 32; off; off >>= 1) {
+        sum += __shfl_xor(sum, off);
+        count += __shfl_xor(count, off);
+    }
+    if ((threadIdx.x & 63) == 0) {
+        sums[threadIdx.x >> 6] = sum;
+        counts[threadIdx.x >> 6] = count;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        sum = 0.0;
+        count = 0;
+        for (int i = 0; i < kSumThreads / 64; ++i) {
+            sum += sums[i];
+            count += counts[i];
+        }
+        const double d = (mean && count > 1) ? (double)count : 1.0;
+        loss[0] = (float)(sum / d);
+        scale[0] = (float)(1.0 / d);
+    }
+}
+
+// Block (row group, split): the dense part of the split's columns, then the listed classes among them.
+// The dense pass has written tau p g / T there; the second write replaces it with the difference, computed
+// in float32 from x again, so that nothing is lost where p and t nearly cancel.
+template <typename T, int WPR>
+__global__ __launch_bounds__(kThreads) void distill_backward_kernel(const T* __restrict__ x, long long ld, long long n,
+                                                                    long long v, float c, float inv_t, int splits,
+                                                                    long long split_len, const int* __restrict__ idx,
+                                                                    const float* __restrict__ top, int k, float ca,
+                                                                    const float4* __restrict__ stats,
+                                                                    const float* __restrict__ grad, long long grad_stride,
+                                                                    const float* __restrict__ scale, T* __restrict__ dx,
+                                                                    long long ldd) {
+    constexpr int N = Vec16<T>::N;
+    extern __shared__ int listed[];       // [kWaves / WPR][k]
+    const int wave = wave_id(), lane = threadIdx.x & 63;
+    const int w = wave % WPR, group = wave / WPR;
+    const long long row = (long long)blockIdx.x * (kWaves / WPR) + group;
+    const bool live = row < n;
+    const int split = blockIdx.y;
+    const long long lo = split * split_len, hi = min(v, lo + split_len);
+    const T* xr = x + row * ld;
+    T* dr = dx + row * ldd;
+    float4 st = make_float4(0.f, 0.f, 0.f, 0.f);
+    float g = 0.f;
+    if (live) {
+        st = stats[row];
+        g = grad[row * grad_stride] * inv_t;
+        if (scale) g *= scale[0];
+        int* mine = listed + group * k;
+        for (int i = w * 64 + lane; i < k; i += WPR * 64) mine[i] = idx[row * k + i];
+        const float f0 = st.w * g;
+        const bool empty = st.w == 0.f;
+        auto dense = [&](float xv) { return empty ? 0.f : f0 * fast_exp2(fmaf(xv, c, -st.x) - st.y); };
+        if (((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15) == 0) {
+            stream_row<T>(
+                xr, lo, hi, w, WPR,
+                [&](const Vec16<T>& vec, long long first, bool valid) {
+                    float f[N];
+                    unpack<T>(vec, f);
+#pragma unroll
+                    for (int i = 0; i < N; ++i) f[i] = dense(f[i]);
+                    Vec16<T> out;
+                    out.set(f);
+                    if (valid) *reinterpret_cast<u32x4*>(dr + first) = out.raw;
+                },
+                [&](float xv, long long index, bool valid) {
+                    if (valid) dr[index] = from_f32<T>(dense(xv));
+                });
+        } else {      // rows of x and dx that start at different offsets from 16 bytes
+            for (long long j = lo + w * 64 + lane; j < hi; j += WPR * 64) dr[j] = from_f32<T>(dense(to_f32(xr[j])));
+        }
+    }
+    __syncthreads();
+    if (!live || st.w == 0.f) return;
+    const int* mine = listed + group * k;
+    const float* ar = top + row * k;
+    for (int i = w * 64 + lane; i < k; i += WPR * 64) {
+        const int j = mine[i];
+        if (j < lo || j >= hi) continue;
+        // a class that is listed more than once is written by its first entry, with all of its weight
+        bool first = true;
+        for (int q = 0; q < i; ++q) first &= mine[q] != j;
+        if (!first) continue;
+        float t = 0.f;
+        for (int q = i; q < k; ++q)
+            if (mine[q] == j) t += teacher_weight(ar[q], ca, st.z);
+        const float p = fast_exp2(fmaf(to_f32(xr[j]), c, -st.x) - st.y);
+        dr[j] = from_f32<T>(g * fmaf(st.w, p, -t));
+    }
+}
+
+// ------------------------------------------------------------------ launch shapes
+
+// Splits of a row: enough blocks for the chip's 256 compute units several times over, none shorter than
+// 4096 columns (16 KiB of float32: below that a block's start and end cost more than its columns), no
+// more than a join can take.
+constexpr long long kMinSplit = 4096;
+constexpr int kMaxSplits = 256;
+void plan_splits(long long n, long long v, int esize, int& splits, long long& len) {
+    splits = 1;
+    len = v;
+    if (v <= kShortRow || n < 1) return;
+    const long long want = ceil_div(1024, n);
+    long long s = want < v / kMinSplit ? want : v / kMinSplit;
+    if (s > kMaxSplits) s = kMaxSplits;
+    if (s <= 1) return;
+    len = round_up(ceil_div(v, s), 64 * (16 / esize));
+    splits = (int)ceil_div(v, len);
+    if (splits == 1) len = v;
+}
+
+inline int esize_of(int dtype) { return dtype == 0 ? 4 : 2; }
+
+template <typename T>
+hipError_t top_logits_t(const void* x, long long ld, long long n, long long v, int k, float temperature, void* values,
+                        int* idx, float* lse, void* ws, hipStream_t stream) {
+    const float c = kLog2e / temperature;
+    int splits;
+    long long len;
+    plan_splits(n, v, sizeof(T), splits, len);
+    const T* xt = static_cast<const T*>(x);
+    T* vt = static_cast<T*>(values);
+    u64* part = static_cast<u64*>(ws);
+    float2* part_ms = reinterpret_cast<float2*>(part + (size_t)n * splits * k);
+    if (v <= kShortRow) {
+        top_logits_kernel<T, 1><<<dim3((unsigned)ceil_div(n, kWaves)), kThreads, 0, stream>>>(xt, ld, n, v, k, c, 1, v, vt, idx,
+                                                                                               lse, nullptr, nullptr);
+    } else {
+        top_logits_kernel<T, kWaves><<<dim3((unsigned)n, splits), kThreads, 0, stream>>>(xt, ld, n, v, k, c, splits, len, vt,
+                                                                                        idx, lse, part, part_ms);
+        if (splits > 1)
+            top_logits_join_kernel<T><<<dim3((unsigned)n), 64 * kJoinWaves, 0, stream>>>(k, c, splits, part, part_ms, vt, idx, lse);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t distill_forward_t(const DistillArgs& a, int reduction, float* loss, float4* stats, float* scale, void* ws,
+                             hipStream_t stream) {
+    const float c = kLog2e / a.temperature, ca = kLog2e / a.teacher_temperature;
+    int splits;
+    long long len;
+    plan_splits(a.n, a.v, sizeof(T), splits, len);
+    const T* x = static_cast<const T*>(a.x);
+    float2* part_ms = static_cast<float2*>(ws);
+    float* row_loss = reduction == 0 ? loss : reinterpret_cast<float*>(part_ms + (size_t)a.n * splits);
+    if (a.n > 0) {
+        if (a.v <= kShortRow) {
+            distill_forward_kernel<T, 1><<<dim3((unsigned)ceil_div(a.n, kWaves)), kThreads, 0, stream>>>(
+                x, a.ld, a.n, a.v, c, 1, a.v, a.idx, a.top, a.k, a.teacher_lse, ca, row_loss, stats, nullptr);
+        } else {
+            distill_forward_kernel<T, kWaves><<<dim3((unsigned)a.n, splits), kThreads, 0, stream>>>(
+                x, a.ld, a.n, a.v, c, splits, len, a.idx, a.top, a.k, a.teacher_lse, ca, row_loss, stats, part_ms);
+            if (splits > 1)
+                distill_join_kernel<T><<<dim3((unsigned)a.n), 64, 0, stream>>>(x, a.ld, a.v, c, splits, part_ms, a.idx, a.top,
+                                                                              a.k, a.teacher_lse, ca, row_loss, stats);
+        }
+    }
+    if (reduction != 0)
+        distill_sum_kernel<<<1, kSumThreads, 0, stream>>>(row_loss, stats, a.n, reduction == 1, loss, scale);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t distill_backward_t(const DistillArgs& a, const float4* stats, const float* grad, long long grad_stride,
+                              const float* scale, void* dx, long long ldd, hipStream_t stream) {
+    const float c = kLog2e / a.temperature, ca = kLog2e / a.teacher_temperature;
+    int splits;
+    long long len;
+    plan_splits(a.n, a.v, sizeof(T), splits, len);
+    const T* x = static_cast<const T*>(a.x);
+    T* d = static_cast<T*>(dx);
+    if (a.v <= kShortRow)
+        distill_backward_kernel<T, 1><<<dim3((unsigned)ceil_div(a.n, kWaves)), kThreads, sizeof(int) * kWaves * a.k, stream>>>(
+            x, a.ld, a.n, a.v, c, 1.f / a.temperature, 1, a.v, a.idx, a.top, a.k, ca, stats, grad, grad_stride, scale, d, ldd);
+    else
+        distill_backward_kernel<T, kWaves><<<dim3((unsigned)a.n, splits), kThreads, sizeof(int) * a.k, stream>>>(
+            x, a.ld, a.n, a.v, c, 1.f / a.temperature, splits, len, a.idx, a.top, a.k, ca, stats, grad, grad_stride, scale, d,
+            ldd);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+size_t top_logits_workspace_bytes(long long n, long long v, int k, int dtype) {
+    int splits;
+    long long len;
+    plan_splits(n, v, esize_of(dtype), splits, len);
+    return splits > 1 ? (size_t)n * splits * ((size_t)k * sizeof(u64) + sizeof(float2)) : 0;
+}
+
+size_t distill_workspace_bytes(long long n, long long v, int dtype) {
+    if (n == 0) return 0;
+    int splits;
+    long long len;
+    plan_splits(n, v, esize_of(dtype), splits, len);
+    return (size_t)n * splits * sizeof(float2) + (size_t)n * sizeof(float);
+}
+
+hipError_t launch_top_logits(const void* x, long long ld, long long n, long long v, int dtype, int k, float temperature,
+                             void* values, int* idx, float* lse, void* ws, hipStream_t stream) {
+    if (n == 0) return hipSuccess;
+    switch (dtype) {
+        case 0: return top_logits_t<float>(x, ld, n, v, k, temperature, values, idx, lse, ws, stream);
+        case 1: return top_logits_t<f16>(x, ld, n, v, k, temperature, values, idx, lse, ws, stream);
+        default: return top_logits_t<bf16>(x, ld, n, v, k, temperature, values, idx, lse, ws, stream);
+    }
+}
+
+hipError_t launch_distill_forward(const DistillArgs& a, int reduction, float* loss, float* row_stats, float* scale,
+                                  void* ws, hipStream_t stream) {
+    float4* stats = reinterpret_cast<float4*>(row_stats);
+    if (a.n == 0 && reduction == 0) return hipSuccess;
+    switch (a.dtype) {
+        case 0: return distill_forward_t<float>(a, reduction, loss, stats, scale, ws, stream);
+        case 1: return distill_forward_t<f16>(a, reduction, loss, stats, scale, ws, stream);
+        default: return distill_forward_t<bf16>(a, reduction, loss, stats, scale, ws, stream);
+    }
+}
+
+hipError_t launch_distill_backward(const DistillArgs& a, const float* row_stats, const float* grad, long long grad_stride,
+                                   const float* scale, void* dx, long long ldd, hipStream_t stream) {
+    const float4* stats = reinterpret_cast<const float4*>(row_stats);
+    if (a.n == 0) return hipSuccess;
+    switch (a.dtype) {
+        case 0: return distill_backward_t<float>(a, stats, grad, grad_stride, scale, dx, ldd, stream);
+        case 1: return distill_backward_t<f16>(a, stats, grad, grad_stride, scale, dx, ldd, stream);
+        default: return distill_backward_t<bf16>(a, stats, grad, grad_stride, scale, dx, ldd, stream);
+    }
+}
+
+}  // namespace scmiac
