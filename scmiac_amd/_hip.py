@@ -212,7 +212,8 @@ def knn_kept_fraction(q, r, k, *, groups=AUTO_PROBE_GROUPS, group_rows=None):
         group_rows = knn_grid_plan(n, m, q.shape[1], k, mode="pruned")["queries_per_block"]
     group_rows = max(1, min(group_rows, n))
     centres = q[torch.arange(groups, device=q.device) * (n // groups) + n // (2 * groups)]
-    score = (q * q).sum(1)[None, :] - 2.0 * (centres @ q.T)                # |q - c|^2 - |c|^2, a row per centre
+    # |q - c|^2 - |c|^2, a row per centre: q is read once for all of them
+    score = linear_forward(-2.0 * centres, q, (q * q).sum(1))[0]
     # a radius that holds the clump with room to spare, read off at most 65 536 evenly spaced
     # queries, so that the exact selection runs over a few thousand rows instead of all
     pool = score[:, ::max(1, n // AUTO_PROBE_POOL)] if n > AUTO_PROBE_POOL else score
@@ -566,6 +567,11 @@ def _size_of(name, *args):
     return nbytes.value
 
 
+def _raw_stream(device):
+    """:func:`_stream` for the operators of a training step, where its two microseconds count."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
 def _scratch(nbytes, device):
     """Scratch of one call.  Unlike :func:`_workspace`'s it belongs to the stream (or the graph under
     capture) that the call runs on, so that calls on two streams and two captured graphs never share it."""
@@ -592,7 +598,7 @@ def linear_forward(x, weight, bias=None, residual=None, activation="none", keep_
         y = torch.empty((m, n), dtype=x.dtype, device=device)
         z = torch.empty((m, n), dtype=x.dtype, device=device) if keep_z and act else None
         _check(load_library().scmiac_linear_forward(_ptr(x), ldx, _ptr(weight), ldw, _ptr(bias), _ptr(residual), ldr, m, n, k, code,
-                                          act, _ptr(y), _ptr(z), _ptr(ws), need, _stream()))
+                                          act, _ptr(y), _ptr(z), _ptr(ws), need, _raw_stream(device)))
     return y, z
 
 
@@ -612,7 +618,7 @@ def linear_backward(x, weight, z, dy, k, activation="none", need=(True, True, Tr
         dw = torch.empty((n, k), dtype=dy.dtype, device=device) if need[1] else None
         db = torch.empty((n,), dtype=dy.dtype, device=device) if need[2] else None
         _check(load_library().scmiac_linear_backward(_ptr(x), ldx, _ptr(weight), ldw, _ptr(z), _ptr(dy), m, n, k, code, act, _ptr(dx),
-                                           _ptr(dw), _ptr(db), _ptr(ws), size, _stream()))
+                                           _ptr(dw), _ptr(db), _ptr(ws), size, _raw_stream(device)))
     return dx, dw, db
 
 
@@ -628,7 +634,7 @@ def top_logits(x, k, temperature=1.0):
         idx = torch.empty((n, k), dtype=torch.int32, device=device)
         lse = torch.empty((n,), dtype=torch.float32, device=device)
         _check(load_library().scmiac_top_logits(_ptr(x), ld, n, v, code, k, float(temperature), _ptr(values), _ptr(idx), _ptr(lse),
-                                      _ptr(ws), size, _stream()))
+                                      _ptr(ws), size, _raw_stream(device)))
     return values, idx, lse
 
 
@@ -646,7 +652,7 @@ def distill_forward(x, idx, top, teacher_lse, temperature, teacher_temperature, 
         scale = torch.empty((), dtype=torch.float32, device=device) if red else None
         _check(load_library().scmiac_distill_forward(_ptr(x), ld, n, v, code, _ptr(idx), _ptr(top), idx.shape[1], _ptr(teacher_lse),
                                            temperature, teacher_temperature, red, _ptr(loss), _ptr(stats), _ptr(scale),
-                                           _ptr(ws), size, _stream()))
+                                           _ptr(ws), size, _raw_stream(device)))
     return loss, stats, scale
 
 
@@ -662,7 +668,7 @@ def distill_backward(x, idx, top, temperature, teacher_temperature, stats, scale
         dx = torch.empty((n, ldd), dtype=x.dtype, device=device)[:, :v]
         _check(load_library().scmiac_distill_backward(_ptr(x), ld, n, v, code, _ptr(idx), _ptr(top), idx.shape[1], temperature,
                                             teacher_temperature, _ptr(stats), _ptr(grad), grad_stride, _ptr(scale),
-                                            _ptr(dx), ldd, _stream()))
+                                            _ptr(dx), ldd, _raw_stream(device)))
     return dx
 
 

@@ -14,6 +14,7 @@ namespace {
 
 constexpr int64_t kMaxRows = ((int64_t)1 << 24) - 1;    // blocks of 256 threads in one launch
 constexpr int64_t kMaxWidth = ((int64_t)1 << 31) - 1;
+constexpr int64_t kMaxTiles = ((int64_t)1 << 23) - 1024;  // two products and their splits in one launch
 
 __attribute__((format(printf, 2, 3))) int fail(int code, const char* fmt, ...) {
     char text[256];
@@ -33,6 +34,7 @@ int check_dtype(int dtype) {
     return SCMIAC_OK;
 }
 int check_workspace(const void* ws, size_t have, size_t need) {
+    if ((reinterpret_cast<uintptr_t>(ws) & 15) != 0) return fail(SCMIAC_ERR_WORKSPACE, "workspace is not aligned to 16 bytes");
     if (need > have || (need && !ws)) return fail(SCMIAC_ERR_WORKSPACE, "workspace holds %zu bytes, %zu needed", have, need);
     return SCMIAC_OK;
 }
@@ -44,8 +46,8 @@ int check_linear(int64_t m, int64_t n, int64_t k, int dtype, int act) {
         return fail(SCMIAC_ERR_ARG, "m=%lld, n=%lld, k=%lld: needs 0 <= m, 1 <= n, k, below 2^31", (long long)m, (long long)n,
                     (long long)k);
     const int64_t tm = (m + 63) / 64, tn = (n + 63) / 64, tk = (k + 63) / 64;
-    if (tm * tn > kMaxRows || tm * tk > kMaxRows || tn * tk > kMaxRows)
-        return fail(SCMIAC_ERR_ARG, "m=%lld, n=%lld, k=%lld: a product of 2^24 tiles of 64 x 64 or more", (long long)m, (long long)n,
+    if (tm * tn > kMaxTiles || tm * tk > kMaxTiles || tn * tk > kMaxTiles)
+        return fail(SCMIAC_ERR_ARG, "m=%lld, n=%lld, k=%lld: a product of more than 2^23 - 1024 tiles of 64 x 64", (long long)m, (long long)n,
                     (long long)k);
     return SCMIAC_OK;
 }

@@ -6,12 +6,11 @@
 //                    tau = sum t_i,   L = sum_i t_i (log t_i - x[idx_i] / T) + tau lse(x / T)
 //   distill backward dL/dx_j = (tau p_j - sum_{i: idx_i = j} t_i) / T,   p = softmax(x / T)
 //
-// All of it is bound by reading the rows once (and, backward, writing them once); one pass keeps a
-// running maximum and sum of exponentials per lane, in the exponent's own unit (base 2, so that
-// the scale c = log2(e) / T is one multiply-add in front of v_exp_f32):
-//     s = sum exp2(x c - mc),  mc = the rounded product max * c.
-// Every later use takes the same mc, so its rounding cancels.  A row belongs to one wave (short rows), to the
-// four waves of a block, or to several blocks whose results a second kernel joins (few rows).
+// All of it is bound by reading the rows once (and, backward, writing them once): one pass keeps a running
+// maximum m and sum of exponentials s per lane, s = sum exp2((x - m) c) with c = log2(e) / T for v_exp_f32.  The
+// difference comes first: x c alone overflows for the lowest values of float32 and bfloat16, which serve as
+// masks, and near the maximum, where the weight is, it is exact.  A row belongs to one wave (short
+// rows), to the four waves of a block, or to several blocks whose results a second kernel joins (few rows).
 #include <hip/hip_runtime.h>
 
 #include "train_common.h"
@@ -27,31 +26,35 @@ typedef unsigned long long u64;
 constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;        // one entry per lane of a wave
+constexpr int kGather = 4;         // candidates of a row, in 64s, that are sorted out in one go (>= kWaves)
 constexpr int kShortRow = 1024;    // up to here a wave takes a whole row: a block's four waves would find less than
                                    // one 16-byte vector per lane each
 constexpr int kLoads = 4;          // vectors a lane has in flight
-constexpr int kAhead = 2;          // vectors fetched ahead of the one at work, where the k best are kept
+constexpr int kAhead = 4;          // vectors fetched ahead of the one at work, where the k best are kept
 
 // ------------------------------------------------------------------ running log-sum-exp
 
 struct LseAcc {
-    float m, mc, s;   // maximum, its rounded product with c, sum of exp2(x c - mc)
-    __device__ __forceinline__ void init() { m = -INFINITY, mc = 0.f, s = 0.f; }
+    float m, r, s;   // maximum; the same, or 0 while that is -inf; sum of exp2((x - r) c)
+    __device__ __forceinline__ void init() { m = -INFINITY, r = 0.f, s = 0.f; }
     __device__ __forceinline__ void raise(float vm, float c) {
         if (vm > m) {
             s *= fast_exp2((m - vm) * c);   // m = -inf: 0
-            m = vm;
-            mc = vm * c;
+            m = r = vm;
         }
     }
-    __device__ __forceinline__ void add(float x, float c) { s += fast_exp2(fmaf(x, c, -mc)); }
+    __device__ __forceinline__ void add(float x, float c) { s += fast_exp2((x - r) * c); }
+    // another sum, of entries up to its maximum om
+    __device__ __forceinline__ void join(float om, float os, float c) {
+        raise(om, c);
+        if (om != -INFINITY) s += os * fast_exp2((om - r) * c);
+    }
     // all lanes of the wave
     __device__ __forceinline__ void join_wave(float c) {
         const float top = wave_max(m);
-        const float tc = (top == -INFINITY) ? 0.f : top * c;
-        s = wave_sum((m == -INFINITY) ? 0.f : s * fast_exp2(mc - tc));
+        s = wave_sum((m == -INFINITY) ? s : s * fast_exp2((m - top) * c));   // (a NaN stays)
         m = top;
-        mc = tc;
+        r = (top == -INFINITY) ? 0.f : top;
     }
 };
 // joins n (m, s) pairs; the result is the same in whatever lane it is computed
@@ -59,14 +62,14 @@ __device__ __forceinline__ LseAcc join_pairs(const float2* p, int n, float c) {
     LseAcc a;
     a.init();
     for (int i = 0; i < n; ++i) a.m = fmaxf(a.m, p[i].x);
-    a.mc = (a.m == -INFINITY) ? 0.f : a.m * c;
-    for (int i = 0; i < n; ++i)
-        if (p[i].x != -INFINITY) a.s += p[i].y * fast_exp2(p[i].x * c - a.mc);
+    a.r = (a.m == -INFINITY) ? 0.f : a.m;
+    for (int i = 0; i < n; ++i) a.s += (p[i].x == -INFINITY) ? p[i].y : p[i].y * fast_exp2((p[i].x - a.r) * c);
     return a;
 }
-__device__ __forceinline__ float lse_value(const LseAcc& a) {
-    if (a.m == -INFINITY || a.m == INFINITY) return a.s != a.s && a.m == -INFINITY ? a.s : a.m;
-    return (a.mc + log2f(a.s)) * kLn2;
+__device__ __forceinline__ float lse_value(const LseAcc& a, float inv_t) {
+    if (a.m == INFINITY) return a.m;
+    if (a.s == 0.f) return -INFINITY;               // every entry -inf
+    return fmaf(a.m == -INFINITY ? 0.f : a.m, inv_t, kLn2 * log2f(a.s));
 }
 
 // ------------------------------------------------------------------ a row, vector by vector
@@ -269,10 +272,54 @@ __device__ __forceinline__ void write_top(u64 e, int found, int k, T* __restrict
     }
 }
 
+// A value that at least k of the row's (or split's) entries reach, from the largest entry of every lane's first few
+// vectors: 256 lanes (64 of a short row) of 8 to 32 entries each, whose k-th largest maximum is rarely far below the
+// k-th largest entry, so that of those few thousand entries little more than k become candidates instead of all.
+// 0: fewer than k lanes have one.  `keys`: 64 WPR words of LDS of this row.
+template <int WPR>
+__device__ __forceinline__ uint32_t bound_of_maxima(float lane_max, bool any, int k, uint32_t* keys, int w) {
+    const int lane = threadIdx.x & 63;
+    uint32_t e[WPR];
+    const uint32_t mine = any ? order_key(lane_max) : 0u;
+    if (WPR == 1) {
+        e[0] = mine;
+    } else {
+        keys[w * 64 + lane] = mine;
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < WPR; ++q) e[q] = keys[q * 64 + lane];
+    }
+    auto count = [&](uint32_t t) {
+        int c = 0;
+#pragma unroll
+        for (int q = 0; q < WPR; ++q) c += __popcll(__ballot(e[q] >= t));
+        return c;
+    };
+    if (count(1u) < k) return 0u;
+    uint32_t hi = e[0];
+#pragma unroll
+    for (int q = 1; q < WPR; ++q) hi = max(hi, e[q]);
+#pragma unroll
+    for (int off = 32; off; off >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, off));
+    hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)hi);
+    uint32_t lo = 1u;                                    // count(lo) >= k
+    for (int step = 0; step < 18 && lo < hi; ++step) {   // (near is enough: an eighth of an octave after 12 steps)
+        const uint32_t mid = lo + (hi - lo + 1) / 2;
+        const int c = count(mid);
+        if (c >= k) {
+            lo = mid;
+            if (c <= k + k / 8) break;
+        } else {
+            hi = mid - 1;
+        }
+    }
+    return lo;
+}
+
 // Block (row group, split).  WPR: waves per row.
 template <typename T, int WPR>
 __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restrict__ x, long long ld, long long n, long long v,
-                                                              int k, float c, int splits, long long split_len,
+                                                              int k, float c, float inv_t, int splits, long long split_len,
                                                               T* __restrict__ values, int* __restrict__ idx,
                                                               float* __restrict__ lse, u64* __restrict__ part,
                                                               float2* __restrict__ part_ms) {
@@ -280,6 +327,7 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
     __shared__ u64 lists[kWaves][WaveList<T>::kCap];
     __shared__ float2 ms[kWaves];
     __shared__ int counts[kWaves];
+    __shared__ uint32_t maxima[kThreads];
     const int wave = wave_id(), lane = threadIdx.x & 63;
     const int w = wave % WPR;
     const long long row = (long long)blockIdx.x * (kWaves / WPR) + wave / WPR;
@@ -310,6 +358,27 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
         u32x4 ahead[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) ahead[u] = fetch(at + u * step);
+        {
+            float top = -INFINITY;
+            bool any = false;
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                Vec16<T> v;
+                v.raw = ahead[u];
+                float f[N];
+                const float m = unpack<T>(v, f);
+                if (at + u * step + lane < nv) {
+                    top = any ? fmaxf(top, m) : m;
+                    any = true;
+                }
+            }
+            const uint32_t bound = bound_of_maxima<WPR>(top, any, k, maxima, w);
+            if (bound > order_key(-INFINITY)) {
+                // everything from the bound on: what exceeds the value below it (-0, just below +0, is no less)
+                list.tau = key_value(bound - (bound == order_key(0.f) ? 2u : 1u));
+                list.open = false;
+            }
+        }
         while (true) {
             float f[N], vm;
             int valid;              // elements of this lane
@@ -349,27 +418,48 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
         }
         acc.join_wave(c);
     }
-    // the k best of the wave, then of the row's waves
+    // the k best of the row's candidates: of all waves' at once, or, where there are many, of each wave's best
     u64 mine = 0;
     int found = 0;
-    {
+    if (WPR == 1) {
         list.shrink(0);
         found = list.cnt;
-        if (WPR == 1) mine = (lane < found) ? list.buf[lane] : 0ull;
-    }
-    if (WPR > 1) {
+        mine = (lane < found) ? list.buf[lane] : 0ull;
+    } else {
         if (lane == 0) {
             ms[wave] = make_float2(acc.m, acc.s);
-            counts[wave] = found;
+            counts[wave] = list.cnt;
         }
         __syncthreads();
-        if (wave != 0) return;
-        u64 e[kWaves];
+        int ends[kWaves], total = 0;
 #pragma unroll
-        for (int q = 0; q < kWaves; ++q) e[q] = (lane < counts[q]) ? lists[q][lane] : 0ull;
+        for (int q = 0; q < kWaves; ++q) ends[q] = total += counts[q];
+        const bool many = total > 64 * kGather;
+        if (many) {
+            list.shrink(0);
+            __syncthreads();
+            if (lane == 0) counts[wave] = list.cnt;
+            __syncthreads();
+        }
+        if (wave != 0) return;
+        u64 e[kGather];
+#pragma unroll
+        for (int r = 0; r < kGather; ++r) {
+            if (many) {
+                e[r] = (r < kWaves && lane < counts[r % kWaves]) ? lists[r % kWaves][lane] : 0ull;
+            } else {
+                const int at = r * 64 + lane;
+                int q = 0, from = 0;
+#pragma unroll
+                for (int o = 0; o + 1 < kWaves; ++o)
+                    if (at >= ends[o]) q = o + 1, from = ends[o];
+                e[r] = at < total ? lists[q][at - from] : 0ull;
+            }
+        }
+        wave_lds_fence();
         acc = join_pairs(ms, kWaves, c);
-        const u64 t = select_from<kWaves>(e, k, 0);
-        found = keep_entries<kWaves>(e, t, lists[0]);
+        const u64 t = select_from<kGather>(e, k, 0);
+        found = keep_entries<kGather>(e, t, lists[0]);
         wave_lds_fence();
         mine = (lane < found) ? lists[0][lane] : 0ull;
     }
@@ -380,14 +470,14 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
         return;
     }
     write_top<T>(mine, found, k, values + row * k, idx + row * k);
-    if (lane == 0) lse[row] = lse_value(acc);
+    if (lane == 0) lse[row] = lse_value(acc, inv_t);
 }
 
 // Joins the splits of a row: sixteen waves take up to 1024 entries each, the first joins their best.
 constexpr int kJoinWaves = 16;
 constexpr int kJoinR = 16;
 template <typename T>
-__global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k, float c, int splits, const u64* __restrict__ part,
+__global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k, float c, float inv_t, int splits, const u64* __restrict__ part,
                                                                           const float2* __restrict__ part_ms,
                                                                           T* __restrict__ values, int* __restrict__ idx,
                                                                           float* __restrict__ lse) {
@@ -412,15 +502,10 @@ __global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k,
         acc.init();
         for (int i = lane; i < splits; i += 64) {
             const float2 p = part_ms[row * splits + i];
-            if (p.x > acc.m) {
-                acc.s *= fast_exp2((acc.m - p.x) * c);
-                acc.m = p.x;
-                acc.mc = p.x * c;
-            }
-            if (p.x != -INFINITY) acc.s += p.y * fast_exp2(p.x * c - acc.mc);
+            acc.join(p.x, p.y, c);
         }
         acc.join_wave(c);
-        if (lane == 0) lse[row] = lse_value(acc);
+        if (lane == 0) lse[row] = lse_value(acc, inv_t);
     }
     if (wave != 0) return;
 #pragma unroll
@@ -434,16 +519,19 @@ __global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k,
 
 // ------------------------------------------------------------------ distillation
 
-// What a row's forward pass leaves for its backward pass, and for the loss.
-//   x = mc, y = log2 of the sum (softmax p = exp2(x c - mc - y)); z = the teacher's normaliser (base 2),
-//   w = tau: 0 for a row without a teacher (or without a class), NaN for a row with an index that is none
-__device__ __forceinline__ float teacher_weight(float a, float ca, float cn) { return fast_exp2(fmaf(a, ca, -cn)); }
+// What a row's forward pass leaves for its backward pass, and for the loss:
+//   x = the student's maximum m,  y = tau / s, so that tau p_j = y exp2((x_j - m) c): 0 for a row without a teacher (or
+//   without a class), NaN for a row with an index that is none;
+//   z, w: t_i = exp2((a_i - z) ca - w), the teacher's maximum and log of its sum, or its own normaliser and 0
+__device__ __forceinline__ float teacher_weight(float a, float ca, float ref, float log_sum) {
+    return fast_exp2(fmaf(a - ref, ca, -log_sum));
+}
 
 // One wave: the teacher's distribution of a row against the student's log-sum-exp.
 template <typename T>
 __device__ __forceinline__ void finish_row(const T* __restrict__ xr, long long v, float c, const LseAcc& acc,
                                            const int* __restrict__ idx, const float* __restrict__ top, int k,
-                                           const float* __restrict__ teacher_lse, float ca, long long row,
+                                           const float* __restrict__ teacher_lse, float ca, float teacher_t, long long row,
                                            float* __restrict__ loss, float4* __restrict__ stats) {
     const int lane = threadIdx.x & 63;
     const int* ir = idx + row * k;
@@ -461,28 +549,27 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ xr, long long v
     }
     top_max = wave_max(top_max);
     bad = __any(bad);
-    float cn;   // base 2
-    if (teacher_lse) {
-        cn = teacher_lse[row] * kLog2e;
-    } else {
-        const float mc = (top_max == -INFINITY) ? 0.f : top_max * ca;
-        float s = 0.f;
-        for (int i = lane; i < k; i += 64) {
-            const int j = ir[i];
-            if (j >= 0 && j < v) s += fast_exp2(fmaf(ar[i], ca, -mc));
+    const bool empty = top_max == -INFINITY || (acc.m == -INFINITY && acc.s == 0.f);
+    float ref = 0.f, log_sum = 0.f, tau = 0.f, part = 0.f;
+    if (!empty) {
+        if (teacher_lse) {
+            ref = teacher_lse[row] * teacher_t;
+        } else {
+            ref = top_max;
+            float s = 0.f;
+            for (int i = lane; i < k; i += 64) {
+                const int j = ir[i];
+                if (j >= 0 && j < v) s += fast_exp2((ar[i] - ref) * ca);
+            }
+            log_sum = log2f(wave_sum(s));
         }
-        cn = mc + log2f(wave_sum(s));
-    }
-    // sum t (log t - (x - max)) + tau log(sum): differences from the row's maximum, where little cancels
-    float tau = 0.f, part = 0.f;
-    if (top_max != -INFINITY && acc.m != -INFINITY) {
+        // sum t (log t - (x - max)) + tau log(sum): differences from the row's maximum, where little cancels
         for (int i = lane; i < k; i += 64) {
             const int j = ir[i];
             if (j >= 0 && j < v) {
-                const float t = teacher_weight(ar[i], ca, cn);
+                const float t = teacher_weight(ar[i], ca, ref, log_sum);
                 if (!(t <= 0.f)) {
-                    const float s = fmaf(to_f32(xr[j]), c, -acc.mc);
-                    part += t * (fmaf(ar[i], ca, -cn) - s);
+                    part += t * (fmaf(ar[i] - ref, ca, -log_sum) - (to_f32(xr[j]) - acc.r) * c);
                     tau += t;
                 }
             }
@@ -490,13 +577,12 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ xr, long long v
         tau = wave_sum(tau);
         part = wave_sum(part);
     }
-    const float l2s = log2f(acc.s);
     if (lane == 0) {
-        const bool empty = top_max == -INFINITY || acc.m == -INFINITY;
-        float value = empty ? 0.f : kLn2 * fmaf(tau, l2s, part);
-        if (bad || acc.s != acc.s) value = tau = NAN;
+        float value = empty ? 0.f : kLn2 * fmaf(tau, log2f(acc.s), part);
+        float share = empty ? 0.f : tau / acc.s;
+        if (bad || acc.s != acc.s) value = share = NAN;
         loss[row] = value;
-        stats[row] = make_float4(acc.mc, l2s, cn, tau);
+        stats[row] = make_float4(acc.r, share, ref, log_sum);
     }
 }
 
@@ -504,7 +590,7 @@ template <typename T, int WPR>
 __global__ __launch_bounds__(kThreads) void distill_forward_kernel(const T* __restrict__ x, long long ld, long long n,
                                                                    long long v, float c, int splits, long long split_len,
                                                                    const int* __restrict__ idx, const float* __restrict__ top,
-                                                                   int k, const float* __restrict__ teacher_lse, float ca,
+                                                                   int k, const float* __restrict__ teacher_lse, float ca, float teacher_t,
                                                                    float* __restrict__ loss, float4* __restrict__ stats,
                                                                    float2* __restrict__ part_ms) {
     constexpr int N = Vec16<T>::N;
@@ -549,29 +635,24 @@ __global__ __launch_bounds__(kThreads) void distill_forward_kernel(const T* __re
         if (lane == 0) part_ms[row * splits + split] = make_float2(acc.m, acc.s);
         return;
     }
-    finish_row<T>(xr, v, c, acc, idx, top, k, teacher_lse, ca, row, loss, stats);
+    finish_row<T>(xr, v, c, acc, idx, top, k, teacher_lse, ca, teacher_t, row, loss, stats);
 }
 
 template <typename T>
 __global__ __launch_bounds__(64) void distill_join_kernel(const T* __restrict__ x, long long ld, long long v, float c, int splits,
                                                           const float2* __restrict__ part_ms, const int* __restrict__ idx,
                                                           const float* __restrict__ top, int k,
-                                                          const float* __restrict__ teacher_lse, float ca,
+                                                          const float* __restrict__ teacher_lse, float ca, float teacher_t,
                                                           float* __restrict__ loss, float4* __restrict__ stats) {
     const long long row = blockIdx.x;
     LseAcc acc;
     acc.init();
     for (int i = threadIdx.x; i < splits; i += 64) {
         const float2 p = part_ms[row * splits + i];
-        if (p.x > acc.m) {
-            acc.s *= fast_exp2((acc.m - p.x) * c);
-            acc.m = p.x;
-            acc.mc = p.x * c;
-        }
-        if (p.x != -INFINITY) acc.s += p.y * fast_exp2(p.x * c - acc.mc);
+        acc.join(p.x, p.y, c);
     }
     acc.join_wave(c);
-    finish_row<T>(x + row * ld, v, c, acc, idx, top, k, teacher_lse, ca, row, loss, stats);
+    finish_row<T>(x + row * ld, v, c, acc, idx, top, k, teacher_lse, ca, teacher_t, row, loss, stats);
 }
 
 // Sum (mean: over the rows that have a teacher) of the rows' losses, in an order that depends on n alone.
@@ -585,7 +666,7 @@ __global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* _
     int count = 0;
     for (long long i = threadIdx.x; i < n; i += kSumThreads) {
         sum += (double)row_loss[i];
-        count += !(stats[i].w == 0.f);
+        count += !(stats[i].y == 0.f);
     }
     for (int off = 32; off; off >>= 1) {
         sum += __shfl_xor(sum, off);
@@ -639,9 +720,9 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(const T* __r
         if (scale) g *= scale[0];
         int* mine = listed + group * k;
         for (int i = w * 64 + lane; i < k; i += WPR * 64) mine[i] = idx[row * k + i];
-        const float f0 = st.w * g;
-        const bool empty = st.w == 0.f;
-        auto dense = [&](float xv) { return empty ? 0.f : f0 * fast_exp2(fmaf(xv, c, -st.x) - st.y); };
+        const float f0 = st.y * g;
+        const bool empty = st.y == 0.f;
+        auto dense = [&](float xv) { return empty ? 0.f : f0 * fast_exp2((xv - st.x) * c); };
         if (((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15) == 0) {
             stream_row<T>(
                 xr, lo, hi, w, WPR,
@@ -662,7 +743,7 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(const T* __r
         }
     }
     __syncthreads();
-    if (!live || st.w == 0.f) return;
+    if (!live || st.y == 0.f) return;
     const int* mine = listed + group * k;
     const float* ar = top + row * k;
     for (int i = w * 64 + lane; i < k; i += WPR * 64) {
@@ -674,9 +755,8 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(const T* __r
         if (!first) continue;
         float t = 0.f;
         for (int q = i; q < k; ++q)
-            if (mine[q] == j) t += teacher_weight(ar[q], ca, st.z);
-        const float p = fast_exp2(fmaf(to_f32(xr[j]), c, -st.x) - st.y);
-        dr[j] = from_f32<T>(g * fmaf(st.w, p, -t));
+            if (mine[q] == j) t += teacher_weight(ar[q], ca, st.z, st.w);
+        dr[j] = from_f32<T>(g * fmaf(st.y, fast_exp2((to_f32(xr[j]) - st.x) * c), -t));
     }
 }
 
@@ -714,13 +794,13 @@ hipError_t top_logits_t(const void* x, long long ld, long long n, long long v, i
     u64* part = static_cast<u64*>(ws);
     float2* part_ms = reinterpret_cast<float2*>(part + (size_t)n * splits * k);
     if (v <= kShortRow) {
-        top_logits_kernel<T, 1><<<dim3((unsigned)ceil_div(n, kWaves)), kThreads, 0, stream>>>(xt, ld, n, v, k, c, 1, v, vt, idx,
+        top_logits_kernel<T, 1><<<dim3((unsigned)ceil_div(n, kWaves)), kThreads, 0, stream>>>(xt, ld, n, v, k, c, 1.f / temperature, 1, v, vt, idx,
                                                                                                lse, nullptr, nullptr);
     } else {
-        top_logits_kernel<T, kWaves><<<dim3((unsigned)n, splits), kThreads, 0, stream>>>(xt, ld, n, v, k, c, splits, len, vt,
+        top_logits_kernel<T, kWaves><<<dim3((unsigned)n, splits), kThreads, 0, stream>>>(xt, ld, n, v, k, c, 1.f / temperature, splits, len, vt,
                                                                                         idx, lse, part, part_ms);
         if (splits > 1)
-            top_logits_join_kernel<T><<<dim3((unsigned)n), 64 * kJoinWaves, 0, stream>>>(k, c, splits, part, part_ms, vt, idx, lse);
+            top_logits_join_kernel<T><<<dim3((unsigned)n), 64 * kJoinWaves, 0, stream>>>(k, c, 1.f / temperature, splits, part, part_ms, vt, idx, lse);
     }
     return hipGetLastError();
 }
@@ -738,13 +818,13 @@ hipError_t distill_forward_t(const DistillArgs& a, int reduction, float* loss, f
     if (a.n > 0) {
         if (a.v <= kShortRow) {
             distill_forward_kernel<T, 1><<<dim3((unsigned)ceil_div(a.n, kWaves)), kThreads, 0, stream>>>(
-                x, a.ld, a.n, a.v, c, 1, a.v, a.idx, a.top, a.k, a.teacher_lse, ca, row_loss, stats, nullptr);
+                x, a.ld, a.n, a.v, c, 1, a.v, a.idx, a.top, a.k, a.teacher_lse, ca, a.teacher_temperature, row_loss, stats, nullptr);
         } else {
             distill_forward_kernel<T, kWaves><<<dim3((unsigned)a.n, splits), kThreads, 0, stream>>>(
-                x, a.ld, a.n, a.v, c, splits, len, a.idx, a.top, a.k, a.teacher_lse, ca, row_loss, stats, part_ms);
+                x, a.ld, a.n, a.v, c, splits, len, a.idx, a.top, a.k, a.teacher_lse, ca, a.teacher_temperature, row_loss, stats, part_ms);
             if (splits > 1)
                 distill_join_kernel<T><<<dim3((unsigned)a.n), 64, 0, stream>>>(x, a.ld, a.v, c, splits, part_ms, a.idx, a.top,
-                                                                              a.k, a.teacher_lse, ca, row_loss, stats);
+                                                                              a.k, a.teacher_lse, ca, a.teacher_temperature, row_loss, stats);
         }
     }
     if (reduction != 0)

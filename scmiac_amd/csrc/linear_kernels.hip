@@ -58,15 +58,60 @@ __device__ __forceinline__ float keep_z<float>(float z) {
     return z;
 }
 
-// One value of the forward product through the epilogue.
-template <typename T>
-__device__ __forceinline__ void forward_out(float z, long long i, long long j, long long n, int act, const T* __restrict__ bias,
-                                            const T* __restrict__ residual, long long ldr, T* __restrict__ y, T* __restrict__ zk) {
-    if (bias) z += to_f32(bias[j]);
-    if (zk) zk[i * n + j] = keep_z<T>(z);
-    float v = act_value(act, z);
-    if (residual) v += to_f32(residual[i * ldr + j]);
-    y[i * n + j] = from_f32<T>(v);
+// A few neighbouring values of one row of the forward product through the epilogue.
+template <int V>
+__device__ __forceinline__ void act_values(int act, float (&v)[V]) {
+    switch (act) {       // (the same for everybody: the loops stay small)
+        case kActRelu:
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = act_value(kActRelu, v[e]);
+            break;
+        case kActGelu:
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = act_value(kActGelu, v[e]);
+            break;
+        case kActSilu:
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[e] = act_value(kActSilu, v[e]);
+            break;
+        default: break;
+    }
+}
+template <typename T, int V>
+__device__ __forceinline__ void add_run(float (&v)[V], const T* __restrict__ p, int count) {
+    T in[V];
+    if (count >= V) {
+        __builtin_memcpy(in, p, sizeof(in));
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) in[e] = e < count ? p[e] : T(0);
+    }
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] += to_f32(in[e]);
+}
+template <typename T, int V, bool kKeep = false>
+__device__ __forceinline__ void store_run(const float (&v)[V], T* __restrict__ p, int count) {
+    T out[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) out[e] = kKeep ? keep_z<T>(v[e]) : from_f32<T>(v[e]);
+    if (count >= V) {
+        __builtin_memcpy(p, out, sizeof(out));
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+            if (e < count) p[e] = out[e];
+    }
+}
+// v: z without the bias, columns [j, j + count) of row i (count <= V)
+template <typename T, int V>
+__device__ __forceinline__ void forward_out(float (&v)[V], long long i, long long j, int count, long long n, int act,
+                                            const T* __restrict__ bias, const T* __restrict__ residual, long long ldr,
+                                            T* __restrict__ y, T* __restrict__ zk) {
+    if (bias) add_run<T, V>(v, bias + j, count);
+    if (zk) store_run<T, V, true>(v, zk + i * n + j, count);
+    act_values<V>(act, v);
+    if (residual) add_run<T, V>(v, residual + i * ldr + j, count);
+    store_run<T, V>(v, y + i * n + j, count);
 }
 
 // ------------------------------------------------------------------ 64 x 64 tiles, any shape
@@ -85,24 +130,63 @@ struct TileArgs {
     long long lda, ldb, ldr;
     long long rows, cols, depth;   // of C and of the contraction
     long long n;                   // row length of z, dy, y
-    int act, splits;
-    unsigned tiles_i;              // 64-row tiles of C
+    int act, splits, lanes;
+    unsigned tiles_i, tiles;       // 64-row tiles of C, and all
     long long split_len;
     void *out, *keep, *dbias;
     float *part, *part_bias;       // [splits][rows][cols], [splits][rows]
 };
 
+template <typename T>
+struct TileLds {
+    union {
+        struct {
+            __align__(16) T a[kTile * Lds<T>::LD];
+            __align__(16) T b[kTile * Lds<T>::LD];
+        };
+        __align__(16) float c[kTile * kTile];
+    };
+    float bias_sum[kThreads];
+};
+
+// C leaves through LDS: an accumulator holds one column of four rows a lane, memory wants runs of columns.  A 64 x 64 tile
+// of it lies row by row, every second group of four rows with its halves exchanged, so that the
+// two halves of a wave, four rows apart, write to different banks.
+__device__ __forceinline__ int place(int row, int col) { return row * 64 + (col ^ ((row & 4) << 3)); }
+__device__ __forceinline__ void put_quadrant(const f32x16& acc, float* c, int qi, int qj) {
+    const int lane = threadIdx.x & 63, half = lane >> 5;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) c[place(qi * 32 + 8 * (r >> 2) + 4 * half + (r & 3), qj * 32 + (lane & 31))] = acc[r];
+}
+// a 64 x 64 tile from LDS through the epilogue, eight columns at a time, by `threads` threads
 template <typename T, int OP>
-__global__ __launch_bounds__(kThreads) void linear_tile_kernel(TileArgs p) {
+__device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long long i0, long long j0, int t, int threads) {
+    for (int e = t; e < kTile * 8; e += threads) {
+        const int row = e >> 3, col = (e & 7) * 8;
+        const long long i = i0 + row, j = j0 + col;
+        if (i >= p.rows || j >= p.cols) continue;
+        const int count = (int)min(8ll, p.cols - j);
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(c + place(row, col)), hi = *reinterpret_cast<const f32x4*>(c + place(row, col + 4));
+        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        if (OP == kForward)
+            forward_out<T, 8>(v, i, j, count, p.n, p.act, static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), p.ldr,
+                              static_cast<T*>(p.out), static_cast<T*>(p.keep));
+        else
+            store_run<T, 8>(v, static_cast<T*>(p.out) + i * p.cols + j, count);
+    }
+}
+
+// piece `piece` of the work on one product: a tile of C, and within it a split of the contraction
+template <typename T, int OP>
+__device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, TileLds<T>& lds) {
     constexpr int LD = Lds<T>::LD;
     constexpr int NV = kTile * kDepth / kThreads;   // elements of a tile per thread
-    __shared__ __align__(16) T as[kTile * LD];
-    __shared__ __align__(16) T bs[kTile * LD];
-    __shared__ float bias_sum[kThreads];
+    T *as = lds.a, *bs = lds.b;
+    float* bias_sum = lds.bias_sum;
     const int t = threadIdx.x, lane = t & 63, wave = wave_id();
-    const unsigned tile_j = blockIdx.x / p.tiles_i;
-    const long long i0 = (long long)(blockIdx.x - tile_j * p.tiles_i) * kTile, j0 = (long long)tile_j * kTile;
-    const long long c_lo = (long long)blockIdx.y * p.split_len;
+    const unsigned split = piece / p.tiles, tile = piece - split * p.tiles, tile_j = tile / p.tiles_i;
+    const long long i0 = (long long)(tile - tile_j * p.tiles_i) * kTile, j0 = (long long)tile_j * kTile;
+    const long long c_lo = (long long)split * p.split_len;
     const long long c_hi = min(p.depth, c_lo + p.split_len);
     const T* __restrict__ a = static_cast<const T*>(p.a);
     const T* __restrict__ b = static_cast<const T*>(p.b);
@@ -140,7 +224,7 @@ __global__ __launch_bounds__(kThreads) void linear_tile_kernel(TileArgs p) {
         for (int q = 0; q < NV; ++q) {
             const long long r = j0 + rb + q * kStepRB, c = c0 + cb + q * kStepCB;
             T v = T(0);
-            if (r < p.cols && c < c_hi) v = kAlongB ? b[r * p.ldb + c] : b[c * p.ldb + r];
+            if (b && r < p.cols && c < c_hi) v = kAlongB ? b[r * p.ldb + c] : b[c * p.ldb + r];
             vb[q] = v;
         }
     };
@@ -183,18 +267,17 @@ __global__ __launch_bounds__(kThreads) void linear_tile_kernel(TileArgs p) {
         }
     }
 
-    const long long j = j0 + wc;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const long long i = i0 + (wave & 1) * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
-        if (i >= p.rows || j >= p.cols) continue;
-        if (p.splits > 1)
-            p.part[((long long)blockIdx.y * p.rows + i) * p.cols + j] = acc[r];
-        else if (OP == kForward)
-            forward_out<T>(acc[r], i, j, p.n, p.act, static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), p.ldr,
-                           static_cast<T*>(p.out), static_cast<T*>(p.keep));
-        else if (p.out)
-            static_cast<T*>(p.out)[i * p.cols + j] = from_f32<T>(acc[r]);
+    __syncthreads();     // the operands' tiles are read: C's 64 x 64 values take their place
+    float* c = lds.c;
+    put_quadrant(acc, c, wave & 1, wave >> 1);
+    __syncthreads();
+    if (p.splits > 1) {
+        for (int e = t; e < kTile * kTile; e += kThreads) {
+            const long long i = i0 + (e >> 6), j = j0 + (e & 63);
+            if (i < p.rows && j < p.cols) p.part[((long long)split * p.rows + i) * p.cols + j] = c[place(e >> 6, e & 63)];
+        }
+    } else if (p.out) {
+        tile_out<T, OP>(p, c, i0, j0, t, kThreads);
     }
     if (OP == kDw && p.dbias && tile_j == 0) {   // rows of C are the outputs: their sums of dz, four partial sums each
         bias_sum[t] = dsum;
@@ -202,23 +285,39 @@ __global__ __launch_bounds__(kThreads) void linear_tile_kernel(TileArgs p) {
         if (t < kTile && i0 + t < p.rows) {
             const float s = (bias_sum[t] + bias_sum[t + 64]) + (bias_sum[t + 128] + bias_sum[t + 192]);
             if (p.splits > 1)
-                p.part_bias[(long long)blockIdx.y * p.rows + i0 + t] = s;
+                p.part_bias[(long long)split * p.rows + i0 + t] = s;
             else
                 static_cast<T*>(p.dbias)[i0 + t] = from_f32<T>(s);
         }
     }
 }
 
+template <typename T>
+__global__ __launch_bounds__(kThreads) void linear_tile_forward_kernel(TileArgs p) {
+    __shared__ TileLds<T> lds;
+    tile_product<T, kForward>(p, blockIdx.x, lds);
+}
+// both products of the backward pass in one launch, the first pieces_dx blocks on dx
+template <typename T>
+__global__ __launch_bounds__(kThreads) void linear_tile_backward_kernel(TileArgs dx, unsigned pieces_dx, TileArgs dw) {
+    __shared__ TileLds<T> lds;
+    if (blockIdx.x < pieces_dx)
+        tile_product<T, kDx>(dx, blockIdx.x, lds);
+    else
+        tile_product<T, kDw>(dw, blockIdx.x - pieces_dx, lds);
+}
+
 // Joins the splits of the contraction, in their order.
 template <typename T, int OP>
-__global__ __launch_bounds__(kThreads) void linear_join_kernel(TileArgs p) {
+__device__ __forceinline__ void join_splits(const TileArgs& p) {
     const long long total = p.rows * p.cols;
     for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < total; e += (long long)gridDim.x * kThreads) {
         float s = 0.f;
         for (int q = 0; q < p.splits; ++q) s += p.part[q * total + e];
+        float v[1] = {s};
         if (OP == kForward)
-            forward_out<T>(s, e / p.cols, e % p.cols, p.n, p.act, static_cast<const T*>(p.bias),
-                           static_cast<const T*>(p.residual), p.ldr, static_cast<T*>(p.out), static_cast<T*>(p.keep));
+            forward_out<T, 1>(v, e / p.cols, e % p.cols, 1, p.n, p.act, static_cast<const T*>(p.bias),
+                              static_cast<const T*>(p.residual), p.ldr, static_cast<T*>(p.out), static_cast<T*>(p.keep));
         else if (p.out)
             static_cast<T*>(p.out)[e] = from_f32<T>(s);
     }
@@ -228,6 +327,19 @@ __global__ __launch_bounds__(kThreads) void linear_join_kernel(TileArgs p) {
             for (int q = 0; q < p.splits; ++q) s += p.part_bias[(long long)q * p.rows + e];
             static_cast<T*>(p.dbias)[e] = from_f32<T>(s);
         }
+}
+template <typename T, int OP>
+__global__ __launch_bounds__(kThreads) void linear_join_kernel(TileArgs p) {
+    join_splits<T, OP>(p);
+}
+template <typename T>
+__global__ __launch_bounds__(kThreads) void linear_join_backward_kernel(TileArgs dx, TileArgs dw) {
+    if (dx.splits > 1) join_splits<T, kDx>(dx);
+    if (dw.splits > 1) join_splits<T, kDw>(dw);
+}
+inline unsigned join_blocks(long long elements) {
+    const long long blocks = ceil_div(elements, kThreads);
+    return (unsigned)(blocks < 4096 ? blocks : 4096);
 }
 
 // Pieces of the contraction: enough blocks to give every compute unit two, none of them shorter than 256.
@@ -248,19 +360,645 @@ size_t tile_bytes(long long rows, long long cols, long long depth) {
     return splits > 1 ? sizeof(float) * (size_t)splits * ((size_t)rows * cols + rows) : 0;
 }
 
-template <typename T, int OP>
-hipError_t run_tiles(TileArgs p, void* ws, hipStream_t stream) {
+// fills in the splits of a product whose partial sums start at ws; returns its number of pieces
+unsigned set_tiles(TileArgs& p, void* ws) {
     plan_tiles(p.rows, p.cols, p.depth, p.splits, p.split_len);
     p.part = static_cast<float*>(ws);
     p.part_bias = p.part + (size_t)p.splits * p.rows * p.cols;
     p.tiles_i = (unsigned)ceil_div(p.rows, kTile);
-    const dim3 grid((unsigned)(p.tiles_i * ceil_div(p.cols, kTile)), p.splits);
-    linear_tile_kernel<T, OP><<<grid, kThreads, 0, stream>>>(p);
+    p.tiles = (unsigned)(p.tiles_i * ceil_div(p.cols, kTile));
+    return p.tiles * (unsigned)p.splits;
+}
+
+// ------------------------------------------------------------------ up to eight rows
+//
+// With a handful of rows the layer is one reading of w: every lane streams 16-byte pieces of w's rows
+// past the few rows of x (forward), or of dz (dx), in float32 FMAs.
+
+constexpr int kFewRows = 8;
+constexpr int kFewCols = 4;      // rows of w a wave has in hand at a time: each piece of x serves four of w
+
+// y: p.lanes lanes (8 to 64, a power of two, by the length of a row) share kFewCols rows of w.
+template <typename T, int M>
+__global__ __launch_bounds__(kThreads) void linear_few_rows_kernel(TileArgs p) {
+    constexpr int V = Vec16<T>::N;
+    const int lane = threadIdx.x & (p.lanes - 1);
+    const long long j0 = ((long long)blockIdx.x * (kThreads / p.lanes) + threadIdx.x / p.lanes) * kFewCols;
+    const T* __restrict__ x = static_cast<const T*>(p.a);
+    const T* __restrict__ w = static_cast<const T*>(p.b);
+    const T *xr[M], *wr[kFewCols];
+#pragma unroll
+    for (int i = 0; i < M; ++i) xr[i] = x + min((long long)i, p.rows - 1) * p.lda;
+#pragma unroll
+    for (int j = 0; j < kFewCols; ++j) wr[j] = w + min(j0 + j, p.cols - 1) * p.ldb;
+    float acc[M][kFewCols] = {};
+    const long long pieces = p.depth / V;
+#pragma unroll 2
+    for (long long c = lane; c < pieces; c += p.lanes) {
+        float fw[kFewCols][V];
+        Vec16<T> vw[kFewCols], vx[M];
+#pragma unroll
+        for (int j = 0; j < kFewCols; ++j) vw[j] = load_vec(wr[j] + c * V);
+#pragma unroll
+        for (int i = 0; i < M; ++i) vx[i] = load_vec(xr[i] + c * V);
+#pragma unroll
+        for (int j = 0; j < kFewCols; ++j)
+#pragma unroll
+            for (int e = 0; e < V; ++e) fw[j][e] = vw[j].get(e);
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float f = vx[i].get(e);
+#pragma unroll
+                for (int j = 0; j < kFewCols; ++j) acc[i][j] = fmaf(f, fw[j][e], acc[i][j]);
+            }
+    }
+    const long long c = pieces * V + lane;      // fewer than V left
+    if (c < p.depth)
+#pragma unroll
+        for (int i = 0; i < M; ++i)
+#pragma unroll
+            for (int j = 0; j < kFewCols; ++j) acc[i][j] = fmaf(to_f32(xr[i][c]), to_f32(wr[j][c]), acc[i][j]);
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int j = 0; j < kFewCols; ++j) {
+            float z = acc[i][j];
+            for (int off = p.lanes >> 1; off; off >>= 1) z += __shfl_xor(z, off);
+            acc[i][j] = z;
+        }
+    if (lane >= M || lane >= p.rows || j0 >= p.cols) return;     // a lane for each row: all its values at once
+    float v[kFewCols];
+#pragma unroll
+    for (int i = 0; i < M; ++i)
+#pragma unroll
+        for (int j = 0; j < kFewCols; ++j) v[j] = (i == 0 || lane == i) ? acc[i][j] : v[j];
+    forward_out<T, kFewCols>(v, lane, j0, (int)min((long long)kFewCols, p.cols - j0), p.n, p.act, static_cast<const T*>(p.bias),
+                             static_cast<const T*>(p.residual), p.ldr, static_cast<T*>(p.out), static_cast<T*>(p.keep));
+}
+
+// dx: a block takes one piece of columns per lane (512 columns in the half types) and `split_len` rows of w, its
+// waves every fourth of them; dz of those rows is worked out once, into LDS.
+constexpr int kFewDepth = 256;   // longest split
+template <typename T, int M>
+__global__ __launch_bounds__(kThreads) void linear_few_rows_dx_kernel(TileArgs p) {
+    constexpr int V = Vec16<T>::N;
+    __shared__ float dz[M][kFewDepth];
+    __shared__ float meet[kThreads / 64][64 * V];
+    const int t = threadIdx.x, lane = t & 63, wave = wave_id();
+    const long long c0 = ((long long)blockIdx.x * 64 + lane) * V;
+    const long long lo = (long long)blockIdx.y * p.split_len;
+    const int len = (int)(min(p.depth, lo + p.split_len) - lo);
+    const T* __restrict__ w = static_cast<const T*>(p.b);
+    const T* __restrict__ dy = static_cast<const T*>(p.dy);
+    const T* __restrict__ z = static_cast<const T*>(p.z);
+    for (int e = t; e < M * len; e += kThreads) {
+        const int i = e / len, r = e - i * len;
+        float g = 0.f;
+        if (i < p.rows) {
+            const long long at = i * p.n + lo + r;
+            g = to_f32(dy[at]);
+            if (p.act != kActNone) g *= act_slope(p.act, to_f32(z[at]));
+        }
+        dz[i][r] = g;
+    }
+    __syncthreads();
+    float acc[M][V] = {};
+    const bool whole = c0 + V <= p.cols;
+    const int rest = (int)max(0ll, min((long long)V, p.cols - c0));
+#pragma unroll 4
+    for (int r = wave; r < len; r += kThreads / 64) {
+        const T* row = w + (lo + r) * p.ldb + c0;
+        float f[V];
+        if (whole) {
+            const Vec16<T> v = load_vec(row);
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = v.get(e);
+        } else {
+#pragma unroll
+            for (int e = 0; e < V; ++e) f[e] = e < rest ? to_f32(row[e]) : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            const float g = dz[i][r];
+#pragma unroll
+            for (int e = 0; e < V; ++e) acc[i][e] = fmaf(g, f[e], acc[i][e]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        __syncthreads();
+#pragma unroll
+        for (int e = 0; e < V; ++e) meet[wave][lane * V + e] = acc[i][e];
+        __syncthreads();
+        if (i >= p.rows) continue;
+        for (int e = t; e < 64 * V; e += kThreads) {
+            const long long c = (long long)blockIdx.x * 64 * V + e;
+            if (c >= p.cols) continue;
+            const float s = (meet[0][e] + meet[1][e]) + (meet[2][e] + meet[3][e]);
+            if (p.splits > 1)
+                p.part[((long long)blockIdx.y * p.rows + i) * p.cols + c] = s;
+            else
+                static_cast<T*>(p.out)[i * p.cols + c] = from_f32<T>(s);
+        }
+    }
+}
+
+constexpr long long kMaxFewCols = 1 << 22;   // splits of dx fit a grid's second dimension
+// From 2^18 weights on; below that a launch of 64 x 64 tiles is as short.
+bool has_few_rows(long long m, long long n, long long k) { return m >= 1 && m <= kFewRows && n <= kMaxFewCols && n * k >= (1 << 18); }
+
+void plan_few_dx(long long n, long long k, int esize, int& splits, long long& len) {
+    const long long groups = ceil_div(k, 64 * (16 / esize));
+    long long s = ceil_div(1024, groups);                 // four blocks for every compute unit
+    if (s > n / 32) s = n / 32;                           // none shorter than eight rows a wave
+    if (s < 1) s = 1;
+    len = ceil_div(n, s);
+    if (len > kFewDepth) len = kFewDepth;
+    splits = (int)ceil_div(n, len);
+}
+size_t few_dx_bytes(long long m, long long n, long long k, int esize) {
+    int splits;
+    long long len;
+    plan_few_dx(n, k, esize, splits, len);
+    return splits > 1 ? sizeof(float) * (size_t)splits * m * k : 0;
+}
+
+template <typename T>
+hipError_t run_few_rows(TileArgs p, hipStream_t stream) {
+    p.lanes = 8;
+    while (p.lanes < 64 && p.lanes * Vec16<T>::N < p.depth) p.lanes *= 2;
+    const dim3 grid((unsigned)ceil_div(p.cols, kFewCols * (kThreads / p.lanes)));
+    if (p.rows == 1) linear_few_rows_kernel<T, 1><<<grid, kThreads, 0, stream>>>(p);
+    else if (p.rows == 2) linear_few_rows_kernel<T, 2><<<grid, kThreads, 0, stream>>>(p);
+    else if (p.rows <= 4) linear_few_rows_kernel<T, 4><<<grid, kThreads, 0, stream>>>(p);
+    else linear_few_rows_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
+    plan_few_dx(p.depth, p.cols, sizeof(T), p.splits, p.split_len);
+    p.part = static_cast<float*>(ws);
+    const dim3 grid((unsigned)ceil_div(p.cols, 64 * Vec16<T>::N), (unsigned)p.splits);
+    if (p.rows == 1) linear_few_rows_dx_kernel<T, 1><<<grid, kThreads, 0, stream>>>(p);
+    else if (p.rows == 2) linear_few_rows_dx_kernel<T, 2><<<grid, kThreads, 0, stream>>>(p);
+    else if (p.rows <= 4) linear_few_rows_dx_kernel<T, 4><<<grid, kThreads, 0, stream>>>(p);
+    else linear_few_rows_dx_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
     if (p.splits > 1) {
-        const long long blocks = ceil_div(p.rows * p.cols, kThreads);
-        linear_join_kernel<T, OP><<<dim3((unsigned)(blocks < 4096 ? blocks : 4096)), kThreads, 0, stream>>>(p);
+        linear_join_kernel<T, kDx><<<dim3(join_blocks(p.rows * p.cols)), kThreads, 0, stream>>>(p);
     }
     return hipGetLastError();
+}
+
+// ------------------------------------------------------------------ large products
+//
+// C[i, j] = sum_c A[i, c] B[j, c] on 16-bit operands whose rows are padded to whole 128-byte lines (64 elements).  A block
+// owns a BM x BN tile; its operands pass through LDS in steps of 64 along the contraction, two buffers deep,
+// written by the memory pipe itself (16 bytes a lane, no registers).  Such a write lands lane after lane, eight
+// 16-byte chunks a row, and reading one chunk column of 32 rows would hit the same banks every time;
+// so lane l fetches chunk (l % 8) ^ (row % 8) of its row, and the reads look it up there.
+//
+// float32 operands come as three bf16 planes whose sum is the value to 2^-25 or better: the product is
+// the six products of planes that matter (the other three are below 2^-24 of the result), run as one
+// contraction six times as long.  Six passes at the bf16 rate are 2.6 times as fast as float32 MFMA.
+
+constexpr int kBK = 64;
+constexpr long long kMaxLd = 1 << 22;    // a tile's 256 rows are addressed by 32-bit byte offsets
+constexpr int kPlanes = 3, kPairs = 6;
+
+struct GemmArgs {
+    const void *a, *b;
+    long long lda, ldb;              // elements
+    long long plane_a, plane_b;      // elements between planes
+    long long rows, cols;
+    int k_blocks;                    // 64-wide steps of one plane pair
+    int pairs;                       // 1, or kPairs
+    int splits, split_len;           // in steps
+    unsigned tiles_i, tiles_j;
+    TileArgs t;                      // the epilogue's part
+};
+
+template <typename T16>
+struct Frag;
+template <>
+struct Frag<bf16> {
+    typedef bf16x8 type;
+    static __device__ __forceinline__ f32x16 mfma(type a, type b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Frag<f16> {
+    typedef f16x8 type;
+    static __device__ __forceinline__ f32x16 mfma(type a, type b, f32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+    }
+};
+
+// 64 lanes x 16 bytes from global memory to LDS at `lds` + 16 lane
+__device__ __forceinline__ void load_to_lds(const void* g, char* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
+                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+
+template <typename T16, typename OutT, int BM, int BN, int WM, int WN, int OP>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel(GemmArgs p) {
+    constexpr int kWavesN = BN / WN, kWavesAll = (BM / WM) * kWavesN;
+    constexpr int FA = WM / 32, FB = WN / 32;
+    constexpr int kLoadsA = BM / 8 / kWavesAll, kLoadsB = BN / 8 / kWavesAll;
+    constexpr int kBytesA = BM * kBK * 2, kBytes = (BM + BN) * kBK * 2;
+    __shared__ __align__(128) char lds[2 * kBytes];
+    typedef typename Frag<T16>::type frag;
+    const int lane = threadIdx.x & 63, wave = wave_id();
+    const int wm = (wave / kWavesN) * WM, wn = (wave % kWavesN) * WN;
+
+    // Blocks go to the eight XCDs in turn: give each XCD a run of tiles of its own, and within it walk
+    // eight rows of tiles at a time, so that the tiles at work share their operands in that XCD's L2.
+    const unsigned tiles = p.tiles_i * p.tiles_j;
+    const unsigned xcd = blockIdx.x & 7, per = tiles / 8, extra = tiles % 8;
+    unsigned id = xcd * per + min(xcd, extra) + (blockIdx.x >> 3);
+    const unsigned group = 8 * p.tiles_j, first = id / group * 8;
+    const unsigned high = min(8u, p.tiles_i - first);
+    id %= group;
+    const unsigned ti = first + id % high, tj = id / high;
+    const long long i0 = (long long)ti * BM, j0 = (long long)tj * BN;
+    const int s_lo = blockIdx.y * p.split_len, s_hi = min(p.k_blocks * p.pairs, s_lo + p.split_len);
+
+    // byte offsets of this lane's pieces within the tile's rows (rows behind the last one repeat it: what
+    // they give is not written)
+    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    const char* base_a = reinterpret_cast<const char*>(p.a) + i0 * p.lda * 2;
+    const char* base_b = reinterpret_cast<const char*>(p.b) + j0 * p.ldb * 2;
+    unsigned off_a[kLoadsA], off_b[kLoadsB];
+    const int rows_left = (int)min((long long)BM, p.rows - i0), cols_left = (int)min((long long)BN, p.cols - j0);
+#pragma unroll
+    for (int q = 0; q < kLoadsA; ++q)
+        off_a[q] = (unsigned)min((q * kWavesAll + wave) * 8 + (lane >> 3), rows_left - 1) * (unsigned)(p.lda * 2) + chunk;
+#pragma unroll
+    for (int q = 0; q < kLoadsB; ++q)
+        off_b[q] = (unsigned)min((q * kWavesAll + wave) * 8 + (lane >> 3), cols_left - 1) * (unsigned)(p.ldb * 2) + chunk;
+
+    auto stage = [&](int step, int buf) {
+        long long oa = 0, ob = 0;
+        int kb = step;
+        if (p.pairs > 1) {
+            const int pair = step / p.k_blocks;
+            kb -= pair * p.k_blocks;
+            // the small products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
+            const int pa = (pair == 0) ? 2 : (pair == 2 || pair == 3) ? 1 : 0;
+            const int pb = (pair == 1) ? 2 : (pair == 2 || pair == 4) ? 1 : 0;
+            oa = pa * p.plane_a * 2;
+            ob = pb * p.plane_b * 2;
+        }
+        const char* ga = base_a + oa + (long long)kb * (kBK * 2);
+        const char* gb = base_b + ob + (long long)kb * (kBK * 2);
+        char* to = lds + buf * kBytes + wave * 1024;
+#pragma unroll
+        for (int q = 0; q < kLoadsA; ++q) load_to_lds(ga + off_a[q], to + q * kWavesAll * 1024);
+#pragma unroll
+        for (int q = 0; q < kLoadsB; ++q) load_to_lds(gb + off_b[q], to + kBytesA + q * kWavesAll * 1024);
+    };
+
+    f32x16 acc[FA][FB] = {};
+    const int half = lane >> 5, l31 = lane & 31;
+    const int row_a = (wm + l31) * 128, row_b = kBytesA + (wn + l31) * 128;
+    int buf = 0;
+    stage(s_lo, 0);
+    for (int step = s_lo; step < s_hi; ++step) {
+        __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this step's tiles have landed (this wave's share)
+        __syncthreads();                         // everybody's have, and nobody reads the other buffer any more
+        if (step + 1 < s_hi) stage(step + 1, buf ^ 1);
+        const char* from = lds + buf * kBytes;
+#pragma unroll
+        for (int kk = 0; kk < kBK / 16; ++kk) {
+            const int at = ((2 * kk + half) ^ (lane & 7)) * 16;
+            frag fa[FA], fb[FB];
+#pragma unroll
+            for (int f = 0; f < FA; ++f) fa[f] = *reinterpret_cast<const frag*>(from + row_a + at + f * 4096);
+#pragma unroll
+            for (int f = 0; f < FB; ++f) fb[f] = *reinterpret_cast<const frag*>(from + row_b + at + f * 4096);
+#pragma unroll
+            for (int f = 0; f < FA; ++f)
+#pragma unroll
+                for (int g = 0; g < FB; ++g) acc[f][g] = Frag<T16>::mfma(fa[f], fb[g], acc[f][g]);
+        }
+        buf ^= 1;
+    }
+
+    if (p.splits > 1) {
+#pragma unroll
+        for (int f = 0; f < FA; ++f)
+#pragma unroll
+            for (int g = 0; g < FB; ++g) {
+                const long long j = j0 + wn + g * 32 + l31;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const long long i = i0 + wm + f * 32 + 8 * (r >> 2) + 4 * half + (r & 3);
+                    if (i < p.rows && j < p.cols) p.t.part[((long long)blockIdx.y * p.rows + i) * p.cols + j] = acc[f][g][r];
+                }
+            }
+        return;
+    }
+    static_assert(WN == 64 && WM % 64 == 0 && kWavesAll * kTile * kTile * 4 <= 2 * kBytes, "a 64 x 64 tile of LDS for every wave");
+    __syncthreads();                             // the operands are read: the room is each wave's own now
+    float* c = reinterpret_cast<float*>(lds) + wave * (kTile * kTile);
+#pragma unroll
+    for (int m = 0; m < WM / 64; ++m) {
+        wave_lds_fence();
+#pragma unroll
+        for (int q = 0; q < 4; ++q) put_quadrant(acc[2 * m + (q >> 1)][q & 1], c, q >> 1, q & 1);
+        wave_lds_fence();
+        tile_out<OutT, OP>(p.t, c, i0 + wm + m * 64, j0 + wn, lane, 64);
+    }
+}
+
+// An operand of the large products from a matrix src [rows, cols] (or from dz = dy act'(z), given as src = dy and z):
+// as it stands, its rows padded with zeros to pc elements, and / or turned, its rows then padded to pr;
+// float32 as three bf16 planes.  `sums` [ceil(rows / 64)][cols]: what each 64 rows add up to, before any rounding.
+struct PackArgs {
+    const void *src, *z;
+    long long ld, rows, cols, pr, pc;
+    int act;
+    void *out, *turned;
+    float* sums;
+};
+template <typename T>
+struct Plane {
+    typedef T type;
+    static constexpr int N = 1;
+};
+template <>
+struct Plane<float> {
+    typedef bf16 type;
+    static constexpr int N = kPlanes;
+};
+template <typename T>
+__device__ __forceinline__ void split_planes(float v, typename Plane<T>::type (&o)[Plane<T>::N]) {
+    if constexpr (sizeof(T) == 4) {
+        // each plane is what the ones before leave; a value that rounds up to infinity, or is not finite,
+        // is cut short instead, or stands in the first plane alone
+        bf16 h = static_cast<bf16>(v);
+        if (!(fabsf(static_cast<float>(h)) < INFINITY) && fabsf(v) < INFINITY)
+            h = __builtin_bit_cast(bf16, (uint16_t)(__float_as_uint(v) >> 16));
+        const bool finite = fabsf(v) < INFINITY;
+        const float r1 = finite ? v - static_cast<float>(h) : 0.f;
+        const bf16 m = static_cast<bf16>(r1);
+        o[0] = h;
+        o[1] = m;
+        o[2] = static_cast<bf16>(r1 - static_cast<float>(m));
+    } else {
+        o[0] = from_f32<T>(v);
+    }
+}
+template <typename T, bool kSlope>
+__global__ __launch_bounds__(kThreads) void linear_pack_kernel(PackArgs p) {
+    typedef typename Plane<T>::type P;
+    constexpr int NP = Plane<T>::N;
+    typedef P Four __attribute__((ext_vector_type(4)));
+    __shared__ float tile[64][65];
+    __shared__ float part[4][64];
+    const int t = threadIdx.x, q = (t & 15) * 4, r0 = t >> 4;
+    const unsigned tiles_c = (unsigned)(p.pc / 64), tile_r = blockIdx.x / tiles_c;
+    const long long c0 = (long long)(blockIdx.x - tile_r * tiles_c) * 64, y0 = (long long)tile_r * 64;
+    const T* __restrict__ src = static_cast<const T*>(p.src);
+    const T* __restrict__ z = static_cast<const T*>(p.z);
+    P* out = static_cast<P*>(p.out);
+    P* turned = static_cast<P*>(p.turned);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const long long r = y0 + r0 + 16 * i;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (r < p.rows && c0 + q + 4 <= p.cols) {
+            T in[4], zi[4];
+            __builtin_memcpy(in, src + r * p.ld + c0 + q, sizeof(in));
+            if (kSlope) __builtin_memcpy(zi, z + r * p.ld + c0 + q, sizeof(zi));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = kSlope ? to_f32(in[e]) * act_slope(p.act, to_f32(zi[e])) : to_f32(in[e]);
+        } else if (r < p.rows) {
+            for (int e = 0; e < 4; ++e) {
+                const long long c = c0 + q + e;
+                if (c < p.cols) v[e] = to_f32(src[r * p.ld + c]) * (kSlope ? act_slope(p.act, to_f32(z[r * p.ld + c])) : 1.f);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) tile[r0 + 16 * i][q + e] = v[e];
+        if (out && r < p.rows) {
+            Four w[NP];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                P o[NP];
+                split_planes<T>(v[e], o);
+#pragma unroll
+                for (int s = 0; s < NP; ++s) w[s][e] = o[s];
+            }
+#pragma unroll
+            for (int s = 0; s < NP; ++s) *reinterpret_cast<Four*>(out + (s * p.rows + r) * p.pc + c0 + q) = w[s];
+        }
+    }
+    __syncthreads();
+    if (turned) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const long long c = c0 + r0 + 16 * i;
+            if (c >= p.cols) continue;
+            Four w[NP];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                P o[NP];
+                split_planes<T>(tile[q + e][r0 + 16 * i], o);
+#pragma unroll
+                for (int s = 0; s < NP; ++s) w[s][e] = o[s];
+            }
+#pragma unroll
+            for (int s = 0; s < NP; ++s) *reinterpret_cast<Four*>(turned + (s * p.cols + c) * p.pr + y0 + q) = w[s];
+        }
+    }
+    if (p.sums) {
+        float s = 0.f;
+        for (int r = (t >> 6) * 16; r < (t >> 6) * 16 + 16; ++r) s += tile[r][t & 63];
+        part[t >> 6][t & 63] = s;
+        __syncthreads();
+        if (t < 64 && c0 + t < p.cols && y0 < p.rows)
+            p.sums[(long long)tile_r * p.cols + c0 + t] = (part[0][t] + part[1][t]) + (part[2][t] + part[3][t]);
+    }
+}
+
+// dbias from the sums of the pack: 64 columns a block, four runs of partial sums each, joined in order
+template <typename T>
+__global__ __launch_bounds__(kThreads) void linear_bias_kernel(const float* __restrict__ sums, long long parts, long long cols,
+                                                               T* __restrict__ dbias) {
+    __shared__ float run[4][64];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const long long c = (long long)blockIdx.x * 64 + lane;
+    const long long len = (parts + 3) / 4, lo = w * len, hi = min(parts, lo + len);
+    float s = 0.f;
+    if (c < cols) {
+#pragma unroll 8
+        for (long long i = lo; i < hi; ++i) s += sums[i * cols + c];
+    }
+    run[w][lane] = s;
+    __syncthreads();
+    if (w == 0 && c < cols) dbias[c] = from_f32<T>((run[0][lane] + run[1][lane]) + (run[2][lane] + run[3][lane]));
+}
+
+// Whether a layer goes through the large tiles: from 2^27 multiply-adds on, of at least 64 inputs and outputs; below,
+// packing the operands and filling a few tiles cost more than the 64 x 64 tiles' slower inner loop.
+bool is_large(long long rows, long long cols, long long depth) {
+    if (rows <= kFewRows || cols < 64 || depth < 64) return false;
+    if (rows > kMaxLd || cols > kMaxLd || depth > kMaxLd) return false;
+    return (double)rows * (double)cols * (double)depth >= 134217728.0;
+}
+
+struct GemmPlan {
+    bool wide;               // 256 x 256 tiles (8 waves), or 128 x 128 (4 waves)
+    unsigned tiles_i, tiles_j;
+    int steps, splits, split_len;
+    size_t part_bytes;
+};
+GemmPlan plan_gemm(long long rows, long long cols, long long depth_padded, int pairs) {
+    GemmPlan g;
+    const long long t256 = ceil_div(rows, 256) * ceil_div(cols, 256);
+    g.wide = t256 >= 192;    // three quarters of the compute units at least
+    const int b = g.wide ? 256 : 128;
+    g.tiles_i = (unsigned)ceil_div(rows, b);
+    g.tiles_j = (unsigned)ceil_div(cols, b);
+    g.steps = (int)(depth_padded / kBK) * pairs;
+    const long long tiles = (long long)g.tiles_i * g.tiles_j;
+    // few tiles: pieces of the contraction, until every compute unit has one (two of the small ones), none under 8 steps
+    long long s = g.wide ? 1 : 512 / tiles;
+    if (s > g.steps / 8) s = g.steps / 8;
+    if (s < 1) s = 1;
+    g.split_len = (int)ceil_div(g.steps, s);
+    g.splits = (int)ceil_div(g.steps, g.split_len);
+    g.part_bytes = g.splits > 1 ? sizeof(float) * (size_t)g.splits * rows * cols : 0;
+    return g;
+}
+
+template <typename T, int OP>
+hipError_t run_gemm(const void* a, long long lda, long long plane_a, const void* b, long long ldb, long long plane_b,
+                    long long rows, long long cols, long long depth_padded, TileArgs t, void* part, hipStream_t stream) {
+    typedef typename Plane<T>::type P;
+    const GemmPlan g = plan_gemm(rows, cols, depth_padded, sizeof(T) == 4 ? kPairs : 1);
+    GemmArgs p = {};
+    p.a = a, p.b = b, p.lda = lda, p.ldb = ldb, p.plane_a = plane_a, p.plane_b = plane_b;
+    p.rows = rows, p.cols = cols, p.k_blocks = (int)(depth_padded / kBK), p.pairs = sizeof(T) == 4 ? kPairs : 1;
+    p.splits = g.splits, p.split_len = g.split_len, p.tiles_i = g.tiles_i, p.tiles_j = g.tiles_j;
+    t.part = static_cast<float*>(part);
+    t.rows = rows, t.cols = cols, t.splits = g.splits;
+    p.t = t;
+    const dim3 grid(g.tiles_i * g.tiles_j, g.splits);
+    if (g.wide)
+        linear_gemm_kernel<P, T, 256, 256, 128, 64, OP><<<grid, 512, 0, stream>>>(p);
+    else
+        linear_gemm_kernel<P, T, 128, 128, 64, 64, OP><<<grid, 256, 0, stream>>>(p);
+    if (g.splits > 1) {
+        linear_join_kernel<T, OP><<<dim3(join_blocks(rows * cols)), kThreads, 0, stream>>>(t);
+    }
+    return hipGetLastError();
+}
+
+template <typename T>
+hipError_t run_pack(const PackArgs& p, hipStream_t stream) {
+    const dim3 grid((unsigned)((p.pc / 64) * (p.pr / 64)));
+    if (p.act != kActNone)
+        linear_pack_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
+    else
+        linear_pack_kernel<T, false><<<grid, kThreads, 0, stream>>>(p);
+    return hipGetLastError();
+}
+
+// A 16-bit matrix that the large products can read where it stands: whole lines, on 16 bytes.
+bool reads_in_place(const void* x, long long ld, long long cols, int dtype) {
+    return dtype != 0 && cols % kBK == 0 && ld % 8 == 0 && ld <= kMaxLd && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+}
+
+// Scratch of a forward / backward call through the large products (offsets from the workspace's start).
+struct BigWs {
+    long long pm, pn, pk;    // m, n, k padded
+    size_t x, w, dz, turned_dz, turned_w, turned_x, sums, part, total;
+};
+BigWs carve_big(long long m, long long n, long long k, int dtype, bool backward) {
+    BigWs o = {};
+    o.pm = round_up(m, kBK), o.pn = round_up(n, kBK), o.pk = round_up(k, kBK);
+    const size_t e = dtype == 0 ? 2 * kPlanes : 2;
+    const int pairs = dtype == 0 ? kPairs : 1;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        const size_t here = at;
+        at += (bytes + 255) & ~(size_t)255;
+        return here;
+    };
+    if (!backward) {
+        o.x = take(e * m * o.pk);
+        o.w = take(e * n * o.pk);
+        o.part = take(plan_gemm(m, n, o.pk, pairs).part_bytes);
+    } else {
+        o.dz = take(e * m * o.pn);
+        o.turned_dz = take(e * n * o.pm);
+        o.turned_w = take(e * k * o.pn);
+        o.turned_x = take(e * k * o.pm);
+        o.sums = take(sizeof(float) * (o.pm / 64) * n);
+        const size_t dx = plan_gemm(m, k, o.pn, pairs).part_bytes, dw = plan_gemm(n, k, o.pm, pairs).part_bytes;
+        o.part = take(dx > dw ? dx : dw);
+    }
+    o.total = at;
+    return o;
+}
+
+template <typename T>
+hipError_t forward_large(const LinearArgs& a, TileArgs t, void* ws_, hipStream_t stream) {
+    char* ws = static_cast<char*>(ws_);
+    const BigWs o = carve_big(a.m, a.n, a.k, a.dtype, false);
+    const void *x = a.x, *w = a.w;
+    long long ldx = a.ldx, ldw = a.ldw;
+    if (!reads_in_place(a.x, a.ldx, a.k, a.dtype)) {
+        if (hipError_t e = run_pack<T>({a.x, nullptr, a.ldx, a.m, a.k, o.pm, o.pk, kActNone, ws + o.x, nullptr, nullptr}, stream)) return e;
+        x = ws + o.x, ldx = o.pk;
+    }
+    if (!reads_in_place(a.w, a.ldw, a.k, a.dtype)) {
+        if (hipError_t e = run_pack<T>({a.w, nullptr, a.ldw, a.n, a.k, o.pn, o.pk, kActNone, ws + o.w, nullptr, nullptr}, stream)) return e;
+        w = ws + o.w, ldw = o.pk;
+    }
+    return run_gemm<T, kForward>(x, ldx, a.m * o.pk, w, ldw, a.n * o.pk, a.m, a.n, o.pk, t, ws + o.part, stream);
+}
+
+template <typename T>
+hipError_t backward_large(const LinearArgs& a, const void* z, const void* dy, void* dx, void* dw, void* dbias, void* ws_,
+                          hipStream_t stream) {
+    char* ws = static_cast<char*>(ws_);
+    const BigWs o = carve_big(a.m, a.n, a.k, a.dtype, true);
+    const bool dy_as_it_is = a.act == kActNone && reads_in_place(dy, a.n, a.n, a.dtype);
+    const bool pack_dz = dx && !dy_as_it_is;
+    float* sums = dbias ? reinterpret_cast<float*>(ws + o.sums) : nullptr;
+    if (pack_dz || dw || dbias)
+        if (hipError_t e = run_pack<T>({dy, z, a.n, a.m, a.n, o.pm, o.pn, a.act, pack_dz ? ws + o.dz : nullptr,
+                                        dw ? ws + o.turned_dz : nullptr, sums}, stream)) return e;
+    TileArgs t = {};
+    if (dx) {
+        if (hipError_t e = run_pack<T>({a.w, nullptr, a.ldw, a.n, a.k, o.pn, o.pk, kActNone, nullptr, ws + o.turned_w, nullptr}, stream)) return e;
+        t.out = dx;
+        if (hipError_t e = run_gemm<T, kDx>(pack_dz ? ws + o.dz : dy, o.pn, a.m * o.pn, ws + o.turned_w, o.pn, a.k * o.pn, a.m, a.k,
+                                            o.pn, t, ws + o.part, stream)) return e;
+    }
+    if (dw) {
+        if (hipError_t e = run_pack<T>({a.x, nullptr, a.ldx, a.m, a.k, o.pm, o.pk, kActNone, nullptr, ws + o.turned_x, nullptr}, stream)) return e;
+        t.out = dw;
+        if (hipError_t e = run_gemm<T, kDw>(ws + o.turned_dz, o.pm, a.n * o.pm, ws + o.turned_x, o.pm, a.k * o.pm, a.n, a.k, o.pm, t,
+                                            ws + o.part, stream)) return e;
+    }
+    if (dbias) {
+        linear_bias_kernel<T><<<dim3((unsigned)ceil_div(a.n, 64)), kThreads, 0, stream>>>(sums, ceil_div(a.m, 64), a.n,
+                                                                                          static_cast<T*>(dbias));
+    }
+    return hipGetLastError();
+}
+
+// scratch of dx in front of that of dw, where neither goes through the large tiles
+size_t backward_dx_bytes(long long m, long long n, long long k, int dtype) {
+    const size_t bytes = has_few_rows(m, n, k) ? few_dx_bytes(m, n, k, dtype == 0 ? 4 : 2) : tile_bytes(m, k, n);
+    return (bytes + 255) & ~(size_t)255;
 }
 
 template <typename T>
@@ -270,32 +1008,54 @@ hipError_t forward_t(const LinearArgs& a, void* y, void* z, void* ws, hipStream_
     p.bias = a.bias, p.residual = a.residual, p.ldr = a.ldr;
     p.rows = a.m, p.cols = a.n, p.depth = a.k, p.n = a.n, p.act = a.act;
     p.out = y, p.keep = z;
-    return run_tiles<T, kForward>(p, ws, stream);
+    if (has_few_rows(a.m, a.n, a.k)) return run_few_rows<T>(p, stream);
+    if (is_large(a.m, a.n, a.k)) return forward_large<T>(a, p, ws, stream);
+    const unsigned pieces = set_tiles(p, ws);
+    linear_tile_forward_kernel<T><<<dim3(pieces), kThreads, 0, stream>>>(p);
+    if (p.splits > 1) linear_join_kernel<T, kForward><<<dim3(join_blocks(p.rows * p.cols)), kThreads, 0, stream>>>(p);
+    return hipGetLastError();
 }
 
 template <typename T>
-hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* dx, void* dw, void* dbias, void* ws,
+hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* dx, void* dw, void* dbias, void* ws_,
                       hipStream_t stream) {
+    if (is_large(a.m, a.n, a.k)) return backward_large<T>(a, z, dy, dx, dw, dbias, ws_, stream);
+    char* ws = static_cast<char*>(ws_);
     TileArgs p = {};
-    p.z = z, p.dy = dy, p.n = a.n, p.act = a.act;
+    p.z = z, p.dy = dy, p.n = a.n, p.act = a.act, p.splits = 1;
+    TileArgs q = p;
+    unsigned pieces_dx = 0, pieces_dw = 0;
     if (dx) {
         p.b = a.w, p.ldb = a.ldw, p.rows = a.m, p.cols = a.k, p.depth = a.n, p.out = dx;
-        if (hipError_t e = run_tiles<T, kDx>(p, ws, stream)) return e;
+        if (has_few_rows(a.m, a.n, a.k)) {
+            if (hipError_t e = run_few_rows_dx<T>(p, ws, stream)) return e;
+        } else {
+            pieces_dx = set_tiles(p, ws);
+        }
     }
     if (dw || dbias) {
-        p.b = a.x, p.ldb = a.ldx, p.rows = a.n, p.cols = a.k, p.depth = a.m, p.out = dw, p.dbias = dbias;
-        if (hipError_t e = run_tiles<T, kDw>(p, ws, stream)) return e;
+        // (for dbias alone there is no product: one column of tiles, and x, which may be NULL, is not read)
+        q.b = dw ? a.x : nullptr, q.ldb = a.ldx, q.rows = a.n, q.cols = dw ? a.k : 1, q.depth = a.m, q.out = dw, q.dbias = dbias;
+        pieces_dw = set_tiles(q, ws + backward_dx_bytes(a.m, a.n, a.k, a.dtype));
     }
-    return hipSuccess;
+    if (pieces_dx + pieces_dw == 0) return hipGetLastError();
+    linear_tile_backward_kernel<T><<<dim3(pieces_dx + pieces_dw), kThreads, 0, stream>>>(p, pieces_dx, q);
+    if (pieces_dx == 0) p.splits = 1;      // (its own launches have joined it)
+    if (p.splits > 1 || q.splits > 1) {
+        const long long ex = p.splits > 1 ? p.rows * p.cols : 0, ew = q.splits > 1 ? q.rows * q.cols : 0;
+        linear_join_backward_kernel<T><<<dim3(join_blocks(ex > ew ? ex : ew)), kThreads, 0, stream>>>(p, q);
+    }
+    return hipGetLastError();
 }
 
 }  // namespace
 
 size_t linear_workspace_bytes(long long m, long long n, long long k, int dtype, int act, int backward) {
-    (void)dtype, (void)act;
-    if (!backward) return tile_bytes(m, n, k);
-    const size_t a = tile_bytes(m, k, n), b = tile_bytes(n, k, m);
-    return a > b ? a : b;
+    (void)act;
+    if (is_large(m, n, k)) return carve_big(m, n, k, dtype, backward).total;
+    if (!backward) return has_few_rows(m, n, k) ? 0 : tile_bytes(m, n, k);
+    const size_t dw = tile_bytes(n, k, m), bias = tile_bytes(n, 1, m);      // (dbias alone is cut up by itself)
+    return backward_dx_bytes(m, n, k, dtype) + (dw > bias ? dw : bias);
 }
 
 hipError_t launch_linear_forward(const LinearArgs& a, void* y, void* z, void* ws, hipStream_t stream) {

@@ -71,6 +71,14 @@ __device__ __forceinline__ void Vec16<f16>::set(const float (&v)[8]) {
     raw = __builtin_bit_cast(u32x4, t);
 }
 
+// 16 bytes that start at any element (the memory pipe takes unaligned addresses; a load then touches one line more)
+template <typename T>
+__device__ __forceinline__ Vec16<T> load_vec(const T* p) {
+    Vec16<T> v;
+    __builtin_memcpy(&v.raw, p, 16);
+    return v;
+}
+
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // the wave's number in its block, known to be the same in all lanes
