@@ -29,6 +29,9 @@ constexpr int kMaxTop = 64;        // one entry per lane of a wave
 constexpr int kGather = 4;         // candidates of a row, in 64s, that are sorted out in one go (>= kWaves)
 constexpr int kShortRow = 1024;    // up to here a wave takes a whole row: a block's four waves would find less than
                                    // one 16-byte vector per lane each
+// A wave takes a row of up to kShortTopRow classes by itself, too, where there are kManyRows of them (top logits):
+// sorting out a row's candidates is one wave's work, and this keeps all of them at it.
+constexpr int kShortTopRow = 16384, kManyRows = 2048;
 constexpr int kLoads = 4;          // vectors a lane has in flight
 constexpr int kAhead = 4;          // vectors fetched ahead of the one at work, where the k best are kept
 
@@ -71,6 +74,46 @@ __device__ __forceinline__ float lse_value(const LseAcc& a, float inv_t) {
     if (a.s == 0.f) return -INFINITY;               // every entry -inf
     return fmaf(a.m == -INFINITY ? 0.f : a.m, inv_t, kLn2 * log2f(a.s));
 }
+
+// The same for a wave that has seen a sample of its entries: one reference r for all lanes and no running
+// maximum.  An entry may exceed r by up to 64 in the exponent before it is moved (the sum stays
+// far from overflow), and (x - r) c is one multiply-add with the product r c rounded; what that rounding does to
+// all terms alike is taken out at the end.  Where r c would overflow (masks at the lowest value), the difference comes first.
+struct WaveLse {
+    float r, rc, err, limit, s;
+    int far;
+    __device__ __forceinline__ void init(float sample_max, float c) {
+        r = -INFINITY, rc = err = s = 0.f, far = 0, limit = -INFINITY;
+        if (sample_max != -INFINITY) refer(sample_max, c);
+    }
+    __device__ __forceinline__ void refer(float to, float c) {
+        s *= fast_exp2((r - to) * c - err);
+        r = to;
+        far = uniform((int)!(fabsf(r) * c < 1e37f));
+        rc = far ? 0.f : r * c;
+        err = far ? 0.f : fmaf(r, c, -rc);
+        limit = r + 64.f / c;
+        s *= fast_exp2(err);
+    }
+    template <int N>
+    __device__ __forceinline__ void add(const float (&f)[N], float vm, float c) {
+        if (any_lane(vm > limit)) refer(uniform(wave_max(vm)), c);
+        if (!far) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s += fast_exp2(fmaf(f[i], c, -rc));
+        } else {
+#pragma unroll
+            for (int i = 0; i < N; ++i) s += fast_exp2((f[i] - r) * c);
+        }
+    }
+    __device__ __forceinline__ LseAcc finish() {
+        LseAcc a;
+        a.s = wave_sum(s) * fast_exp2(-err);
+        a.m = r;
+        a.r = (r == -INFINITY) ? 0.f : r;
+        return a;
+    }
+};
 
 // ------------------------------------------------------------------ a row, vector by vector
 
@@ -138,6 +181,33 @@ __device__ __forceinline__ u64 make_entry(float x, long long index) {
     return ((u64)order_key(x) << 32) | (uint32_t)~(uint32_t)index;
 }
 
+// Candidates lie in the lists as they were read, the value's bits in the upper half and the index in the lower (most
+// are dropped again, and turning them into entries would be half of what keeping one costs).
+__device__ __forceinline__ u64 raw_candidate(float x, uint32_t index) { return ((u64)__float_as_uint(x) << 32) | index; }
+__device__ __forceinline__ u64 entry_of(u64 raw) { return make_entry(__uint_as_float((uint32_t)(raw >> 32)), (uint32_t)raw); }
+__device__ __forceinline__ u64 raw_of(u64 entry) { return raw_candidate(key_value((uint32_t)(entry >> 32)), ~(uint32_t)entry); }
+
+// The largest t in [lo, hi] with count(t) >= k, where count falls and count(lo) >= k; an earlier one as soon as its count is
+// at most k + slack.  Three thresholds a step: the steps depend on each other, a step's counts do not.
+template <typename Count>
+__device__ __forceinline__ uint32_t search_threshold(uint32_t lo, uint32_t hi, int k, int slack, bool& exact, int steps, Count count) {
+    exact = false;
+    while (lo < hi && steps-- > 0) {
+        const uint32_t t2 = lo + (hi - lo) / 2 + 1, t1 = lo + (t2 - lo + 1) / 2, t3 = t2 + (hi - t2 + 1) / 2;
+        const int c1 = count(t1), c2 = count(t2), c3 = count(t3);
+        int c = k + slack + 1;
+        if (c3 >= k) lo = t3, c = c3;
+        else if (c2 >= k) lo = t2, hi = t3 - 1, c = c2;
+        else if (c1 >= k) lo = t1, hi = t2 - 1, c = c1;
+        else hi = t1 - 1;
+        if (c <= k + slack) {
+            exact = true;
+            break;
+        }
+    }
+    return lo;
+}
+
 // The smallest entry of a selection of at least k of the wave's entries e[0..R) (0: none): exactly the k
 // best where slack is 0, up to `slack` more otherwise.  Bisection over the values, then over the
 // indices of one value, each step a compare and a population count per 64 entries.
@@ -146,7 +216,7 @@ __device__ __forceinline__ u64 select_from(const u64 (&e)[R], int k, int slack) 
     auto count_hi = [&](uint32_t t) {
         int c = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r) c += __popcll(__ballot((uint32_t)(e[r] >> 32) >= t));
+        for (int r = 0; r < R; ++r) c += __popcll(ballot((uint32_t)(e[r] >> 32) >= t));
         return c;
     };
     if (count_hi(1u) <= k) return 1ull;
@@ -156,46 +226,31 @@ __device__ __forceinline__ u64 select_from(const u64 (&e)[R], int k, int slack) 
 #pragma unroll
     for (int off = 32; off; off >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, off));
     best = (uint32_t)__builtin_amdgcn_readfirstlane((int)best);
-    uint32_t lo = 1u, hi = best;              // count(lo) >= k;  count(hi + 1) = 0
-    while (lo < hi) {
-        const uint32_t mid = lo + (hi - lo + 1) / 2;
-        const int c = count_hi(mid);
-        if (c >= k) {
-            lo = mid;
-            if (c <= k + slack) return (u64)lo << 32;
-        } else {
-            hi = mid - 1;
-        }
-    }
+    bool exact;
+    const uint32_t lo = search_threshold(1u, best, k, slack, exact, 64, count_hi);
+    if (exact) return (u64)lo << 32;
     // more than k + slack entries >= lo, fewer than k above it: the rest by index among those of value lo
     int above = 0;
 #pragma unroll
-    for (int r = 0; r < R; ++r) above += __popcll(__ballot((uint32_t)(e[r] >> 32) > lo));
+    for (int r = 0; r < R; ++r) above += __popcll(ballot((uint32_t)(e[r] >> 32) > lo));
     const int need = k - above;
-    uint32_t l2 = 0u, h2 = 0xffffffffu;
-    while (l2 < h2) {
-        const uint32_t mid = l2 + (h2 - l2) / 2 + 1;
+    const uint32_t l2 = search_threshold(0u, 0xffffffffu, need, 0, exact, 64, [&](uint32_t t) {
         int c = 0;
 #pragma unroll
-        for (int r = 0; r < R; ++r) c += __popcll(__ballot((uint32_t)(e[r] >> 32) == lo && (uint32_t)e[r] >= mid));
-        if (c >= need) {
-            l2 = mid;
-            if (c == need) break;
-        } else {
-            h2 = mid - 1;
-        }
-    }
+        for (int r = 0; r < R; ++r) c += __popcll(ballot((uint32_t)(e[r] >> 32) == lo && (uint32_t)e[r] >= t));
+        return c;
+    });
     return ((u64)lo << 32) | l2;
 }
 
 // writes the entries >= t of the wave to dst[0..), in any order; returns how many
-template <int R>
+template <int R, bool kRaw = false>
 __device__ __forceinline__ int keep_entries(const u64 (&e)[R], u64 t, u64* dst) {
     int n = 0;
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-        const u64 mask = __ballot(e[r] >= t);
-        if (e[r] >= t) dst[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] = e[r];
+        const u64 mask = ballot(e[r] >= t);
+        if (e[r] >= t) dst[n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] = kRaw ? raw_of(e[r]) : e[r];
         n += __popcll(mask);
     }
     return n;
@@ -208,9 +263,9 @@ __device__ __forceinline__ int shrink_list(u64* buf, int cnt, int k, int slack, 
     u64 e[R];
     wave_lds_fence();
 #pragma unroll
-    for (int r = 0; r < R; ++r) e[r] = (r * 64 + lane < cnt) ? buf[r * 64 + lane] : 0ull;
+    for (int r = 0; r < R; ++r) e[r] = (r * 64 + lane < cnt) ? entry_of(buf[r * 64 + lane]) : 0ull;
     t = select_from<R>(e, k, slack);
-    const int n = keep_entries<R>(e, t, buf);
+    const int n = keep_entries<R, true>(e, t, buf);
     wave_lds_fence();
     return n;
 }
@@ -219,7 +274,7 @@ __device__ __forceinline__ int shrink_list(u64* buf, int cnt, int k, int slack, 
 template <typename T>
 struct WaveList {
     static constexpr int kTrigger = 256;
-    static constexpr int kCap = kTrigger + 64 * Vec16<T>::N;   // a vector adds up to 64 N entries
+    static constexpr int kCap = kTrigger + 64 * 4;             // four elements of every lane add up to 256 entries
     u64* buf;
     int cnt, k;
     float tau;      // k entries of the list are >= tau; all of them came earlier, so a later entry must exceed it
@@ -236,12 +291,36 @@ struct WaveList {
             open = false;
         }
     }
-    __device__ __forceinline__ void push(float x, long long index, bool valid) {
-        const bool take = valid && (open || x > tau);
-        const u64 mask = __ballot(take);
-        if (mask) {
-            if (take) buf[cnt + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u))] = make_entry(x, index);
-            cnt += __popcll(mask);
+    // The lanes that `take`: their candidates go behind the others, in the lanes' order; what there is no room for lands in
+    // one slot behind the list, and cnt says so (kept free of conditions: cnt stays in a scalar register).
+    __device__ __forceinline__ void append(u64 mask, bool take, float x, uint32_t index) {
+        if (take) {
+            const int at = cnt + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+            buf[min(at, kCap)] = raw_candidate(x, index);
+        }
+        cnt += __popcll(mask);
+    }
+    // what of a vector of every lane exceeds tau
+    template <int N>
+    __device__ __forceinline__ void push(const float (&f)[N], uint32_t first) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const bool take = f[i] > tau;
+            append(ballot(take), take, f[i], first + i);
+        }
+    }
+    // The same with room made first; also while everything is taken (`valid` entries of the lane are real).
+    template <int N>
+    __device__ __forceinline__ void push_careful(const float (&f)[N], uint32_t first, int valid) {
+#pragma unroll 1
+        for (int h = 0; h < N; h += 4) {
+            room();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float x = (N > 4 && h) ? f[N - 4 + i] : f[i];
+                const bool take = h + i < valid && (open || x > tau);
+                append(ballot(take), take, x, first + h + i);
+            }
         }
     }
     __device__ __forceinline__ void room() {
@@ -273,18 +352,19 @@ __device__ __forceinline__ void write_top(u64 e, int found, int k, T* __restrict
 }
 
 // A value that at least k of the row's (or split's) entries reach, from the largest entry of every lane's first few
-// vectors: 256 lanes (64 of a short row) of 8 to 32 entries each, whose k-th largest maximum is rarely far below the
-// k-th largest entry, so that of those few thousand entries little more than k become candidates instead of all.
-// 0: fewer than k lanes have one.  `keys`: 64 WPR words of LDS of this row.
+// vectors (of a row with one wave, the largest two): the k-th largest of 256 (128) such maxima is
+// rarely far below the k-th largest entry, so that of those few thousand entries little more than k become
+// candidates instead of all.  0: there are fewer than k maxima.  `keys`: 64 WPR words of LDS of this row.
 template <int WPR>
-__device__ __forceinline__ uint32_t bound_of_maxima(float lane_max, bool any, int k, uint32_t* keys, int w) {
+__device__ __forceinline__ uint32_t bound_of_maxima(float max1, float max2, bool any, int k, uint32_t* keys, int w) {
+    constexpr int R = WPR == 1 ? 2 : WPR;
     const int lane = threadIdx.x & 63;
-    uint32_t e[WPR];
-    const uint32_t mine = any ? order_key(lane_max) : 0u;
-    if (WPR == 1) {
-        e[0] = mine;
+    uint32_t e[R];
+    e[0] = any ? order_key(max1) : 0u;
+    if constexpr (WPR == 1) {
+        e[1] = any ? order_key(max2) : 0u;
     } else {
-        keys[w * 64 + lane] = mine;
+        keys[w * 64 + lane] = e[0];
         __syncthreads();
 #pragma unroll
         for (int q = 0; q < WPR; ++q) e[q] = keys[q * 64 + lane];
@@ -292,39 +372,31 @@ __device__ __forceinline__ uint32_t bound_of_maxima(float lane_max, bool any, in
     auto count = [&](uint32_t t) {
         int c = 0;
 #pragma unroll
-        for (int q = 0; q < WPR; ++q) c += __popcll(__ballot(e[q] >= t));
+        for (int q = 0; q < R; ++q) c += __popcll(ballot(e[q] >= t));
         return c;
     };
     if (count(1u) < k) return 0u;
     uint32_t hi = e[0];
+    if constexpr (WPR > 1) {
 #pragma unroll
-    for (int q = 1; q < WPR; ++q) hi = max(hi, e[q]);
+        for (int q = 1; q < R; ++q) hi = max(hi, e[q]);
+    }
 #pragma unroll
     for (int off = 32; off; off >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, off));
     hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)hi);
-    uint32_t lo = 1u;                                    // count(lo) >= k
-    for (int step = 0; step < 18 && lo < hi; ++step) {   // (near is enough: an eighth of an octave after 12 steps)
-        const uint32_t mid = lo + (hi - lo + 1) / 2;
-        const int c = count(mid);
-        if (c >= k) {
-            lo = mid;
-            if (c <= k + k / 8) break;
-        } else {
-            hi = mid - 1;
-        }
-    }
-    return lo;
+    bool exact;      // (near is enough: ten steps end within 2^12 of it, a two-thousandth of an octave)
+    return search_threshold(1u, hi, k, k / 8, exact, 10, count);
 }
 
 // Block (row group, split).  WPR: waves per row.
 template <typename T, int WPR>
-__global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restrict__ x, long long ld, long long n, long long v,
-                                                              int k, float c, float inv_t, int splits, long long split_len,
+__global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restrict__ x, long long ld, long long n, int v,
+                                                              int k, float c, float inv_t, int splits, int split_len,
                                                               T* __restrict__ values, int* __restrict__ idx,
                                                               float* __restrict__ lse, u64* __restrict__ part,
                                                               float2* __restrict__ part_ms) {
     constexpr int N = Vec16<T>::N;
-    __shared__ u64 lists[kWaves][WaveList<T>::kCap];
+    __shared__ u64 lists[kWaves][WaveList<T>::kCap + 1];
     __shared__ float2 ms[kWaves];
     __shared__ int counts[kWaves];
     __shared__ uint32_t maxima[kThreads];
@@ -333,98 +405,124 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
     const long long row = (long long)blockIdx.x * (kWaves / WPR) + wave / WPR;
     const bool live = row < n;
     const int split = blockIdx.y;
-    const long long lo = split * split_len, hi = min(v, lo + split_len);
+    const int lo = split * split_len, hi = (int)min((long long)v, (long long)lo + split_len);   // (positions in a row fit 31 bits)
 
-    LseAcc acc;
-    acc.init();
+    WaveLse sum;
+    sum.init(-INFINITY, c);
     WaveList<T> list;
     list.init(lists[wave], k);
     if (live) {
-        // the elements in front of the first 16-byte vector, the vectors (every WPR-th kilobyte), the
-        // elements behind the last one: one step each of one loop, so that the list's code exists once
         const T* xr = x + row * ld;
-        long long head = (long long)(((16 - (reinterpret_cast<uintptr_t>(xr + lo) & 15)) & 15) / sizeof(T));
+        int head = (int)(((16 - (reinterpret_cast<uintptr_t>(xr + lo) & 15)) & 15) / sizeof(T));
         if (head > hi - lo) head = hi - lo;
-        const long long nv = (hi - lo - head) / N, body = lo + head, tail = body + nv * N;
+        const int nv = (hi - lo - head) / N, body = lo + head, tail = body + nv * N;
         const u32x4* vecs = reinterpret_cast<const u32x4*>(xr + body);
-        const long long step = (long long)WPR * 64;
-        long long at = (long long)w * 64;
-        bool front = w == 0 && head > 0, back = w == 0 && tail < hi;
-        auto fetch = [&](long long v0) {
-            u32x4 r = {0u, 0u, 0u, 0u};
-            if (v0 + lane < nv) r = vecs[v0 + lane];
+        constexpr int step = WPR * 64;
+        int at = w * 64;
+        const float none = -INFINITY;
+        Vec16<T> empty;
+        {
+            float f[N];
+#pragma unroll
+            for (int i = 0; i < N; ++i) f[i] = none;
+            empty.set(f);
+        }
+        auto fetch = [&](int v0) {
+            Vec16<T> r = empty;
+            const u32x4* p = vecs + v0;
+            if (v0 + 64 <= nv || v0 + lane < nv) r.raw = p[lane];
             return r;
         };
-        u32x4 ahead[kAhead];
+        Vec16<T> ahead[kAhead];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) ahead[u] = fetch(at + u * step);
         {
-            float top = -INFINITY;
-            bool any = false;
+            float max1 = none, max2 = none;
 #pragma unroll
             for (int u = 0; u < kAhead; ++u) {
-                Vec16<T> v;
-                v.raw = ahead[u];
                 float f[N];
-                const float m = unpack<T>(v, f);
-                if (at + u * step + lane < nv) {
-                    top = any ? fmaxf(top, m) : m;
-                    any = true;
+                if constexpr (WPR == 1) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) {
+                        const float x = ahead[u].get(i);
+                        max2 = fmaxf(max2, fminf(max1, x));
+                        max1 = fmaxf(max1, x);
+                    }
+                } else {
+                    max1 = fmaxf(max1, unpack<T>(ahead[u], f));
                 }
             }
-            const uint32_t bound = bound_of_maxima<WPR>(top, any, k, maxima, w);
-            if (bound > order_key(-INFINITY)) {
+            sum.init(uniform(wave_max(max1)), c);
+            const uint32_t bound = bound_of_maxima<WPR>(max1, max2, at + lane < nv, k, maxima, w);
+            if (bound > order_key(none)) {
                 // everything from the bound on: what exceeds the value below it (-0, just below +0, is no less)
                 list.tau = key_value(bound - (bound == order_key(0.f) ? 2u : 1u));
                 list.open = false;
             }
         }
+        // In turn: the elements in front of the first 16-byte vector; the vectors, every WPR-th kilobyte, kAhead of them at a
+        // time while as many are on their way; the elements behind the last one.  A group whose candidates
+        // do not fit its list (equal values, rising rows), and everything while fewer than k entries are known, goes vector
+        // by vector through the careful path, of which there is one copy.
+        bool front = w == 0 && head > 0, back = w == 0 && tail < hi;
         while (true) {
-            float f[N], vm;
-            int valid;              // elements of this lane
-            long long first;
-            if (!front && at < nv) {
-                Vec16<T> cur;
-                cur.raw = ahead[0];
+            int from = 0, to = 0;      // the single elements of this turn
+            bool careful = false;
+            if (front) {
+                from = lo, to = body, front = false, careful = true;
+            } else if (at < nv) {
+                if (list.cnt > WaveList<T>::kTrigger) list.shrink(k / 4);
+                const int before = list.cnt;
 #pragma unroll
-                for (int u = 0; u + 1 < kAhead; ++u) ahead[u] = ahead[u + 1];
-                ahead[kAhead - 1] = fetch(at + kAhead * step);
-                vm = unpack<T>(cur, f);
-                valid = (at + lane < nv) ? N : 0;
-                first = body + (at + lane) * N;
-                at += step;
-            } else if (front || back) {
-                const long long from = front ? lo : tail, to = front ? body : hi;
-                valid = (from + lane < to) ? 1 : 0;
-                first = from + lane;
-                f[0] = vm = valid ? to_f32(xr[first]) : -INFINITY;
-#pragma unroll
-                for (int i = 1; i < N; ++i) f[i] = -INFINITY;
-                if (front) front = false;
-                else back = false;
-            } else {
-                break;
+                for (int u = 0; u < kAhead; ++u) {
+                    float f[N];
+                    const float vm = unpack<T>(ahead[u], f);
+                    ahead[u] = fetch(at + (kAhead + u) * step);
+                    sum.add(f, vm, c);
+                    if (any_lane(vm > list.tau)) list.push(f, (uint32_t)(body + (at + u * step + lane) * N));
+                    __builtin_amdgcn_sched_barrier(0);      // one vector's floats in registers at a time
+                }
+                if (!list.open && list.cnt <= WaveList<T>::kCap) {
+                    at += kAhead * step;
+                    continue;
+                }
+                list.cnt = before;
+                careful = true;
+            } else if (back) {
+                from = tail, to = hi, back = false, careful = true;
             }
-            if (valid) {
-                acc.raise(vm, c);
+            if (!careful) break;
+            const bool single = to > from;
+            for (int u = 0; u < (single ? 1 : kAhead); ++u) {
+                float f[N];
+                int first;
+                int valid;
+                if (single) {
+                    first = from + lane;
+                    valid = first < to ? 1 : 0;
+                    f[0] = valid ? to_f32(xr[first]) : none;
 #pragma unroll
-                for (int i = 0; i < N; ++i) acc.add(f[i], c);
+                    for (int i = 1; i < N; ++i) f[i] = none;
+                    sum.add(f, f[0], c);
+                } else {
+                    const Vec16<T> v = fetch(at + u * step);
+                    unpack<T>(v, f);
+                    valid = at + u * step + lane < nv ? N : 0;
+                    first = body + (at + u * step + lane) * N;
+                }
+                list.push_careful(f, (uint32_t)first, valid);
             }
-            if (__any(valid && (list.open || vm > list.tau))) {
-                list.room();
-#pragma unroll
-                for (int i = 0; i < N; ++i) list.push(f[i], first + i, i < valid);
-            }
+            if (!single) at += kAhead * step;
         }
-        acc.join_wave(c);
     }
+    LseAcc acc = sum.finish();
     // the k best of the row's candidates: of all waves' at once, or, where there are many, of each wave's best
     u64 mine = 0;
     int found = 0;
     if (WPR == 1) {
         list.shrink(0);
         found = list.cnt;
-        mine = (lane < found) ? list.buf[lane] : 0ull;
+        mine = (lane < found) ? entry_of(list.buf[lane]) : 0ull;
     } else {
         if (lane == 0) {
             ms[wave] = make_float2(acc.m, acc.s);
@@ -446,14 +544,14 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
 #pragma unroll
         for (int r = 0; r < kGather; ++r) {
             if (many) {
-                e[r] = (r < kWaves && lane < counts[r % kWaves]) ? lists[r % kWaves][lane] : 0ull;
+                e[r] = (r < kWaves && lane < counts[r % kWaves]) ? entry_of(lists[r % kWaves][lane]) : 0ull;
             } else {
                 const int at = r * 64 + lane;
                 int q = 0, from = 0;
 #pragma unroll
                 for (int o = 0; o + 1 < kWaves; ++o)
                     if (at >= ends[o]) q = o + 1, from = ends[o];
-                e[r] = at < total ? lists[q][at - from] : 0ull;
+                e[r] = at < total ? entry_of(lists[q][at - from]) : 0ull;
             }
         }
         wave_lds_fence();
@@ -548,7 +646,7 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ xr, long long v
         }
     }
     top_max = wave_max(top_max);
-    bad = __any(bad);
+    bad = any_lane(bad);
     const bool empty = top_max == -INFINITY || (acc.m == -INFINITY && acc.s == 0.f);
     float ref = 0.f, log_sum = 0.f, tau = 0.f, part = 0.f;
     if (!empty) {
@@ -793,11 +891,11 @@ hipError_t top_logits_t(const void* x, long long ld, long long n, long long v, i
     T* vt = static_cast<T*>(values);
     u64* part = static_cast<u64*>(ws);
     float2* part_ms = reinterpret_cast<float2*>(part + (size_t)n * splits * k);
-    if (v <= kShortRow) {
-        top_logits_kernel<T, 1><<<dim3((unsigned)ceil_div(n, kWaves)), kThreads, 0, stream>>>(xt, ld, n, v, k, c, 1.f / temperature, 1, v, vt, idx,
+    if (v <= kShortRow || (v <= kShortTopRow && n >= kManyRows)) {
+        top_logits_kernel<T, 1><<<dim3((unsigned)ceil_div(n, kWaves)), kThreads, 0, stream>>>(xt, ld, n, (int)v, k, c, 1.f / temperature, 1, (int)v, vt, idx,
                                                                                                lse, nullptr, nullptr);
     } else {
-        top_logits_kernel<T, kWaves><<<dim3((unsigned)n, splits), kThreads, 0, stream>>>(xt, ld, n, v, k, c, 1.f / temperature, splits, len, vt,
+        top_logits_kernel<T, kWaves><<<dim3((unsigned)n, splits), kThreads, 0, stream>>>(xt, ld, n, (int)v, k, c, 1.f / temperature, splits, (int)len, vt,
                                                                                         idx, lse, part, part_ms);
         if (splits > 1)
             top_logits_join_kernel<T><<<dim3((unsigned)n), 64 * kJoinWaves, 0, stream>>>(k, c, 1.f / temperature, splits, part, part_ms, vt, idx, lse);

@@ -84,6 +84,10 @@ __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_ex
 // the wave's number in its block, known to be the same in all lanes
 __device__ __forceinline__ int wave_id() { return __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6)); }
 
+// lanes for which b holds (straight from the comparison's mask)
+__device__ __forceinline__ unsigned long long ballot(bool b) { return __builtin_amdgcn_ballot_w64(b); }
+__device__ __forceinline__ bool any_lane(bool b) { return ballot(b) != 0; }
+
 // Between LDS writes and reads of different lanes of one wave (which the LDS serves in order): keeps the
 // compiler from moving one across the other.
 __device__ __forceinline__ void wave_lds_fence() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
@@ -98,6 +102,12 @@ __device__ __forceinline__ float wave_max(float v) {
     for (int off = 32; off; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
     return v;
 }
+
+// a value that is the same in all lanes, known to be
+__device__ __forceinline__ float uniform(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
+}
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 static inline long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 static inline long long round_up(long long a, long long b) { return ceil_div(a, b) * b; }

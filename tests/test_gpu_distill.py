@@ -302,7 +302,7 @@ def test_a_teachers_table_trains_a_student_to_it():
     want = (t * (torch.log(t) - logp.gather(1, idx.long()))).sum(1).mean()
     ww, wb = torch.autograd.grad(want, [wd, bd])
     # float32 logits of about 20: the softmax carries 2^-24 x 20 x a few, relative to the largest gradient
-    assert abs(float(loss) - float(want)) < 2e-5 * float(want)
+    assert abs(loss.item() - want.item()) < 2e-5 * want.item()
     assert float((dw - ww).abs().max()) < 2e-5 * float(ww.abs().max())
     assert float((db - wb).abs().max()) < 2e-5 * float(wb.abs().max())
 
@@ -324,7 +324,7 @@ def test_neighbor_loss_from_a_search_table(metric):
     t = torch.softmax(-table.dist2.double() / 4.0, 1)
     want = (t * (torch.log(t) - torch.log_softmax(s / 0.5, 1).gather(1, table.idx.long()))).sum(1).mean()
     wide = torch.autograd.grad(want, [a, b])
-    assert abs(float(loss) - float(want)) < 1e-5 * float(want)
+    assert abs(loss.item() - want.item()) < 1e-5 * want.item()
     for g, w in zip(grads, wide):
         assert float((g - w).abs().max()) < 5e-5 * float(w.abs().max())
     # beside the contrastive loss of the same embeddings, and with a table that pads
