@@ -7,7 +7,6 @@ if the library is missing or no MI355X is visible, the calls raise.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 from pathlib import Path
 
@@ -213,7 +212,7 @@ def knn_kept_fraction(q, r, k, *, groups=AUTO_PROBE_GROUPS, group_rows=None):
     group_rows = max(1, min(group_rows, n))
     centres = q[torch.arange(groups, device=q.device) * (n // groups) + n // (2 * groups)]
     # |q - c|^2 - |c|^2, a row per centre: q is read once for all of them
-    score = linear_forward(-2.0 * centres, q, (q * q).sum(1))[0]
+    score = torch_ops().linear_act(-2.0 * centres, q, (q * q).sum(1), None, ACTIVATIONS["none"])
     # a radius that holds the clump with room to spare, read off at most 65 536 evenly spaced
     # queries, so that the exact selection runs over a few thousand rows instead of all
     pool = score[:, ::max(1, n // AUTO_PROBE_POOL)] if n > AUTO_PROBE_POOL else score
@@ -544,132 +543,27 @@ def ntxent2_backward(zi, zj, temperature, lse_row, lse_col, grad_out):
     return dzi, dzj
 
 
-# ------------------------------------------------------------------ dense layer, distillation, top logits
-DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}   # SCMIAC_F32 / SCMIAC_F16 / SCMIAC_BF16
+# dense layer, distillation, top logits: the numbers the C ABI has for the names of the Python functions
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}         # SCMIAC_ACT_*
 REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}                      # SCMIAC_REDUCE_*
-TOP_MAX_K = 64
-DISTILL_MAX_K = 1024
+
+_torch_ops = None
 
 
-def _rows(t):
-    """``t`` (2-D) and its row stride, copied only if its columns are not next to each other."""
-    if t.shape[1] != 1 and t.stride(1) != 1:
-        t = t.contiguous()
-    return t, t.stride(0)
-
-
-@functools.lru_cache(maxsize=4096)
-def _size_of(name, *args):
-    """Answer of a ``*_workspace_size`` entry point (it depends on the arguments alone)."""
-    nbytes = ctypes.c_size_t(0)
-    _check(getattr(load_library(), name)(*args, ctypes.byref(nbytes)))
-    return nbytes.value
-
-
-def _raw_stream(device):
-    """:func:`_stream` for the operators of a training step, where its two microseconds count."""
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-def _scratch(nbytes, device):
-    """Scratch of one call.  Unlike :func:`_workspace`'s it belongs to the stream (or the graph under
-    capture) that the call runs on, so that calls on two streams and two captured graphs never share it."""
-    return torch.empty((nbytes,), dtype=torch.uint8, device=device) if nbytes else None
-
-
-def linear_forward(x, weight, bias=None, residual=None, activation="none", keep_z=False):
-    """``act(x @ weight.T + bias) + residual`` of 2-D device tensors of one type (no checks of shapes:
-    :func:`scmiac_amd.modeling.linear_act` makes them).  Returns ``(y, z)``; ``z`` is the pre-activation
-    that :func:`linear_backward` reads (None unless ``keep_z`` and the activation needs it)."""
-    device = x.device
-    act, code = ACTIVATIONS[activation], DTYPES[x.dtype]
-    (m, k), n = x.shape, weight.shape[0]
-    x, ldx = _rows(x)
-    weight, ldw = _rows(weight)
-    ldr = 0
-    if residual is not None:
-        residual, ldr = _rows(residual)
-    if bias is not None:
-        bias = bias.contiguous()
-    with _on_device(device):
-        need = _size_of("scmiac_linear_workspace_size", m, n, k, code, act, 0)
-        ws = _scratch(need, device)
-        y = torch.empty((m, n), dtype=x.dtype, device=device)
-        z = torch.empty((m, n), dtype=x.dtype, device=device) if keep_z and act else None
-        _check(load_library().scmiac_linear_forward(_ptr(x), ldx, _ptr(weight), ldw, _ptr(bias), _ptr(residual), ldr, m, n, k, code,
-                                          act, _ptr(y), _ptr(z), _ptr(ws), need, _raw_stream(device)))
-    return y, z
-
-
-def linear_backward(x, weight, z, dy, k, activation="none", need=(True, True, True)):
-    """Gradients ``(dx, dweight, dbias)`` of :func:`linear_forward`, None where ``need`` says so.  ``k``: columns of
-    ``x``, which is only read for ``dweight`` as ``weight`` is for ``dx`` (None otherwise)."""
-    device = dy.device
-    act, code = ACTIVATIONS[activation], DTYPES[dy.dtype]
-    m, n = dy.shape
-    x, ldx = (None, 0) if x is None else _rows(x)
-    weight, ldw = (None, 0) if weight is None else _rows(weight)
-    dy = dy.contiguous()
-    with _on_device(device):
-        size = _size_of("scmiac_linear_workspace_size", m, n, k, code, act, 1)
-        ws = _scratch(size, device)
-        dx = torch.empty((m, k), dtype=dy.dtype, device=device) if need[0] else None
-        dw = torch.empty((n, k), dtype=dy.dtype, device=device) if need[1] else None
-        db = torch.empty((n,), dtype=dy.dtype, device=device) if need[2] else None
-        _check(load_library().scmiac_linear_backward(_ptr(x), ldx, _ptr(weight), ldw, _ptr(z), _ptr(dy), m, n, k, code, act, _ptr(dx),
-                                           _ptr(dw), _ptr(db), _ptr(ws), size, _raw_stream(device)))
-    return dx, dw, db
-
-
-def top_logits(x, k, temperature=1.0):
-    """``(values, idx, lse)`` of the rows of a 2-D device tensor, see ``scmiac_top_logits``."""
-    device, code = x.device, DTYPES[x.dtype]
-    x, ld = _rows(x)
-    n, v = x.shape
-    with _on_device(device):
-        size = _size_of("scmiac_top_logits_workspace_size", n, v, k, code)
-        ws = _scratch(size, device)
-        values = torch.empty((n, k), dtype=x.dtype, device=device)
-        idx = torch.empty((n, k), dtype=torch.int32, device=device)
-        lse = torch.empty((n,), dtype=torch.float32, device=device)
-        _check(load_library().scmiac_top_logits(_ptr(x), ld, n, v, code, k, float(temperature), _ptr(values), _ptr(idx), _ptr(lse),
-                                      _ptr(ws), size, _raw_stream(device)))
-    return values, idx, lse
-
-
-def distill_forward(x, idx, top, teacher_lse, temperature, teacher_temperature, reduction):
-    """``(loss, row_stats, scale)`` of ``scmiac_distill_forward`` on 2-D device tensors (``idx`` int32 and
-    contiguous, ``top`` / ``teacher_lse`` float32 and contiguous)."""
-    device, code, red = x.device, DTYPES[x.dtype], REDUCTIONS[reduction]
-    x, ld = _rows(x)
-    n, v = x.shape
-    with _on_device(device):
-        size = _size_of("scmiac_distill_workspace_size", n, v, code)
-        ws = _scratch(size, device)
-        stats = torch.empty((n, 4), dtype=torch.float32, device=device)
-        loss = torch.empty((n,) if red == 0 else (), dtype=torch.float32, device=device)
-        scale = torch.empty((), dtype=torch.float32, device=device) if red else None
-        _check(load_library().scmiac_distill_forward(_ptr(x), ld, n, v, code, _ptr(idx), _ptr(top), idx.shape[1], _ptr(teacher_lse),
-                                           temperature, teacher_temperature, red, _ptr(loss), _ptr(stats), _ptr(scale),
-                                           _ptr(ws), size, _raw_stream(device)))
-    return loss, stats, scale
-
-
-def distill_backward(x, idx, top, temperature, teacher_temperature, stats, scale, grad):
-    """Gradient with respect to ``x``.  ``grad``: float32, one per row or (with a ``scale``) one in all."""
-    device, code = x.device, DTYPES[x.dtype]
-    x, ld = _rows(x)
-    n, v = x.shape
-    grad_stride = 0 if grad.dim() == 0 else grad.stride(0)
-    with _on_device(device):
-        # rows as far apart as x's where those are padded: both then start alike with respect to 16 bytes
-        ldd = ld if v <= ld <= 2 * v else v
-        dx = torch.empty((n, ldd), dtype=x.dtype, device=device)[:, :v]
-        _check(load_library().scmiac_distill_backward(_ptr(x), ld, n, v, code, _ptr(idx), _ptr(top), idx.shape[1], temperature,
-                                            teacher_temperature, _ptr(stats), _ptr(grad), grad_stride, _ptr(scale),
-                                            _ptr(dx), ldd, _raw_stream(device)))
-    return dx
+def torch_ops():
+    """The compiled torch functions (``csrc/torch_ops.cpp``) of the operators that run in every training step:
+    a Python autograd function around a ctypes call costs more time than their kernels."""
+    global _torch_ops
+    if _torch_ops is None:
+        load_library()
+        try:
+            from . import _torch_ops as module
+        except ImportError as exc:
+            raise ScmiacHipError(f"scmiac_amd/_torch_ops.so cannot be loaded ({exc}): build it with "
+                                 f"`make -C {LIB_PATH.parent}`; there is no fallback") from exc
+        module.bind(str(LIB_PATH))
+        _torch_ops = module
+    return _torch_ops
 
 
 def lu_row_perm(pivots, n, status=None):

@@ -8,9 +8,7 @@ neighbours a teacher's table lists instead of one positive per row.
 """
 from __future__ import annotations
 
-import torch
 import torch.nn as nn
-from torch.autograd.function import once_differentiable
 
 from .. import _hip
 from .dense import linear_act
@@ -23,34 +21,7 @@ def top_logits(logits, k, temperature=1.0):
     ``lse`` is ``log sum exp(logits / temperature)`` over the whole row.  Rows of fewer than ``k`` classes are padded
     with ``-inf`` and -1.  No gradient flows: a teacher is a constant."""
     _hip._cuda_device(logits, "logits")
-    _hip.load_library()
-    if logits.dtype not in _hip.DTYPES:
-        raise TypeError(f"top_logits expects float32, float16 or bfloat16, not {logits.dtype}")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError("logits need at least one class")
-    k = int(k)
-    if not 1 <= k <= _hip.TOP_MAX_K:
-        raise ValueError(f"k={k} outside 1..{_hip.TOP_MAX_K}")
-    rows = logits.detach()
-    shape = rows.shape[:-1]
-    values, idx, lse = _hip.top_logits(rows if rows.dim() == 2 else rows.reshape(-1, rows.shape[-1]), k, temperature)
-    return values.view(*shape, k), idx.view(*shape, k), lse.view(shape)
-
-
-class _TopkDistill(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, idx, top, teacher_lse, temperature, teacher_temperature, reduction):
-        loss, stats, scale = _hip.distill_forward(logits, idx, top, teacher_lse, temperature, teacher_temperature,
-                                                  reduction)
-        ctx.save_for_backward(logits, idx, top, stats, scale)
-        ctx.temperatures = temperature, teacher_temperature
-        return loss
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        logits, idx, top, stats, scale = ctx.saved_tensors
-        return _hip.distill_backward(logits, idx, top, *ctx.temperatures, stats, scale, grad), *[None] * 6
+    return _hip.torch_ops().top_logits(logits, int(k), temperature)
 
 
 def topk_distill(logits, teacher_idx, teacher_logits, temperature=1.0, teacher_lse=None, teacher_temperature=None,
@@ -67,47 +38,14 @@ def topk_distill(logits, teacher_idx, teacher_logits, temperature=1.0, teacher_l
     of padding only, of teacher logits that are all ``-inf`` and of student logits that are all ``-inf`` have loss and
     gradient 0 and are left out.  An index that is no class makes its row's loss and gradient NaN (nothing waits for the GPU
     to raise).  Gradients for ``logits`` alone: the teacher has to be detached."""
-    device = _hip._cuda_device(logits, "logits")
-    _hip.load_library()
-    if logits.dtype not in _hip.DTYPES:
-        raise TypeError(f"topk_distill expects float32, float16 or bfloat16 logits, not {logits.dtype}")
-    if reduction not in _hip.REDUCTIONS:
+    _hip._cuda_device(logits, "logits")
+    number = _hip.REDUCTIONS.get(reduction)
+    if number is None:
         raise ValueError(f"reduction must be one of {sorted(_hip.REDUCTIONS)}")
-    if logits.dim() < 1 or logits.shape[-1] < 1:
-        raise ValueError("logits need at least one class")
-    shape = logits.shape[:-1]
-    for name, t in (("teacher_idx", teacher_idx), ("teacher_logits", teacher_logits), ("teacher_lse", teacher_lse)):
-        if t is None and name == "teacher_lse":
-            continue
-        if _hip._cuda_device(t, name) != device:
-            raise ValueError(f"{name} is on {t.device}, logits on {device}")
-        if t.requires_grad:
-            raise ValueError(f"{name} requires a gradient, which there is none of: detach it")
-        if t.is_floating_point() == (name == "teacher_idx") or t.is_complex() or t.dtype == torch.bool:
-            raise TypeError(f"{name} must not be {t.dtype}")
-    if teacher_idx.shape[:-1] != shape or teacher_idx.dim() != logits.dim() or teacher_idx.shape != teacher_logits.shape:
-        raise ValueError(f"teacher_idx and teacher_logits need one row of k entries per row of logits: {tuple(logits.shape)}, "
-                         f"{tuple(teacher_idx.shape)}, {tuple(teacher_logits.shape)}")
-    k = teacher_idx.shape[-1]
-    if not 1 <= k <= _hip.DISTILL_MAX_K:
-        raise ValueError(f"k={k} outside 1..{_hip.DISTILL_MAX_K}")
-    if teacher_lse is not None and teacher_lse.shape != shape:
-        raise ValueError(f"teacher_lse needs shape {tuple(shape)}, not {tuple(teacher_lse.shape)}")
-    if teacher_idx.dtype != torch.int32:
-        teacher_idx = teacher_idx.clamp(-2, 2147483647).to(torch.int32)    # what is no class stays none
-    idx = teacher_idx.reshape(-1, k).contiguous()
-    top = teacher_logits.reshape(-1, k).to(torch.float32).contiguous()
-    if teacher_lse is not None:
-        teacher_lse = teacher_lse.reshape(-1).to(torch.float32).contiguous()
-    temperature = float(temperature)
-    teacher_temperature = temperature if teacher_temperature is None else float(teacher_temperature)
-    rows = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
-    args = (rows, idx, top, teacher_lse, temperature, teacher_temperature, reduction)
-    if torch.is_grad_enabled() and logits.requires_grad:
-        loss = _TopkDistill.apply(*args)
-    else:
-        loss = _hip.distill_forward(*args)[0]
-    return loss.view(shape) if reduction == "none" else loss
+    if teacher_temperature is None:
+        teacher_temperature = temperature
+    return _hip.torch_ops().topk_distill(logits, teacher_idx, teacher_logits, teacher_lse, temperature, teacher_temperature,
+                                         number)
 
 
 class TopKDistillLoss(nn.Module):
