@@ -78,6 +78,24 @@ __device__ __forceinline__ void act_values(int act, float (&v)[V]) {
     }
 }
 template <typename T, int V>
+__device__ __forceinline__ void slope_values(int act, float (&g)[V], const T (&z)[V]) {
+    switch (act) {
+        case kActRelu:
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[e] *= act_slope(kActRelu, to_f32(z[e]));
+            break;
+        case kActGelu:
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[e] *= act_slope(kActGelu, to_f32(z[e]));
+            break;
+        case kActSilu:
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[e] *= act_slope(kActSilu, to_f32(z[e]));
+            break;
+        default: break;
+    }
+}
+template <typename T, int V>
 __device__ __forceinline__ void add_run(float (&v)[V], const T* __restrict__ p, int count) {
     T in[V];
     if (count >= V) {
@@ -146,7 +164,6 @@ struct TileLds {
         };
         __align__(16) float c[kTile * kTile];
     };
-    float bias_sum[kThreads];
 };
 
 // C leaves through LDS: an accumulator holds one column of four rows a lane, memory wants runs of columns.  A 64 x 64 tile
@@ -176,14 +193,26 @@ __device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long
     }
 }
 
-// piece `piece` of the work on one product: a tile of C, and within it a split of the contraction
-template <typename T, int OP>
-__device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, TileLds<T>& lds) {
+// eight neighbouring elements at p, of which `count` are there
+template <typename T>
+__device__ __forceinline__ void load_run(T (&v)[8], const T* __restrict__ p, long long count) {
+    if (count >= 8) {
+        __builtin_memcpy(v, p, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = e < count ? p[e] : T(0);
+    }
+}
+
+// Piece `piece` of the work on one product: a tile of C, and within it a split of the contraction.  A group of four waves
+// makes a 64 x 64 tile, each wave a quarter, in steps of 32 along the contraction, fetched one step ahead.  Where the
+// pieces are too few to fill the chip, G groups share one: every G-th step each, added up in their order.
+template <typename T, int OP, int G>
+__device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, TileLds<T>* lds) {
     constexpr int LD = Lds<T>::LD;
-    constexpr int NV = kTile * kDepth / kThreads;   // elements of a tile per thread
-    T *as = lds.a, *bs = lds.b;
-    float* bias_sum = lds.bias_sum;
-    const int t = threadIdx.x, lane = t & 63, wave = wave_id();
+    const int group = G == 1 ? 0 : wave_id() / 4, wave = wave_id() % 4;
+    const int t = threadIdx.x % kThreads, lane = t & 63;
+    T *as = lds[group].a, *bs = lds[group].b;
     const unsigned split = piece / p.tiles, tile = piece - split * p.tiles, tile_j = tile / p.tiles_i;
     const long long i0 = (long long)(tile - tile_j * p.tiles_i) * kTile, j0 = (long long)tile_j * kTile;
     const long long c_lo = (long long)split * p.split_len;
@@ -193,54 +222,66 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
     const T* __restrict__ z = static_cast<const T*>(p.z);
     const T* __restrict__ dy = static_cast<const T*>(p.dy);
 
-    // this thread's elements: along the contraction (32 threads a row) or across it (64 threads a column)
+    // This thread's eight elements of each operand's step: along the contraction, four threads a row, or
+    // across it, eight threads a column, whichever way they lie next to each other.
     constexpr bool kAlongA = OP != kDw, kAlongB = OP == kForward;
-    const int ca = kAlongA ? (t & 31) : (t >> 6), ra = kAlongA ? (t >> 5) : (t & 63);
-    const int cb = kAlongB ? (t & 31) : (t >> 6), rb = kAlongB ? (t >> 5) : (t & 63);
-    constexpr int kStepRA = kAlongA ? 8 : 0, kStepCA = kAlongA ? 0 : 4;
-    constexpr int kStepRB = kAlongB ? 8 : 0, kStepCB = kAlongB ? 0 : 4;
+    const int ca = kAlongA ? (t & 3) * 8 : t >> 3, ra = kAlongA ? t >> 2 : (t & 7) * 8;
+    const int cb = kAlongB ? (t & 3) * 8 : t >> 3, rb = kAlongB ? t >> 2 : (t & 7) * 8;
 
-    T va[NV], vb[NV];
-    float dsum = 0.f;
+    T va[8], vb[8];
+    float dsum[8] = {};
     auto load = [&](long long c0) {
+        {
+            const long long r = i0 + ra, c = c0 + ca;
+            const bool there = r < p.rows && c < c_hi;
+            const long long count = there ? (kAlongA ? c_hi - c : p.rows - r) : 0;
+            if constexpr (OP == kForward) {
+                load_run<T>(va, a + r * p.lda + c, count);
+            } else {
+                const long long at = OP == kDx ? r * p.n + c : c * p.n + r;
+                load_run<T>(va, dy + at, count);
+                float g[8];
 #pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            const long long r = i0 + ra + q * kStepRA, c = c0 + ca + q * kStepCA;
-            T v = T(0);
-            if (r < p.rows && c < c_hi) {
-                if (OP == kForward) {
-                    v = a[r * p.lda + c];
-                } else {
-                    const long long at = OP == kDx ? r * p.n + c : c * p.n + r;
-                    float g = to_f32(dy[at]);
-                    if (p.act != kActNone) g *= act_slope(p.act, to_f32(z[at]));
-                    if (OP == kDw) dsum += g;
-                    v = from_f32<T>(g);
+                for (int e = 0; e < 8; ++e) g[e] = to_f32(va[e]);
+                if (p.act != kActNone) {
+                    T vz[8];
+                    load_run<T>(vz, z + at, count);
+                    slope_values(p.act, g, vz);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) va[e] = from_f32<T>(g[e]);
+                }
+                if (OP == kDw) {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) dsum[e] += g[e];
                 }
             }
-            va[q] = v;
         }
-#pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            const long long r = j0 + rb + q * kStepRB, c = c0 + cb + q * kStepCB;
-            T v = T(0);
-            if (b && r < p.cols && c < c_hi) v = kAlongB ? b[r * p.ldb + c] : b[c * p.ldb + r];
-            vb[q] = v;
+        {
+            const long long r = j0 + rb, c = c0 + cb;
+            const long long count = b && r < p.cols && c < c_hi ? (kAlongB ? c_hi - c : p.cols - r) : 0;
+            load_run<T>(vb, b + (kAlongB ? r * p.ldb + c : c * p.ldb + r), count);
         }
     };
 
     f32x16 acc = {};
     const int wr = (wave & 1) * 32 + (lane & 31), wc = (wave >> 1) * 32 + (lane & 31), half = lane >> 5;
-    load(c_lo);
-    for (long long c0 = c_lo; c0 < c_hi; c0 += kDepth) {
+    load(c_lo + group * kDepth);
+    for (long long c0 = c_lo; c0 < c_hi; c0 += G * kDepth) {
         __syncthreads();
+        if constexpr (kAlongA) {
+            __builtin_memcpy(__builtin_assume_aligned(as + ra * LD + ca, 16), va, sizeof(va));
+        } else {
 #pragma unroll
-        for (int q = 0; q < NV; ++q) {
-            as[(ra + q * kStepRA) * LD + ca + q * kStepCA] = va[q];
-            bs[(rb + q * kStepRB) * LD + cb + q * kStepCB] = vb[q];
+            for (int e = 0; e < 8; ++e) as[(ra + e) * LD + ca] = va[e];
+        }
+        if constexpr (kAlongB) {
+            __builtin_memcpy(__builtin_assume_aligned(bs + rb * LD + cb, 16), vb, sizeof(vb));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) bs[(rb + e) * LD + cb] = vb[e];
         }
         __syncthreads();
-        if (c0 + kDepth < c_hi) load(c0 + kDepth);
+        if (c0 + G * kDepth < c_hi) load(c0 + (G + group) * kDepth);
         if constexpr (sizeof(T) == 4) {
             // the two halves of the wave take four neighbouring steps of the contraction each: any order of them
             // gives the same sum of products, and this one reads 16 bytes a lane
@@ -267,44 +308,59 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
         }
     }
 
+    const int all = threadIdx.x;
+    if (OP == kDw && p.dbias && tile_j == 0) {   // rows of C are the outputs: their sums of dz, from 32 threads of every group
+        __syncthreads();
+        float* s = lds[group].c;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s[ca * kTile + ra + e] = dsum[e];
+        __syncthreads();
+        if (all < kTile && i0 + all < p.rows) {
+            float sum = 0.f;
+            for (int g = 0; g < G; ++g)
+                for (int c = 0; c < kDepth; ++c) sum += lds[g].c[c * kTile + all];
+            if (p.splits > 1)
+                p.part_bias[(long long)split * p.rows + i0 + all] = sum;
+            else
+                static_cast<T*>(p.dbias)[i0 + all] = from_f32<T>(sum);
+        }
+    }
     __syncthreads();     // the operands' tiles are read: C's 64 x 64 values take their place
-    float* c = lds.c;
-    put_quadrant(acc, c, wave & 1, wave >> 1);
+    put_quadrant(acc, lds[group].c, wave & 1, wave >> 1);
     __syncthreads();
+    float* c = lds[0].c;
+    if (G > 1) {
+        for (int e = all * 4; e < kTile * kTile; e += G * kThreads * 4) {
+            f32x4 v = *reinterpret_cast<const f32x4*>(c + e);
+#pragma unroll
+            for (int g = 1; g < G; ++g) v += *reinterpret_cast<const f32x4*>(lds[g].c + e);
+            *reinterpret_cast<f32x4*>(c + e) = v;
+        }
+        __syncthreads();
+    }
     if (p.splits > 1) {
-        for (int e = t; e < kTile * kTile; e += kThreads) {
+        for (int e = all; e < kTile * kTile; e += G * kThreads) {
             const long long i = i0 + (e >> 6), j = j0 + (e & 63);
             if (i < p.rows && j < p.cols) p.part[((long long)split * p.rows + i) * p.cols + j] = c[place(e >> 6, e & 63)];
         }
     } else if (p.out) {
-        tile_out<T, OP>(p, c, i0, j0, t, kThreads);
-    }
-    if (OP == kDw && p.dbias && tile_j == 0) {   // rows of C are the outputs: their sums of dz, four partial sums each
-        bias_sum[t] = dsum;
-        __syncthreads();
-        if (t < kTile && i0 + t < p.rows) {
-            const float s = (bias_sum[t] + bias_sum[t + 64]) + (bias_sum[t + 128] + bias_sum[t + 192]);
-            if (p.splits > 1)
-                p.part_bias[(long long)split * p.rows + i0 + t] = s;
-            else
-                static_cast<T*>(p.dbias)[i0 + t] = from_f32<T>(s);
-        }
+        tile_out<T, OP>(p, c, i0, j0, all, G * kThreads);
     }
 }
 
-template <typename T>
-__global__ __launch_bounds__(kThreads) void linear_tile_forward_kernel(TileArgs p) {
-    __shared__ TileLds<T> lds;
-    tile_product<T, kForward>(p, blockIdx.x, lds);
+template <typename T, int G>
+__global__ __launch_bounds__(kThreads* G) void linear_tile_forward_kernel(TileArgs p) {
+    __shared__ TileLds<T> lds[G];
+    tile_product<T, kForward, G>(p, blockIdx.x, lds);
 }
 // both products of the backward pass in one launch, the first pieces_dx blocks on dx
-template <typename T>
-__global__ __launch_bounds__(kThreads) void linear_tile_backward_kernel(TileArgs dx, unsigned pieces_dx, TileArgs dw) {
-    __shared__ TileLds<T> lds;
+template <typename T, int G>
+__global__ __launch_bounds__(kThreads* G) void linear_tile_backward_kernel(TileArgs dx, unsigned pieces_dx, TileArgs dw) {
+    __shared__ TileLds<T> lds[G];
     if (blockIdx.x < pieces_dx)
-        tile_product<T, kDx>(dx, blockIdx.x, lds);
+        tile_product<T, kDx, G>(dx, blockIdx.x, lds);
     else
-        tile_product<T, kDw>(dw, blockIdx.x - pieces_dx, lds);
+        tile_product<T, kDw, G>(dw, blockIdx.x - pieces_dx, lds);
 }
 
 // Joins the splits of the contraction, in their order.
@@ -313,6 +369,7 @@ __device__ __forceinline__ void join_splits(const TileArgs& p) {
     const long long total = p.rows * p.cols;
     for (long long e = (long long)blockIdx.x * kThreads + threadIdx.x; e < total; e += (long long)gridDim.x * kThreads) {
         float s = 0.f;
+#pragma unroll 8
         for (int q = 0; q < p.splits; ++q) s += p.part[q * total + e];
         float v[1] = {s};
         if (OP == kForward)
@@ -341,6 +398,11 @@ inline unsigned join_blocks(long long elements) {
     const long long blocks = ceil_div(elements, kThreads);
     return (unsigned)(blocks < 4096 ? blocks : 4096);
 }
+
+// Up to this many pieces, four groups of waves share each: there is room on the chip for all of them, and a piece's
+// steps, each as long as a fetch from memory takes, become a quarter.
+constexpr unsigned kFewPieces = 256;
+constexpr int kGroups = 4;
 
 // Pieces of the contraction: enough blocks to give every compute unit two, none of them shorter than 256.
 void plan_tiles(long long rows, long long cols, long long depth, int& splits, long long& len) {
@@ -1011,7 +1073,10 @@ hipError_t forward_t(const LinearArgs& a, void* y, void* z, void* ws, hipStream_
     if (has_few_rows(a.m, a.n, a.k)) return run_few_rows<T>(p, stream);
     if (is_large(a.m, a.n, a.k)) return forward_large<T>(a, p, ws, stream);
     const unsigned pieces = set_tiles(p, ws);
-    linear_tile_forward_kernel<T><<<dim3(pieces), kThreads, 0, stream>>>(p);
+    if (pieces <= kFewPieces)
+        linear_tile_forward_kernel<T, kGroups><<<dim3(pieces), kThreads * kGroups, 0, stream>>>(p);
+    else
+        linear_tile_forward_kernel<T, 1><<<dim3(pieces), kThreads, 0, stream>>>(p);
     if (p.splits > 1) linear_join_kernel<T, kForward><<<dim3(join_blocks(p.rows * p.cols)), kThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
@@ -1039,7 +1104,10 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
         pieces_dw = set_tiles(q, ws + backward_dx_bytes(a.m, a.n, a.k, a.dtype));
     }
     if (pieces_dx + pieces_dw == 0) return hipGetLastError();
-    linear_tile_backward_kernel<T><<<dim3(pieces_dx + pieces_dw), kThreads, 0, stream>>>(p, pieces_dx, q);
+    if (pieces_dx + pieces_dw <= kFewPieces)
+        linear_tile_backward_kernel<T, kGroups><<<dim3(pieces_dx + pieces_dw), kThreads * kGroups, 0, stream>>>(p, pieces_dx, q);
+    else
+        linear_tile_backward_kernel<T, 1><<<dim3(pieces_dx + pieces_dw), kThreads, 0, stream>>>(p, pieces_dx, q);
     if (pieces_dx == 0) p.splits = 1;      // (its own launches have joined it)
     if (p.splits > 1 || q.splits > 1) {
         const long long ex = p.splits > 1 ? p.rows * p.cols : 0, ew = q.splits > 1 ? q.rows * q.cols : 0;
