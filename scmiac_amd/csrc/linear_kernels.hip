@@ -95,15 +95,20 @@ __device__ __forceinline__ void slope_values(int act, float (&g)[V], const T (&z
         default: break;
     }
 }
+// V neighbouring elements at p, of which `count` are there
+template <typename T, int V>
+__device__ __forceinline__ void take_run(T (&v)[V], const T* __restrict__ p, long long count) {
+    if (count >= V) {
+        __builtin_memcpy(v, p, sizeof(v));
+    } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] = e < count ? p[e] : T(0);
+    }
+}
 template <typename T, int V>
 __device__ __forceinline__ void add_run(float (&v)[V], const T* __restrict__ p, int count) {
     T in[V];
-    if (count >= V) {
-        __builtin_memcpy(in, p, sizeof(in));
-    } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e) in[e] = e < count ? p[e] : T(0);
-    }
+    take_run<T, V>(in, p, count);
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] += to_f32(in[e]);
 }
@@ -120,16 +125,29 @@ __device__ __forceinline__ void store_run(const float (&v)[V], T* __restrict__ p
             if (e < count) p[e] = out[e];
     }
 }
-// v: z without the bias, columns [j, j + count) of row i (count <= V)
+// v: z without the bias, columns [j, j + count) of row i (count <= V); `added`: the residual there, if there is one
+template <typename T, int V>
+__device__ __forceinline__ void forward_run(float (&v)[V], const float (&bias)[V], bool has_residual, const T (&added)[V], long long at,
+                                            int count, int act, T* __restrict__ y, T* __restrict__ zk) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] += bias[e];
+    if (zk) store_run<T, V, true>(v, zk + at, count);
+    act_values<V>(act, v);
+    if (has_residual) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) v[e] += to_f32(added[e]);
+    }
+    store_run<T, V>(v, y + at, count);
+}
 template <typename T, int V>
 __device__ __forceinline__ void forward_out(float (&v)[V], long long i, long long j, int count, long long n, int act,
                                             const T* __restrict__ bias, const T* __restrict__ residual, long long ldr,
                                             T* __restrict__ y, T* __restrict__ zk) {
-    if (bias) add_run<T, V>(v, bias + j, count);
-    if (zk) store_run<T, V, true>(v, zk + i * n + j, count);
-    act_values<V>(act, v);
-    if (residual) add_run<T, V>(v, residual + i * ldr + j, count);
-    store_run<T, V>(v, y + i * n + j, count);
+    float b[V] = {};
+    T added[V];
+    if (bias) add_run<T, V>(b, bias + j, count);
+    if (residual) take_run<T, V>(added, residual + i * ldr + j, count);
+    forward_run<T, V>(v, b, residual != nullptr, added, i * n + j, count, act, y, zk);
 }
 
 // ------------------------------------------------------------------ 64 x 64 tiles, any shape
@@ -175,32 +193,41 @@ __device__ __forceinline__ void put_quadrant(const f32x16& acc, float* c, int qi
 #pragma unroll
     for (int r = 0; r < 16; ++r) c[place(qi * 32 + 8 * (r >> 2) + 4 * half + (r & 3), qj * 32 + (lane & 31))] = acc[r];
 }
-// a 64 x 64 tile from LDS through the epilogue, eight columns at a time, by `threads` threads
-template <typename T, int OP>
-__device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long long i0, long long j0, int t, int threads) {
-    for (int e = t; e < kTile * 8; e += threads) {
-        const int row = e >> 3, col = (e & 7) * 8;
-        const long long i = i0 + row, j = j0 + col;
-        if (i >= p.rows || j >= p.cols) continue;
-        const int count = (int)min(8ll, p.cols - j);
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(c + place(row, col)), hi = *reinterpret_cast<const f32x4*>(c + place(row, col + 4));
-        float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        if (OP == kForward)
-            forward_out<T, 8>(v, i, j, count, p.n, p.act, static_cast<const T*>(p.bias), static_cast<const T*>(p.residual), p.ldr,
-                              static_cast<T*>(p.out), static_cast<T*>(p.keep));
-        else
-            store_run<T, 8>(v, static_cast<T*>(p.out) + i * p.cols + j, count);
-    }
-}
-
-// eight neighbouring elements at p, of which `count` are there
-template <typename T>
-__device__ __forceinline__ void load_run(T (&v)[8], const T* __restrict__ p, long long count) {
-    if (count >= 8) {
-        __builtin_memcpy(v, p, sizeof(v));
-    } else {
+// A 64 x 64 tile from LDS through the epilogue, eight columns at a time, by kT threads: the same columns every time, so
+// that the bias is fetched once, and the residuals of a few rows are fetched before any of them is used.
+template <typename T, int OP, int kT>
+__device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long long i0, long long j0, int t) {
+    constexpr int kRuns = (kTile * 8 + kT - 1) / kT, kBatch = kRuns < 4 ? kRuns : 4;
+    const int col = (t & 7) * 8;
+    const long long j = j0 + col;
+    if (j >= p.cols || t >= kTile * 8) return;
+    const int count = (int)min(8ll, p.cols - j);
+    float bias[8] = {};
+    if (OP == kForward && p.bias) add_run<T, 8>(bias, static_cast<const T*>(p.bias) + j, count);
+    const T* residual = OP == kForward ? static_cast<const T*>(p.residual) : nullptr;
+#pragma unroll 1
+    for (int r0 = 0; r0 < kRuns; r0 += kBatch) {
+        T added[kBatch][8];
+        if (residual) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < count ? p[e] : T(0);
+            for (int u = 0; u < kBatch; ++u) {
+                const long long i = i0 + ((t + (r0 + u) * kT) >> 3);
+                take_run<T, 8>(added[u], residual + i * p.ldr + j, i < p.rows ? count : 0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+            const int row = (t + (r0 + u) * kT) >> 3;
+            const long long i = i0 + row;
+            if (i >= p.rows) continue;
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(c + place(row, col)), hi = *reinterpret_cast<const f32x4*>(c + place(row, col + 4));
+            float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            if (OP == kForward)
+                forward_run<T, 8>(v, bias, residual != nullptr, added[u], i * p.n + j, count, p.act, static_cast<T*>(p.out),
+                                  static_cast<T*>(p.keep));
+            else
+                store_run<T, 8>(v, static_cast<T*>(p.out) + i * p.cols + j, count);
+        }
     }
 }
 
@@ -236,16 +263,16 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
             const bool there = r < p.rows && c < c_hi;
             const long long count = there ? (kAlongA ? c_hi - c : p.rows - r) : 0;
             if constexpr (OP == kForward) {
-                load_run<T>(va, a + r * p.lda + c, count);
+                take_run<T, 8>(va, a + r * p.lda + c, count);
             } else {
                 const long long at = OP == kDx ? r * p.n + c : c * p.n + r;
-                load_run<T>(va, dy + at, count);
+                take_run<T, 8>(va, dy + at, count);
                 float g[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) g[e] = to_f32(va[e]);
                 if (p.act != kActNone) {
                     T vz[8];
-                    load_run<T>(vz, z + at, count);
+                    take_run<T, 8>(vz, z + at, count);
                     slope_values(p.act, g, vz);
 #pragma unroll
                     for (int e = 0; e < 8; ++e) va[e] = from_f32<T>(g[e]);
@@ -259,7 +286,7 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
         {
             const long long r = j0 + rb, c = c0 + cb;
             const long long count = b && r < p.cols && c < c_hi ? (kAlongB ? c_hi - c : p.cols - r) : 0;
-            load_run<T>(vb, b + (kAlongB ? r * p.ldb + c : c * p.ldb + r), count);
+            take_run<T, 8>(vb, b + (kAlongB ? r * p.ldb + c : c * p.ldb + r), count);
         }
     };
 
@@ -344,7 +371,7 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
             if (i < p.rows && j < p.cols) p.part[((long long)split * p.rows + i) * p.cols + j] = c[place(e >> 6, e & 63)];
         }
     } else if (p.out) {
-        tile_out<T, OP>(p, c, i0, j0, all, G * kThreads);
+        tile_out<T, OP, G * kThreads>(p, c, i0, j0, all);
     }
 }
 
@@ -568,8 +595,10 @@ __global__ __launch_bounds__(kThreads) void linear_few_rows_dx_kernel(TileArgs p
 }
 
 constexpr long long kMaxFewCols = 1 << 22;   // splits of dx fit a grid's second dimension
-// From 2^18 weights on; below that a launch of 64 x 64 tiles is as short.
-bool has_few_rows(long long m, long long n, long long k) { return m >= 1 && m <= kFewRows && n <= kMaxFewCols && n * k >= (1 << 18); }
+bool has_few_rows(long long m, long long n) { return m >= 1 && m <= kFewRows && n <= kMaxFewCols; }
+// dx goes that way from 2^18 weights on: with fewer, its splits and their join cost more than one launch of tiles for dx
+// and dw together (6 rows, 272 -> 172 in float32: 35 us against 24 for the whole pass).
+bool has_few_rows_dx(long long m, long long n, long long k) { return has_few_rows(m, n) && n * k >= (1 << 18); }
 
 void plan_few_dx(long long n, long long k, int esize, int& splits, long long& len) {
     const long long groups = ceil_div(k, 64 * (16 / esize));
@@ -618,9 +647,9 @@ hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
 //
 // C[i, j] = sum_c A[i, c] B[j, c] on 16-bit operands whose rows are padded to whole 128-byte lines (64 elements).  A block
 // owns a BM x BN tile; its operands pass through LDS in steps of 64 along the contraction, two buffers deep,
-// written by the memory pipe itself (16 bytes a lane, no registers).  Such a write lands lane after lane, eight
-// 16-byte chunks a row, and reading one chunk column of 32 rows would hit the same banks every time;
-// so lane l fetches chunk (l % 8) ^ (row % 8) of its row, and the reads look it up there.
+// written by the memory pipe itself (16 bytes a lane, no registers).  Such a write lands lane after lane, row after
+// row, and reading one chunk column of 32 rows would hit the same banks every time; so a lane fetches
+// the chunk that belongs there once rows are turned against each other, and the reads look it up.
 //
 // float32 operands come as three bf16 planes whose sum is the value to 2^-25 or better: the product is
 // the six products of planes that matter (the other three are below 2^-24 of the result), run as one
@@ -635,7 +664,7 @@ struct GemmArgs {
     long long lda, ldb;              // elements
     long long plane_a, plane_b;      // elements between planes
     long long rows, cols;
-    int k_blocks;                    // 64-wide steps of one plane pair
+    int depth;                       // padded length of the contraction, of one plane pair
     int pairs;                       // 1, or kPairs
     int splits, split_len;           // in steps
     unsigned tiles_i, tiles_j;
@@ -659,18 +688,28 @@ struct Frag<f16> {
     }
 };
 
+// Which chunk of row r lies where chunk 0 would: eight rows' chunks of one number cover all banks once.
+__device__ __forceinline__ int swizzle(int r) { return r & 7; }
+
 // 64 lanes x 16 bytes from global memory to LDS at `lds` + 16 lane
 __device__ __forceinline__ void load_to_lds(const void* g, char* lds) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
                                      (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
+// none of the wave's memory operations and LDS reads under way; then all waves
+__device__ __forceinline__ void wait_and_meet() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+}
+
 template <typename T16, typename OutT, int BM, int BN, int WM, int WN, int OP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel(GemmArgs p) {
     constexpr int kWavesN = BN / WN, kWavesAll = (BM / WM) * kWavesN;
     constexpr int FA = WM / 32, FB = WN / 32;
-    constexpr int kLoadsA = BM / 8 / kWavesAll, kLoadsB = BN / 8 / kWavesAll;
-    constexpr int kBytesA = BM * kBK * 2, kBytes = (BM + BN) * kBK * 2;
+    constexpr int BK = kBK, kRow = BK * 2, kChunks = kRow / 16, kRowsPer = 64 / kChunks;     // bytes, chunks of a row; rows of one load
+    constexpr int kLoadsA = BM / kRowsPer / kWavesAll, kLoadsB = BN / kRowsPer / kWavesAll;
+    constexpr int kBytesA = BM * kRow, kBytes = (BM + BN) * kRow;
     __shared__ __align__(128) char lds[2 * kBytes];
     typedef typename Frag<T16>::type frag;
     const int lane = threadIdx.x & 63, wave = wave_id();
@@ -686,36 +725,37 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
     id %= group;
     const unsigned ti = first + id % high, tj = id / high;
     const long long i0 = (long long)ti * BM, j0 = (long long)tj * BN;
-    const int s_lo = blockIdx.y * p.split_len, s_hi = min(p.k_blocks * p.pairs, s_lo + p.split_len);
+    const int k_blocks = p.depth / BK;
+    const int s_lo = blockIdx.y * p.split_len, s_hi = min(k_blocks * p.pairs, s_lo + p.split_len);
 
     // byte offsets of this lane's pieces within the tile's rows (rows behind the last one repeat it: what
     // they give is not written)
-    const int chunk = ((lane & 7) ^ (lane >> 3)) * 16;
+    const int piece_row = lane / kChunks, chunk = ((lane % kChunks) ^ swizzle(piece_row)) * 16;
     const char* base_a = reinterpret_cast<const char*>(p.a) + i0 * p.lda * 2;
     const char* base_b = reinterpret_cast<const char*>(p.b) + j0 * p.ldb * 2;
     unsigned off_a[kLoadsA], off_b[kLoadsB];
     const int rows_left = (int)min((long long)BM, p.rows - i0), cols_left = (int)min((long long)BN, p.cols - j0);
 #pragma unroll
     for (int q = 0; q < kLoadsA; ++q)
-        off_a[q] = (unsigned)min((q * kWavesAll + wave) * 8 + (lane >> 3), rows_left - 1) * (unsigned)(p.lda * 2) + chunk;
+        off_a[q] = (unsigned)min((q * kWavesAll + wave) * kRowsPer + piece_row, rows_left - 1) * (unsigned)(p.lda * 2) + chunk;
 #pragma unroll
     for (int q = 0; q < kLoadsB; ++q)
-        off_b[q] = (unsigned)min((q * kWavesAll + wave) * 8 + (lane >> 3), cols_left - 1) * (unsigned)(p.ldb * 2) + chunk;
+        off_b[q] = (unsigned)min((q * kWavesAll + wave) * kRowsPer + piece_row, cols_left - 1) * (unsigned)(p.ldb * 2) + chunk;
 
     auto stage = [&](int step, int buf) {
         long long oa = 0, ob = 0;
         int kb = step;
         if (p.pairs > 1) {
-            const int pair = step / p.k_blocks;
-            kb -= pair * p.k_blocks;
+            const int pair = step / k_blocks;
+            kb -= pair * k_blocks;
             // the small products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
             const int pa = (pair == 0) ? 2 : (pair == 2 || pair == 3) ? 1 : 0;
             const int pb = (pair == 1) ? 2 : (pair == 2 || pair == 4) ? 1 : 0;
             oa = pa * p.plane_a * 2;
             ob = pb * p.plane_b * 2;
         }
-        const char* ga = base_a + oa + (long long)kb * (kBK * 2);
-        const char* gb = base_b + ob + (long long)kb * (kBK * 2);
+        const char* ga = base_a + oa + (long long)kb * kRow;
+        const char* gb = base_b + ob + (long long)kb * kRow;
         char* to = lds + buf * kBytes + wave * 1024;
 #pragma unroll
         for (int q = 0; q < kLoadsA; ++q) load_to_lds(ga + off_a[q], to + q * kWavesAll * 1024);
@@ -725,22 +765,22 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
 
     f32x16 acc[FA][FB] = {};
     const int half = lane >> 5, l31 = lane & 31;
-    const int row_a = (wm + l31) * 128, row_b = kBytesA + (wn + l31) * 128;
+    const int row_a = (wm + l31) * kRow, row_b = kBytesA + (wn + l31) * kRow;
+    // while one buffer is read, the next step is on its way to the other, which every wave has done with when they meet
     int buf = 0;
     stage(s_lo, 0);
     for (int step = s_lo; step < s_hi; ++step) {
-        __builtin_amdgcn_s_waitcnt(0x0f70);      // vmcnt(0): this step's tiles have landed (this wave's share)
-        __syncthreads();                         // everybody's have, and nobody reads the other buffer any more
+        wait_and_meet();     // this step's tiles have landed: this wave's share of them, then everybody's
         if (step + 1 < s_hi) stage(step + 1, buf ^ 1);
         const char* from = lds + buf * kBytes;
 #pragma unroll
-        for (int kk = 0; kk < kBK / 16; ++kk) {
-            const int at = ((2 * kk + half) ^ (lane & 7)) * 16;
+        for (int kk = 0; kk < BK / 16; ++kk) {
+            const int at = ((2 * kk + half) ^ swizzle(l31)) * 16;
             frag fa[FA], fb[FB];
 #pragma unroll
-            for (int f = 0; f < FA; ++f) fa[f] = *reinterpret_cast<const frag*>(from + row_a + at + f * 4096);
+            for (int f = 0; f < FA; ++f) fa[f] = *reinterpret_cast<const frag*>(from + row_a + at + f * 32 * kRow);
 #pragma unroll
-            for (int f = 0; f < FB; ++f) fb[f] = *reinterpret_cast<const frag*>(from + row_b + at + f * 4096);
+            for (int f = 0; f < FB; ++f) fb[f] = *reinterpret_cast<const frag*>(from + row_b + at + f * 32 * kRow);
 #pragma unroll
             for (int f = 0; f < FA; ++f)
 #pragma unroll
@@ -763,17 +803,19 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
             }
         return;
     }
-    static_assert(WN == 64 && WM % 64 == 0 && kWavesAll * kTile * kTile * 4 <= 2 * kBytes, "a 64 x 64 tile of LDS for every wave");
+    static_assert(WN % 64 == 0 && WM % 64 == 0 && kWavesAll * kTile * kTile * 4 <= 2 * kBytes, "a 64 x 64 tile of LDS for every wave");
     __syncthreads();                             // the operands are read: the room is each wave's own now
     float* c = reinterpret_cast<float*>(lds) + wave * (kTile * kTile);
 #pragma unroll
-    for (int m = 0; m < WM / 64; ++m) {
-        wave_lds_fence();
+    for (int m = 0; m < WM / 64; ++m)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) put_quadrant(acc[2 * m + (q >> 1)][q & 1], c, q >> 1, q & 1);
-        wave_lds_fence();
-        tile_out<OutT, OP>(p.t, c, i0 + wm + m * 64, j0 + wn, lane, 64);
-    }
+        for (int n = 0; n < WN / 64; ++n) {
+            wave_lds_fence();
+#pragma unroll
+            for (int q = 0; q < 4; ++q) put_quadrant(acc[2 * m + (q >> 1)][2 * n + (q & 1)], c, q >> 1, q & 1);
+            wave_lds_fence();
+            tile_out<OutT, OP, 64>(p.t, c, i0 + wm + m * 64, j0 + wn + n * 64, lane);
+        }
 }
 
 // An operand of the large products from a matrix src [rows, cols] (or from dz = dy act'(z), given as src = dy and z):
@@ -945,7 +987,7 @@ hipError_t run_gemm(const void* a, long long lda, long long plane_a, const void*
     const GemmPlan g = plan_gemm(rows, cols, depth_padded, sizeof(T) == 4 ? kPairs : 1);
     GemmArgs p = {};
     p.a = a, p.b = b, p.lda = lda, p.ldb = ldb, p.plane_a = plane_a, p.plane_b = plane_b;
-    p.rows = rows, p.cols = cols, p.k_blocks = (int)(depth_padded / kBK), p.pairs = sizeof(T) == 4 ? kPairs : 1;
+    p.rows = rows, p.cols = cols, p.depth = (int)depth_padded, p.pairs = sizeof(T) == 4 ? kPairs : 1;
     p.splits = g.splits, p.split_len = g.split_len, p.tiles_i = g.tiles_i, p.tiles_j = g.tiles_j;
     t.part = static_cast<float*>(part);
     t.rows = rows, t.cols = cols, t.splits = g.splits;
@@ -1059,7 +1101,7 @@ hipError_t backward_large(const LinearArgs& a, const void* z, const void* dy, vo
 
 // scratch of dx in front of that of dw, where neither goes through the large tiles
 size_t backward_dx_bytes(long long m, long long n, long long k, int dtype) {
-    const size_t bytes = has_few_rows(m, n, k) ? few_dx_bytes(m, n, k, dtype == 0 ? 4 : 2) : tile_bytes(m, k, n);
+    const size_t bytes = has_few_rows_dx(m, n, k) ? few_dx_bytes(m, n, k, dtype == 0 ? 4 : 2) : tile_bytes(m, k, n);
     return (bytes + 255) & ~(size_t)255;
 }
 
@@ -1070,7 +1112,7 @@ hipError_t forward_t(const LinearArgs& a, void* y, void* z, void* ws, hipStream_
     p.bias = a.bias, p.residual = a.residual, p.ldr = a.ldr;
     p.rows = a.m, p.cols = a.n, p.depth = a.k, p.n = a.n, p.act = a.act;
     p.out = y, p.keep = z;
-    if (has_few_rows(a.m, a.n, a.k)) return run_few_rows<T>(p, stream);
+    if (has_few_rows(a.m, a.n)) return run_few_rows<T>(p, stream);
     if (is_large(a.m, a.n, a.k)) return forward_large<T>(a, p, ws, stream);
     const unsigned pieces = set_tiles(p, ws);
     if (pieces <= kFewPieces)
@@ -1092,7 +1134,7 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
     unsigned pieces_dx = 0, pieces_dw = 0;
     if (dx) {
         p.b = a.w, p.ldb = a.ldw, p.rows = a.m, p.cols = a.k, p.depth = a.n, p.out = dx;
-        if (has_few_rows(a.m, a.n, a.k)) {
+        if (has_few_rows_dx(a.m, a.n, a.k)) {
             if (hipError_t e = run_few_rows_dx<T>(p, ws, stream)) return e;
         } else {
             pieces_dx = set_tiles(p, ws);
@@ -1121,7 +1163,7 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
 size_t linear_workspace_bytes(long long m, long long n, long long k, int dtype, int act, int backward) {
     (void)act;
     if (is_large(m, n, k)) return carve_big(m, n, k, dtype, backward).total;
-    if (!backward) return has_few_rows(m, n, k) ? 0 : tile_bytes(m, n, k);
+    if (!backward) return has_few_rows(m, n) ? 0 : tile_bytes(m, n, k);
     const size_t dw = tile_bytes(n, k, m), bias = tile_bytes(n, 1, m);      // (dbias alone is cut up by itself)
     return backward_dx_bytes(m, n, k, dtype) + (dw > bias ? dw : bias);
 }
