@@ -211,8 +211,7 @@ def knn_kept_fraction(q, r, k, *, groups=AUTO_PROBE_GROUPS, group_rows=None):
         group_rows = knn_grid_plan(n, m, q.shape[1], k, mode="pruned")["queries_per_block"]
     group_rows = max(1, min(group_rows, n))
     centres = q[torch.arange(groups, device=q.device) * (n // groups) + n // (2 * groups)]
-    # |q - c|^2 - |c|^2, a row per centre: q is read once for all of them
-    score = torch_ops().linear_act(-2.0 * centres, q, (q * q).sum(1), None, ACTIVATIONS["none"])
+    score = (q * q).sum(1)[None, :] - 2.0 * (centres @ q.T)                # |q - c|^2 - |c|^2, a row per centre
     # a radius that holds the clump with room to spare, read off at most 65 536 evenly spaced
     # queries, so that the exact selection runs over a few thousand rows instead of all
     pool = score[:, ::max(1, n // AUTO_PROBE_POOL)] if n > AUTO_PROBE_POOL else score

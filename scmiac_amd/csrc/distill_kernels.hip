@@ -618,7 +618,7 @@ __global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k,
 // ------------------------------------------------------------------ distillation
 
 // What a row's forward pass leaves for its backward pass, and for the loss:
-//   x = the student's maximum m,  y = tau / s, so that tau p_j = y exp2((x_j - m) c): 0 for a row without a teacher (or
+//   x = the student's maximum m,  y = tau / s, so that tau p_j = y exp2((x_j - m) c): -1 for a row without a teacher (or
 //   without a class), NaN for a row with an index that is none;
 //   z, w: t_i = exp2((a_i - z) ca - w), the teacher's maximum and log of its sum, or its own normaliser and 0
 __device__ __forceinline__ float teacher_weight(float a, float ca, float ref, float log_sum) {
@@ -677,7 +677,7 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ xr, long long v
     }
     if (lane == 0) {
         float value = empty ? 0.f : kLn2 * fmaf(tau, log2f(acc.s), part);
-        float share = empty ? 0.f : tau / acc.s;
+        float share = empty ? -1.f : tau / acc.s;
         if (bad || acc.s != acc.s) value = share = NAN;
         loss[row] = value;
         stats[row] = make_float4(acc.r, share, ref, log_sum);
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* _
     int count = 0;
     for (long long i = threadIdx.x; i < n; i += kSumThreads) {
         sum += (double)row_loss[i];
-        count += !(stats[i].y == 0.f);
+        count += !(stats[i].y < 0.f);
     }
     for (int off = 32; off; off >>= 1) {
         sum += __shfl_xor(sum, off);
@@ -819,7 +819,7 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(const T* __r
         int* mine = listed + group * k;
         for (int i = w * 64 + lane; i < k; i += WPR * 64) mine[i] = idx[row * k + i];
         const float f0 = st.y * g;
-        const bool empty = st.y == 0.f;
+        const bool empty = st.y < 0.f;
         auto dense = [&](float xv) { return empty ? 0.f : f0 * fast_exp2((xv - st.x) * c); };
         if (((reinterpret_cast<uintptr_t>(xr) ^ reinterpret_cast<uintptr_t>(dr)) & 15) == 0) {
             stream_row<T>(
@@ -841,7 +841,7 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(const T* __r
         }
     }
     __syncthreads();
-    if (!live || st.y == 0.f) return;
+    if (!live || st.y < 0.f) return;
     const int* mine = listed + group * k;
     const float* ar = top + row * k;
     for (int i = w * 64 + lane; i < k; i += WPR * 64) {

@@ -33,13 +33,17 @@ __device__ __forceinline__ float act_value(int act, float z) {
         default: return z;
     }
 }
+// (z is cut to where the second terms are 0 in float32: at an infinity, which a kept half-precision z may be, they would be NaN)
 __device__ __forceinline__ float act_slope(int act, float z) {
     switch (act) {
-        case kActRelu: return z > 0.f ? 1.f : 0.f;
-        case kActGelu: return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * fast_exp2(-0.5f * kLog2e * z * z);
+        case kActRelu: return z > 0.f ? 1.f : z != z ? z : 0.f;
+        case kActGelu: {
+            const float c = fminf(fmaxf(z, -30.f), 30.f);
+            return 0.5f * (1.f + erff(z * kSqrtHalf)) + c * kInvSqrt2Pi * fast_exp2(-0.5f * kLog2e * c * c);
+        }
         case kActSilu: {
-            const float s = sigmoid(z);
-            return s * (1.f + z * (1.f - s));
+            const float s = sigmoid(z), c = fminf(fmaxf(z, -100.f), 100.f);
+            return s * (1.f + c * (1.f - s));
         }
         default: return 1.f;
     }
@@ -947,12 +951,12 @@ __global__ __launch_bounds__(kThreads) void linear_bias_kernel(const float* __re
     if (w == 0 && c < cols) dbias[c] = from_f32<T>((run[0][lane] + run[1][lane]) + (run[2][lane] + run[3][lane]));
 }
 
-// Whether a layer goes through the large tiles: from 2^27 multiply-adds on, of at least 64 inputs and outputs; below,
+// Whether a layer goes through the large tiles: from 2^29 multiply-adds on, of at least 64 inputs and outputs; below,
 // packing the operands and filling a few tiles cost more than the 64 x 64 tiles' slower inner loop.
 bool is_large(long long rows, long long cols, long long depth) {
     if (rows <= kFewRows || cols < 64 || depth < 64) return false;
     if (rows > kMaxLd || cols > kMaxLd || depth > kMaxLd) return false;
-    return (double)rows * (double)cols * (double)depth >= 134217728.0;
+    return (double)rows * (double)cols * (double)depth >= 536870912.0;
 }
 
 struct GemmPlan {
@@ -970,10 +974,19 @@ GemmPlan plan_gemm(long long rows, long long cols, long long depth_padded, int p
     g.tiles_j = (unsigned)ceil_div(cols, b);
     g.steps = (int)(depth_padded / kBK) * pairs;
     const long long tiles = (long long)g.tiles_i * g.tiles_j;
-    // few tiles: pieces of the contraction, until every compute unit has one (two of the small ones), none under 8 steps
-    long long s = g.wide ? 1 : 512 / tiles;
-    if (s > g.steps / 8) s = g.steps / 8;
-    if (s < 1) s = 1;
+    // Pieces of the contraction where there are few of the small tiles.  A step of one block on a compute unit takes 0.68 us,
+    // of two at a time 1.13; joining costs a launch and the partial sums' way to memory and back (4 bytes a value
+    // each way, 4 TB/s).  (2048 x 2048 x 2048: 41 us in two pieces, 28 in one.)
+    long long s = 1;
+    if (!g.wide) {
+        double best = 1e30;
+        for (long long c = 1; c <= 32 && c * 4 <= g.steps; ++c) {
+            const long long blocks = ceil_div(tiles * c, 256);       // on the busiest compute unit
+            const double step = (blocks / 2) * 1.13 + (blocks % 2) * 0.68;
+            const double t = (double)ceil_div(g.steps, c) * step + (c > 1 ? 6.0 + c * (double)rows * cols * 2e-6 : 0.0);
+            if (t < best) best = t, s = c;
+        }
+    }
     g.split_len = (int)ceil_div(g.steps, s);
     g.splits = (int)ceil_div(g.steps, g.split_len);
     g.part_bytes = g.splits > 1 ? sizeof(float) * (size_t)g.splits * rows * cols : 0;

@@ -264,3 +264,15 @@ def test_module_streams_and_capture():
         assert torch.equal(y, yy)
         assert all(torch.equal(p, q) for p, q in zip(grads, torch.autograd.grad(yy, eager, dy)))
         torch.cuda.synchronize()
+
+
+def test_half_precision_pre_activations_beyond_the_type():
+    # z of +-70 000 and +-1e5 is no float16; the outputs are 0 or (rightly) infinite, and the slopes 0 or 1
+    x = torch.tensor([[-300.0], [300.0], [-400.0], [1.0]], device="cuda", dtype=torch.float16)
+    w = torch.full((3, 1), 250.0, device="cuda", dtype=torch.float16)
+    for act in ("relu", "gelu", "silu"):
+        xx, ww = x.clone().requires_grad_(), w.clone().requires_grad_()
+        y = linear_act(xx, ww, activation=act)
+        dx, dw = torch.autograd.grad(y, [xx, ww], torch.ones_like(y))
+        assert not y[0].any() and not y[2].any() and torch.isinf(y[1]).all()
+        assert dx.flatten().tolist() == [0.0, 750.0, 0.0, 750.0] and dw.flatten().tolist() == [301.0] * 3

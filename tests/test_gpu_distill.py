@@ -370,3 +370,13 @@ def test_streams_and_capture():
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, step()))
         torch.cuda.synchronize()
+
+
+def test_a_teacher_of_vanishing_weight_still_counts():
+    x, idx, top, _ = _rand(4, 50, 3, torch.float32, seed=3, pads=False)
+    lse = torch.tensor([500.0, 0.0, 0.0, 0.0], device="cuda")     # weights exp(-500): zero in float32
+    idx[1] = -1
+    rows = topk_distill(x, idx, top, teacher_lse=lse, reduction="none")
+    assert rows[0] == 0 and rows[1] == 0
+    # the mean is over the three rows that have a teacher
+    torch.testing.assert_close(topk_distill(x, idx, top, teacher_lse=lse), rows.sum() / 3, rtol=1e-6, atol=0)
