@@ -649,11 +649,21 @@ hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
 
 // ------------------------------------------------------------------ large products
 //
-// C[i, j] = sum_c A[i, c] B[j, c] on 16-bit operands whose rows are padded to whole 128-byte lines (64 elements).  A block
-// owns a BM x BN tile; its operands pass through LDS in steps of 64 along the contraction, two buffers deep,
-// written by the memory pipe itself (16 bytes a lane, no registers).  Such a write lands lane after lane, row after
-// row, and reading one chunk column of 32 rows would hit the same banks every time; so a lane fetches
-// the chunk that belongs there once rows are turned against each other, and the reads look it up.
+// C[i, j] = sum_c A[i, c] B[j, c] on 16-bit operands.  A block owns a BM x BN tile; its operands pass through LDS in steps of
+// 64 along the contraction, two buffers deep, written by the memory pipe itself (16 bytes a lane, no registers).
+//
+// An operand lies along the contraction (x and w forward, dz for dx) or across it ("turned": w for dx, dz and x for dw), and
+// is used as it lies: its 64-wide piece of the contraction is 64 columns of BM rows, or 64 rows of BM columns, in LDS
+// as in memory.  A lane's eight values of one row are then 16 bytes, or come from the LDS through
+// its transposing read, which hands a lane four rows of its column (within 16 lanes, lane 4 e + l / 4 names the row of
+// value e of lane l, four columns each).  The memory pipe writes lane after lane, row after row, and reading one chunk
+// of many rows would hit the same banks every time; so a lane fetches the chunk that belongs there once rows
+// are turned against each other, and the reads look it up.
+// The transposing reads are written out, with their wait: the compiler's form of them waits for all that the memory pipe
+// fetches as well, that is for the next step's tiles.  Forward 8192 x 4096 -> 4096 in bf16 255 us = 1.08 PFLOP/s; with
+// its backward, gelu and residual 850 us, against 890 us with turned copies of the operands.  Without the MFMAs' operand
+// reads the loads alone take 151 us of the 255, without the loads reads and MFMAs 186 us: L2 and LDS share the
+// bound.  Longer pipelines, steps of 32, and tiles of 128 x 128 a wave gave nothing.
 //
 // float32 operands come as three bf16 planes whose sum is the value to 2^-25 or better: the product is
 // the six products of planes that matter (the other three are below 2^-24 of the result), run as one
@@ -663,12 +673,15 @@ constexpr int kBK = 64;
 constexpr long long kMaxLd = 1 << 22;    // a tile's 256 rows are addressed by 32-bit byte offsets
 constexpr int kPlanes = 3, kPairs = 6;
 
+struct Operand {
+    const void* p;
+    long long ld, plane;             // elements between rows, and between planes
+    long long width;                 // elements of a row that may be read: a multiple of 8
+    long long valid;                 // length of the contraction that is there; zeros are taken for the rest of its last step
+};
 struct GemmArgs {
-    const void *a, *b;
-    long long lda, ldb;              // elements
-    long long plane_a, plane_b;      // elements between planes
-    long long rows, cols;
-    int depth;                       // padded length of the contraction, of one plane pair
+    Operand a, b;
+    long long rows, cols, depth;
     int pairs;                       // 1, or kPairs
     int splits, split_len;           // in steps
     unsigned tiles_i, tiles_j;
@@ -692,13 +705,15 @@ struct Frag<f16> {
     }
 };
 
-// Which chunk of row r lies where chunk 0 would: eight rows' chunks of one number cover all banks once.
-__device__ __forceinline__ int swizzle(int r) { return r & 7; }
+__device__ __forceinline__ uint32_t lds_address(const char* lds) {
+    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
+}
+
+__device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
 
 // 64 lanes x 16 bytes from global memory to LDS at `lds` + 16 lane
-__device__ __forceinline__ void load_to_lds(const void* g, char* lds) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g,
-                                     (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+__device__ __forceinline__ void load_to_lds(const char* g, char* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)g, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
 
 // none of the wave's memory operations and LDS reads under way; then all waves
@@ -707,13 +722,123 @@ __device__ __forceinline__ void wait_and_meet() {
     __builtin_amdgcn_s_barrier();
 }
 
+// One operand's share of a tile: W rows of C's (or columns), of which `count` are there from `first` on.
+template <typename T16, int W, int kWavesAll, bool kTurned>
+struct TileOperand {
+    static constexpr int kLoads = W / 8 / kWavesAll;                   // of this wave in each step
+    static constexpr int kChunks = kTurned ? W / 8 : 8, kRowsPer = 64 / kChunks;
+    static constexpr int kBytes = W * kBK * 2;
+    typedef typename Frag<T16>::type frag;
+    const char* base;
+    unsigned off[kLoads];
+    int at_chunk, at_row;           // (of a lane in each load) its chunk's first element, its row
+    long long step_bytes, plane_bytes, valid;
+
+    // `wave`: which of the block's
+    __device__ __forceinline__ void init(const Operand& o, long long first, long long count, int wave) {
+        const int lane = threadIdx.x & 63;
+        at_row = lane / kChunks;
+        // chunk numbers of eight rows differ in their low bits, or of four rows in the next two: a read of one chunk of
+        // 8 rows, or of 32 bytes of 4 rows, then goes round the banks once
+        int chunk = (lane % kChunks) ^ (kTurned ? 2 * ((wave * kRowsPer + at_row) & 3) : at_row & 7);
+        plane_bytes = o.plane * 2;
+        valid = o.valid;
+        if constexpr (kTurned) {
+            base = reinterpret_cast<const char*>(o.p) + first * 2;
+            step_bytes = kBK * o.ld * 2;
+            chunk = min(chunk, (int)min((long long)W, o.width - first) / 8 - 1);      // (columns behind the last: not used)
+        } else {
+            base = reinterpret_cast<const char*>(o.p) + first * o.ld * 2;
+            step_bytes = kBK * 2;
+        }
+        at_chunk = chunk * 8;
+        const int last = (int)min((long long)W, count) - 1;                            // (rows behind the last: not used)
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+            const int r = (q * kWavesAll + wave) * kRowsPer + at_row;
+            off[q] = (unsigned)(kTurned ? r : min(r, last)) * (unsigned)(o.ld * 2) + chunk * 16;
+        }
+    }
+    // step kb of plane `plane`; `edge`: it may reach behind the end of the contraction
+    __device__ __forceinline__ void fetch(int plane, int kb, bool edge, char* lds, int wave) const {
+        const char* g = base + plane * plane_bytes + kb * step_bytes;
+        char* to = lds + wave * 1024;
+        if (!edge) {
+#pragma unroll
+            for (int q = 0; q < kLoads; ++q) load_to_lds(g + off[q], to + q * kWavesAll * 1024);
+        } else {
+            const char* zeros = reinterpret_cast<const char*>(&kZeros);
+#pragma unroll
+            for (int q = 0; q < kLoads; ++q) {
+                const int c = kTurned ? (q * kWavesAll + wave) * kRowsPer + at_row : at_chunk;
+                load_to_lds((long long)kb * kBK + c < valid ? g + off[q] : zeros, to + q * kWavesAll * 1024);
+            }
+        }
+    }
+    // where this lane reads from, for 32 rows of C (columns) from `from` on, and the eight steps of the contraction that are
+    // this half wave's of the sixteen from 16 kk on
+    int at[2];
+    __device__ __forceinline__ void init_reads(int from) {
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+        if constexpr (kTurned) {
+            const int s = lane & 15, row = 8 * half + (s >> 2);
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {
+                const int chunk = (from / 8 + 4 * odd + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1)) ^ (2 * (s >> 2));
+                at[odd] = row * (W * 2) + chunk * 16 + (s & 1) * 8;
+            }
+        } else {
+            at[0] = (from + (lane & 31)) * (kBK * 2);
+            at[1] = 0;
+        }
+    }
+    // F times 32 rows of C (columns)
+    template <int F>
+    __device__ __forceinline__ void read(frag (&out)[F], const char* lds, int kk) const {
+        if constexpr (kTurned) {
+            const uint32_t from = lds_address(lds) + kk * 16 * (W * 2);
+            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+            u32x2 part[2 * F];
+            if constexpr (F == 4) {
+                asm volatile(
+                    "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%c10\n\t"
+                    "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%c10\n\t"
+                    "ds_read_b64_tr_b16 %4, %8 offset:128\n\tds_read_b64_tr_b16 %5, %8 offset:%c11\n\t"
+                    "ds_read_b64_tr_b16 %6, %9 offset:128\n\tds_read_b64_tr_b16 %7, %9 offset:%c11\n\t"
+                    "s_waitcnt lgkmcnt(0)"
+                    : "=&v"(part[0]), "=&v"(part[1]), "=&v"(part[2]), "=&v"(part[3]), "=&v"(part[4]), "=&v"(part[5]),
+                      "=&v"(part[6]), "=&v"(part[7])
+                    : "v"(from + at[0]), "v"(from + at[1]), "n"(4 * W * 2), "n"(4 * W * 2 + 128)
+                    : "memory");
+            } else {
+                static_assert(F == 2, "32 or 64 columns a lane");
+                asm volatile(
+                    "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%c6\n\t"
+                    "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%c6\n\t"
+                    "s_waitcnt lgkmcnt(0)"
+                    : "=&v"(part[0]), "=&v"(part[1]), "=&v"(part[2]), "=&v"(part[3])
+                    : "v"(from + at[0]), "v"(from + at[1]), "n"(4 * W * 2)
+                    : "memory");
+            }
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+                out[f] = __builtin_bit_cast(frag, __builtin_shufflevector(part[2 * f], part[2 * f + 1], 0, 1, 2, 3));
+        } else {
+            const int lane = threadIdx.x & 63;
+#pragma unroll
+            for (int f = 0; f < F; ++f)
+                out[f] = *reinterpret_cast<const frag*>(lds + at[0] + (((2 * kk + (lane >> 5)) ^ (lane & 7)) * 16) + f * 32 * (kBK * 2));
+        }
+    }
+};
+
 template <typename T16, typename OutT, int BM, int BN, int WM, int WN, int OP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel(GemmArgs p) {
     constexpr int kWavesN = BN / WN, kWavesAll = (BM / WM) * kWavesN;
     constexpr int FA = WM / 32, FB = WN / 32;
-    constexpr int BK = kBK, kRow = BK * 2, kChunks = kRow / 16, kRowsPer = 64 / kChunks;     // bytes, chunks of a row; rows of one load
-    constexpr int kLoadsA = BM / kRowsPer / kWavesAll, kLoadsB = BN / kRowsPer / kWavesAll;
-    constexpr int kBytesA = BM * kRow, kBytes = (BM + BN) * kRow;
+    typedef TileOperand<T16, BM, kWavesAll, OP == kDw> OperandA;
+    typedef TileOperand<T16, BN, kWavesAll, OP != kForward> OperandB;
+    constexpr int kBytesA = OperandA::kBytes, kBytes = kBytesA + OperandB::kBytes;
     __shared__ __align__(128) char lds[2 * kBytes];
     typedef typename Frag<T16>::type frag;
     const int lane = threadIdx.x & 63, wave = wave_id();
@@ -729,47 +854,33 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
     id %= group;
     const unsigned ti = first + id % high, tj = id / high;
     const long long i0 = (long long)ti * BM, j0 = (long long)tj * BN;
-    const int k_blocks = p.depth / BK;
+    const int k_blocks = (int)((p.depth + kBK - 1) / kBK);
+    const bool ragged = p.depth % kBK != 0;
     const int s_lo = blockIdx.y * p.split_len, s_hi = min(k_blocks * p.pairs, s_lo + p.split_len);
 
-    // byte offsets of this lane's pieces within the tile's rows (rows behind the last one repeat it: what
-    // they give is not written)
-    const int piece_row = lane / kChunks, chunk = ((lane % kChunks) ^ swizzle(piece_row)) * 16;
-    const char* base_a = reinterpret_cast<const char*>(p.a) + i0 * p.lda * 2;
-    const char* base_b = reinterpret_cast<const char*>(p.b) + j0 * p.ldb * 2;
-    unsigned off_a[kLoadsA], off_b[kLoadsB];
-    const int rows_left = (int)min((long long)BM, p.rows - i0), cols_left = (int)min((long long)BN, p.cols - j0);
-#pragma unroll
-    for (int q = 0; q < kLoadsA; ++q)
-        off_a[q] = (unsigned)min((q * kWavesAll + wave) * kRowsPer + piece_row, rows_left - 1) * (unsigned)(p.lda * 2) + chunk;
-#pragma unroll
-    for (int q = 0; q < kLoadsB; ++q)
-        off_b[q] = (unsigned)min((q * kWavesAll + wave) * kRowsPer + piece_row, cols_left - 1) * (unsigned)(p.ldb * 2) + chunk;
-
+    OperandA a;
+    OperandB b;
+    a.init(p.a, i0, p.rows - i0, wave);
+    b.init(p.b, j0, p.cols - j0, wave);
+    a.init_reads(wm);
+    b.init_reads(wn);
     auto stage = [&](int step, int buf) {
-        long long oa = 0, ob = 0;
-        int kb = step;
+        int kb = step, pa = 0, pb = 0;
         if (p.pairs > 1) {
             const int pair = step / k_blocks;
             kb -= pair * k_blocks;
             // the small products first: (2,0) (0,2) (1,1) (1,0) (0,1) (0,0)
-            const int pa = (pair == 0) ? 2 : (pair == 2 || pair == 3) ? 1 : 0;
-            const int pb = (pair == 1) ? 2 : (pair == 2 || pair == 4) ? 1 : 0;
-            oa = pa * p.plane_a * 2;
-            ob = pb * p.plane_b * 2;
+            pa = (pair == 0) ? 2 : (pair == 2 || pair == 3) ? 1 : 0;
+            pb = (pair == 1) ? 2 : (pair == 2 || pair == 4) ? 1 : 0;
         }
-        const char* ga = base_a + oa + (long long)kb * kRow;
-        const char* gb = base_b + ob + (long long)kb * kRow;
-        char* to = lds + buf * kBytes + wave * 1024;
-#pragma unroll
-        for (int q = 0; q < kLoadsA; ++q) load_to_lds(ga + off_a[q], to + q * kWavesAll * 1024);
-#pragma unroll
-        for (int q = 0; q < kLoadsB; ++q) load_to_lds(gb + off_b[q], to + kBytesA + q * kWavesAll * 1024);
+        const bool edge = ragged && kb == k_blocks - 1;
+        char* to = lds + buf * kBytes;
+        a.fetch(pa, kb, edge, to, wave);
+        b.fetch(pb, kb, edge, to + kBytesA, wave);
     };
 
     f32x16 acc[FA][FB] = {};
     const int half = lane >> 5, l31 = lane & 31;
-    const int row_a = (wm + l31) * kRow, row_b = kBytesA + (wn + l31) * kRow;
     // while one buffer is read, the next step is on its way to the other, which every wave has done with when they meet
     int buf = 0;
     stage(s_lo, 0);
@@ -778,13 +889,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
         if (step + 1 < s_hi) stage(step + 1, buf ^ 1);
         const char* from = lds + buf * kBytes;
 #pragma unroll
-        for (int kk = 0; kk < BK / 16; ++kk) {
-            const int at = ((2 * kk + half) ^ swizzle(l31)) * 16;
+        for (int kk = 0; kk < kBK / 16; ++kk) {
             frag fa[FA], fb[FB];
-#pragma unroll
-            for (int f = 0; f < FA; ++f) fa[f] = *reinterpret_cast<const frag*>(from + row_a + at + f * 32 * kRow);
-#pragma unroll
-            for (int f = 0; f < FB; ++f) fb[f] = *reinterpret_cast<const frag*>(from + row_b + at + f * 32 * kRow);
+            a.read(fa, from, kk);
+            b.read(fb, from + kBytesA, kk);
 #pragma unroll
             for (int f = 0; f < FA; ++f)
 #pragma unroll
@@ -822,14 +930,14 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
         }
 }
 
-// An operand of the large products from a matrix src [rows, cols] (or from dz = dy act'(z), given as src = dy and z):
-// as it stands, its rows padded with zeros to pc elements, and / or turned, its rows then padded to pr;
-// float32 as three bf16 planes.  `sums` [ceil(rows / 64)][cols]: what each 64 rows add up to, before any rounding.
+// An operand of the large products from a matrix src [rows, cols] (or from dz = dy act'(z), given as src = dy and z) that
+// cannot be read as it stands: rows padded with zeros to pc elements, float32 as three bf16 planes.
+// `sums` [ceil(rows / 64)][cols]: what each 64 rows add up to, before any rounding.
 struct PackArgs {
     const void *src, *z;
-    long long ld, rows, cols, pr, pc;
+    long long ld, rows, cols, pc;
     int act;
-    void *out, *turned;
+    void* out;
     float* sums;
 };
 template <typename T>
@@ -865,34 +973,31 @@ __global__ __launch_bounds__(kThreads) void linear_pack_kernel(PackArgs p) {
     typedef typename Plane<T>::type P;
     constexpr int NP = Plane<T>::N;
     typedef P Four __attribute__((ext_vector_type(4)));
-    __shared__ float tile[64][65];
-    __shared__ float part[4][64];
+    __shared__ float part[16][64];
     const int t = threadIdx.x, q = (t & 15) * 4, r0 = t >> 4;
     const unsigned tiles_c = (unsigned)(p.pc / 64), tile_r = blockIdx.x / tiles_c;
     const long long c0 = (long long)(blockIdx.x - tile_r * tiles_c) * 64, y0 = (long long)tile_r * 64;
     const T* __restrict__ src = static_cast<const T*>(p.src);
     const T* __restrict__ z = static_cast<const T*>(p.z);
     P* out = static_cast<P*>(p.out);
-    P* turned = static_cast<P*>(p.turned);
+    const long long left = p.cols - c0 - q;      // of this thread's four columns
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const long long r = y0 + r0 + 16 * i;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        if (r < p.rows && c0 + q + 4 <= p.cols) {
-            T in[4], zi[4];
-            __builtin_memcpy(in, src + r * p.ld + c0 + q, sizeof(in));
-            if (kSlope) __builtin_memcpy(zi, z + r * p.ld + c0 + q, sizeof(zi));
+        if (r >= p.rows) continue;
+        T in[4];
+        float v[4];
+        take_run<T, 4>(in, src + r * p.ld + c0 + q, left);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = kSlope ? to_f32(in[e]) * act_slope(p.act, to_f32(zi[e])) : to_f32(in[e]);
-        } else if (r < p.rows) {
-            for (int e = 0; e < 4; ++e) {
-                const long long c = c0 + q + e;
-                if (c < p.cols) v[e] = to_f32(src[r * p.ld + c]) * (kSlope ? act_slope(p.act, to_f32(z[r * p.ld + c])) : 1.f);
-            }
+        for (int e = 0; e < 4; ++e) v[e] = to_f32(in[e]);
+        if (kSlope) {
+            take_run<T, 4>(in, z + r * p.ld + c0 + q, left);
+            slope_values(p.act, v, in);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) tile[r0 + 16 * i][q + e] = v[e];
-        if (out && r < p.rows) {
+        for (int e = 0; e < 4; ++e) sum[e] += v[e];
+        if (out) {
             Four w[NP];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -905,31 +1010,16 @@ __global__ __launch_bounds__(kThreads) void linear_pack_kernel(PackArgs p) {
             for (int s = 0; s < NP; ++s) *reinterpret_cast<Four*>(out + (s * p.rows + r) * p.pc + c0 + q) = w[s];
         }
     }
-    __syncthreads();
-    if (turned) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const long long c = c0 + r0 + 16 * i;
-            if (c >= p.cols) continue;
-            Four w[NP];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                P o[NP];
-                split_planes<T>(tile[q + e][r0 + 16 * i], o);
-#pragma unroll
-                for (int s = 0; s < NP; ++s) w[s][e] = o[s];
-            }
-#pragma unroll
-            for (int s = 0; s < NP; ++s) *reinterpret_cast<Four*>(turned + (s * p.cols + c) * p.pr + y0 + q) = w[s];
-        }
-    }
     if (p.sums) {
-        float s = 0.f;
-        for (int r = (t >> 6) * 16; r < (t >> 6) * 16 + 16; ++r) s += tile[r][t & 63];
-        part[t >> 6][t & 63] = s;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) part[r0][q + e] = sum[e];
         __syncthreads();
-        if (t < 64 && c0 + t < p.cols && y0 < p.rows)
-            p.sums[(long long)tile_r * p.cols + c0 + t] = (part[0][t] + part[1][t]) + (part[2][t] + part[3][t]);
+        if (t < 64 && c0 + t < p.cols) {
+            float s = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) s += part[i][t];
+            p.sums[(long long)tile_r * p.cols + c0 + t] = s;
+        }
     }
 }
 
@@ -965,14 +1055,14 @@ struct GemmPlan {
     int steps, splits, split_len;
     size_t part_bytes;
 };
-GemmPlan plan_gemm(long long rows, long long cols, long long depth_padded, int pairs) {
+GemmPlan plan_gemm(long long rows, long long cols, long long depth, int pairs) {
     GemmPlan g;
     const long long t256 = ceil_div(rows, 256) * ceil_div(cols, 256);
     g.wide = t256 >= 192;    // three quarters of the compute units at least
     const int b = g.wide ? 256 : 128;
     g.tiles_i = (unsigned)ceil_div(rows, b);
     g.tiles_j = (unsigned)ceil_div(cols, b);
-    g.steps = (int)(depth_padded / kBK) * pairs;
+    g.steps = (int)ceil_div(depth, kBK) * pairs;
     const long long tiles = (long long)g.tiles_i * g.tiles_j;
     // Pieces of the contraction where there are few of the small tiles.  A step of one block on a compute unit takes 0.68 us,
     // of two at a time 1.13; joining costs a launch and the partial sums' way to memory and back (4 bytes a value
@@ -994,31 +1084,26 @@ GemmPlan plan_gemm(long long rows, long long cols, long long depth_padded, int p
 }
 
 template <typename T, int OP>
-hipError_t run_gemm(const void* a, long long lda, long long plane_a, const void* b, long long ldb, long long plane_b,
-                    long long rows, long long cols, long long depth_padded, TileArgs t, void* part, hipStream_t stream) {
+hipError_t run_gemm(const Operand& a, const Operand& b, long long rows, long long cols, long long depth, TileArgs t, void* part,
+                    hipStream_t stream) {
     typedef typename Plane<T>::type P;
-    const GemmPlan g = plan_gemm(rows, cols, depth_padded, sizeof(T) == 4 ? kPairs : 1);
-    GemmArgs p = {};
-    p.a = a, p.b = b, p.lda = lda, p.ldb = ldb, p.plane_a = plane_a, p.plane_b = plane_b;
-    p.rows = rows, p.cols = cols, p.depth = (int)depth_padded, p.pairs = sizeof(T) == 4 ? kPairs : 1;
-    p.splits = g.splits, p.split_len = g.split_len, p.tiles_i = g.tiles_i, p.tiles_j = g.tiles_j;
+    const int pairs = sizeof(T) == 4 ? kPairs : 1;
+    const GemmPlan g = plan_gemm(rows, cols, depth, pairs);
     t.part = static_cast<float*>(part);
     t.rows = rows, t.cols = cols, t.splits = g.splits;
-    p.t = t;
+    const GemmArgs p = {a, b, rows, cols, depth, pairs, g.splits, g.split_len, g.tiles_i, g.tiles_j, t};
     const dim3 grid(g.tiles_i * g.tiles_j, g.splits);
     if (g.wide)
         linear_gemm_kernel<P, T, 256, 256, 128, 64, OP><<<grid, 512, 0, stream>>>(p);
     else
         linear_gemm_kernel<P, T, 128, 128, 64, 64, OP><<<grid, 256, 0, stream>>>(p);
-    if (g.splits > 1) {
-        linear_join_kernel<T, OP><<<dim3(join_blocks(rows * cols)), kThreads, 0, stream>>>(t);
-    }
+    if (g.splits > 1) linear_join_kernel<T, OP><<<dim3(join_blocks(rows * cols)), kThreads, 0, stream>>>(t);
     return hipGetLastError();
 }
 
 template <typename T>
 hipError_t run_pack(const PackArgs& p, hipStream_t stream) {
-    const dim3 grid((unsigned)((p.pc / 64) * (p.pr / 64)));
+    const dim3 grid((unsigned)((p.pc / 64) * ceil_div(p.rows, 64)));
     if (p.act != kActNone)
         linear_pack_kernel<T, true><<<grid, kThreads, 0, stream>>>(p);
     else
@@ -1026,19 +1111,19 @@ hipError_t run_pack(const PackArgs& p, hipStream_t stream) {
     return hipGetLastError();
 }
 
-// A 16-bit matrix that the large products can read where it stands: whole lines, on 16 bytes.
+// A 16-bit matrix that the large products can read where it stands: 16-byte pieces on 16 bytes.
 bool reads_in_place(const void* x, long long ld, long long cols, int dtype) {
-    return dtype != 0 && cols % kBK == 0 && ld % 8 == 0 && ld <= kMaxLd && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+    return dtype != 0 && cols % 8 == 0 && ld % 8 == 0 && ld <= kMaxLd && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 }
 
 // Scratch of a forward / backward call through the large products (offsets from the workspace's start).
 struct BigWs {
-    long long pm, pn, pk;    // m, n, k padded
-    size_t x, w, dz, turned_dz, turned_w, turned_x, sums, part, total;
+    long long pn, pk;        // n, k padded
+    size_t x, w, dz, sums, part, total;
 };
 BigWs carve_big(long long m, long long n, long long k, int dtype, bool backward) {
     BigWs o = {};
-    o.pm = round_up(m, kBK), o.pn = round_up(n, kBK), o.pk = round_up(k, kBK);
+    o.pn = round_up(n, kBK), o.pk = round_up(k, kBK);
     const size_t e = dtype == 0 ? 2 * kPlanes : 2;
     const int pairs = dtype == 0 ? kPairs : 1;
     size_t at = 0;
@@ -1047,38 +1132,42 @@ BigWs carve_big(long long m, long long n, long long k, int dtype, bool backward)
         at += (bytes + 255) & ~(size_t)255;
         return here;
     };
+    o.x = take(e * m * o.pk);
+    o.w = take(e * n * o.pk);
     if (!backward) {
-        o.x = take(e * m * o.pk);
-        o.w = take(e * n * o.pk);
-        o.part = take(plan_gemm(m, n, o.pk, pairs).part_bytes);
+        o.part = take(plan_gemm(m, n, k, pairs).part_bytes);
     } else {
         o.dz = take(e * m * o.pn);
-        o.turned_dz = take(e * n * o.pm);
-        o.turned_w = take(e * k * o.pn);
-        o.turned_x = take(e * k * o.pm);
-        o.sums = take(sizeof(float) * (o.pm / 64) * n);
-        const size_t dx = plan_gemm(m, k, o.pn, pairs).part_bytes, dw = plan_gemm(n, k, o.pm, pairs).part_bytes;
+        o.sums = take(sizeof(float) * ceil_div(m, 64) * n);
+        const size_t dx = plan_gemm(m, k, n, pairs).part_bytes, dw = plan_gemm(n, k, m, pairs).part_bytes;
         o.part = take(dx > dw ? dx : dw);
     }
     o.total = at;
     return o;
 }
 
+// src [rows, cols] as an operand: where it stands, or packed into `room`.  Along the contraction `depth` of
+// its columns are there (zeros from then on, if packed); turned, its rows.
 template <typename T>
-hipError_t forward_large(const LinearArgs& a, TileArgs t, void* ws_, hipStream_t stream) {
+hipError_t make_operand(Operand& o, const void* src, long long ld, long long rows, long long cols, bool turned, int dtype, void* room,
+                        hipStream_t stream) {
+    if (reads_in_place(src, ld, cols, dtype)) {
+        o = {src, ld, 0, cols, turned ? rows : cols};
+        return hipSuccess;
+    }
+    const long long pc = round_up(cols, kBK);
+    o = {room, pc, rows * pc, pc, turned ? rows : pc};
+    return run_pack<T>({src, nullptr, ld, rows, cols, pc, kActNone, room, nullptr}, stream);
+}
+
+template <typename T>
+hipError_t forward_large(const LinearArgs& a, const TileArgs& t, void* ws_, hipStream_t stream) {
     char* ws = static_cast<char*>(ws_);
     const BigWs o = carve_big(a.m, a.n, a.k, a.dtype, false);
-    const void *x = a.x, *w = a.w;
-    long long ldx = a.ldx, ldw = a.ldw;
-    if (!reads_in_place(a.x, a.ldx, a.k, a.dtype)) {
-        if (hipError_t e = run_pack<T>({a.x, nullptr, a.ldx, a.m, a.k, o.pm, o.pk, kActNone, ws + o.x, nullptr, nullptr}, stream)) return e;
-        x = ws + o.x, ldx = o.pk;
-    }
-    if (!reads_in_place(a.w, a.ldw, a.k, a.dtype)) {
-        if (hipError_t e = run_pack<T>({a.w, nullptr, a.ldw, a.n, a.k, o.pn, o.pk, kActNone, ws + o.w, nullptr, nullptr}, stream)) return e;
-        w = ws + o.w, ldw = o.pk;
-    }
-    return run_gemm<T, kForward>(x, ldx, a.m * o.pk, w, ldw, a.n * o.pk, a.m, a.n, o.pk, t, ws + o.part, stream);
+    Operand x, w;
+    if (hipError_t e = make_operand<T>(x, a.x, a.ldx, a.m, a.k, false, a.dtype, ws + o.x, stream)) return e;
+    if (hipError_t e = make_operand<T>(w, a.w, a.ldw, a.n, a.k, false, a.dtype, ws + o.w, stream)) return e;
+    return run_gemm<T, kForward>(x, w, a.m, a.n, a.k, t, ws + o.part, stream);
 }
 
 template <typename T>
@@ -1086,29 +1175,30 @@ hipError_t backward_large(const LinearArgs& a, const void* z, const void* dy, vo
                           hipStream_t stream) {
     char* ws = static_cast<char*>(ws_);
     const BigWs o = carve_big(a.m, a.n, a.k, a.dtype, true);
-    const bool dy_as_it_is = a.act == kActNone && reads_in_place(dy, a.n, a.n, a.dtype);
-    const bool pack_dz = dx && !dy_as_it_is;
+    const bool as_it_is = a.act == kActNone && reads_in_place(dy, a.n, a.n, a.dtype);
+    const bool pack = (dx || dw) && !as_it_is;
     float* sums = dbias ? reinterpret_cast<float*>(ws + o.sums) : nullptr;
-    if (pack_dz || dw || dbias)
-        if (hipError_t e = run_pack<T>({dy, z, a.n, a.m, a.n, o.pm, o.pn, a.act, pack_dz ? ws + o.dz : nullptr,
-                                        dw ? ws + o.turned_dz : nullptr, sums}, stream)) return e;
+    if (pack || dbias)
+        if (hipError_t e = run_pack<T>({dy, z, a.n, a.m, a.n, o.pn, a.act, pack ? ws + o.dz : nullptr, sums}, stream)) return e;
+    Operand dz = {dy, a.n, 0, a.n, a.n};
+    if (pack) dz = {ws + o.dz, o.pn, a.m * o.pn, o.pn, o.pn};
     TileArgs t = {};
     if (dx) {
-        if (hipError_t e = run_pack<T>({a.w, nullptr, a.ldw, a.n, a.k, o.pn, o.pk, kActNone, nullptr, ws + o.turned_w, nullptr}, stream)) return e;
+        Operand w;
+        if (hipError_t e = make_operand<T>(w, a.w, a.ldw, a.n, a.k, true, a.dtype, ws + o.w, stream)) return e;
         t.out = dx;
-        if (hipError_t e = run_gemm<T, kDx>(pack_dz ? ws + o.dz : dy, o.pn, a.m * o.pn, ws + o.turned_w, o.pn, a.k * o.pn, a.m, a.k,
-                                            o.pn, t, ws + o.part, stream)) return e;
+        if (hipError_t e = run_gemm<T, kDx>(dz, w, a.m, a.k, a.n, t, ws + o.part, stream)) return e;
     }
     if (dw) {
-        if (hipError_t e = run_pack<T>({a.x, nullptr, a.ldx, a.m, a.k, o.pm, o.pk, kActNone, nullptr, ws + o.turned_x, nullptr}, stream)) return e;
+        Operand x;
+        if (hipError_t e = make_operand<T>(x, a.x, a.ldx, a.m, a.k, true, a.dtype, ws + o.x, stream)) return e;
         t.out = dw;
-        if (hipError_t e = run_gemm<T, kDw>(ws + o.turned_dz, o.pm, a.n * o.pm, ws + o.turned_x, o.pm, a.k * o.pm, a.n, a.k, o.pm, t,
-                                            ws + o.part, stream)) return e;
+        dz.valid = a.m;
+        if (hipError_t e = run_gemm<T, kDw>(dz, x, a.n, a.k, a.m, t, ws + o.part, stream)) return e;
     }
-    if (dbias) {
+    if (dbias)
         linear_bias_kernel<T><<<dim3((unsigned)ceil_div(a.n, 64)), kThreads, 0, stream>>>(sums, ceil_div(a.m, 64), a.n,
                                                                                           static_cast<T*>(dbias));
-    }
     return hipGetLastError();
 }
 

@@ -119,7 +119,9 @@ def test_activations(act, dtype):
 
 
 # products large enough for the big tiles: whole tiles, a few rows over, odd widths that need padding
-LARGE = [(1024, 512, 768), (1025, 511, 769), (2100, 320, 1000), (520, 1600, 514), (300, 4100, 1100)]
+LARGE = [(1024, 512, 768), (1025, 511, 769), (2100, 320, 1000), (520, 1600, 514), (300, 4100, 1100),
+         # ends of rows and columns within a step of 64 and a tile, read as they lie
+         (1003, 520, 1032), (1032, 1048, 520), (777, 1032, 1096), (2050, 1000, 328)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
