@@ -209,10 +209,10 @@ __device__ __forceinline__ uint32_t search_threshold(uint32_t lo, uint32_t hi, i
 }
 
 // The smallest entry of a selection of at least k of the wave's entries e[0..R) (0: none): exactly the k
-// best where slack is 0, up to `slack` more otherwise.  Bisection over the values, then over the
+// best where slack is 0, up to `slack` more otherwise; k of them reach `from`, if that many are there.  A search over the values, then over the
 // indices of one value, each step a compare and a population count per 64 entries.
 template <int R>
-__device__ __forceinline__ u64 select_from(const u64 (&e)[R], int k, int slack) {
+__device__ __forceinline__ u64 select_from(const u64 (&e)[R], int k, int slack, uint32_t from = 1u) {
     auto count_hi = [&](uint32_t t) {
         int c = 0;
 #pragma unroll
@@ -220,14 +220,8 @@ __device__ __forceinline__ u64 select_from(const u64 (&e)[R], int k, int slack) 
         return c;
     };
     if (count_hi(1u) <= k) return 1ull;
-    uint32_t best = 0;
-#pragma unroll
-    for (int r = 0; r < R; ++r) best = max(best, (uint32_t)(e[r] >> 32));
-#pragma unroll
-    for (int off = 32; off; off >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, off));
-    best = (uint32_t)__builtin_amdgcn_readfirstlane((int)best);
     bool exact;
-    const uint32_t lo = search_threshold(1u, best, k, slack, exact, 64, count_hi);
+    const uint32_t lo = search_threshold(from, 0xffffffffu, k, slack, exact, 64, count_hi);
     if (exact) return (u64)lo << 32;
     // more than k + slack entries >= lo, fewer than k above it: the rest by index among those of value lo
     int above = 0;
@@ -328,10 +322,11 @@ struct WaveList {
     }
 };
 
-// Rank of each lane's entry among the wave's first n lanes (0: the best).
+// Rank of each lane's entry among the wave's (0: the best); lanes from n on have none (0).
 __device__ __forceinline__ int rank_of(u64 e, int n) {
     int rank = 0;
-    for (int j = 0; j < n; ++j) {
+#pragma unroll 8
+    for (int j = 0; j < ((n + 7) & ~7); ++j) {
         const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(e >> 32), j), lo = __builtin_amdgcn_readlane((uint32_t)e, j);
         rank += ((((u64)hi << 32) | lo) > e) ? 1 : 0;
     }
@@ -376,16 +371,8 @@ __device__ __forceinline__ uint32_t bound_of_maxima(float max1, float max2, bool
         return c;
     };
     if (count(1u) < k) return 0u;
-    uint32_t hi = e[0];
-    if constexpr (WPR > 1) {
-#pragma unroll
-        for (int q = 1; q < R; ++q) hi = max(hi, e[q]);
-    }
-#pragma unroll
-    for (int off = 32; off; off >>= 1) hi = max(hi, (uint32_t)__shfl_xor((int)hi, off));
-    hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)hi);
     bool exact;      // (near is enough: ten steps end within 2^12 of it, a two-thousandth of an octave)
-    return search_threshold(1u, hi, k, k / 8, exact, 10, count);
+    return search_threshold(1u, 0xffffffffu, k, k / 8, exact, 10, count);
 }
 
 // Block (row group, split).  WPR: waves per row.
@@ -571,30 +558,66 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
     if (lane == 0) lse[row] = lse_value(acc, inv_t);
 }
 
-// Joins the splits of a row: sixteen waves take up to 1024 entries each, the first joins their best.
+// Joins the splits of a row, k entries each.  The largest value of each of the 64 lanes (of a block's sixteen waves together)
+// is an entry's, and the k-th largest of them bounds the k-th best entry: some k log k entries reach it, which one
+// wave sorts out.  Only if the good ones meet in few lanes, or are equal, are there more than 1024; then every wave
+// keeps the k best of its own first.
+// One block's latencies bound this, its instructions' way from memory among them.  244 splits of k = 64: 14.4 us, 18.6 with
+// every wave's own k best first.
 constexpr int kJoinWaves = 16;
-constexpr int kJoinR = 16;
+constexpr int kJoinR = 16;         // 64 kJoinWaves kJoinR >= kMaxSplits kMaxTop
 template <typename T>
 __global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k, float c, float inv_t, int splits, const u64* __restrict__ part,
                                                                           const float2* __restrict__ part_ms,
                                                                           T* __restrict__ values, int* __restrict__ idx,
                                                                           float* __restrict__ lse) {
-    __shared__ u64 best[kJoinWaves * kMaxTop];
-    __shared__ int counts[kJoinWaves];
+    __shared__ u64 best[kJoinWaves * 64];
+    __shared__ uint32_t keys[kJoinWaves * 64];
+    __shared__ int counter;
     const int wave = wave_id(), lane = threadIdx.x & 63;
     const long long row = blockIdx.x;
     const int total = splits * k;
     const u64* src = part + row * total;
     u64 e[kJoinR];
+    uint32_t key = 0u;
 #pragma unroll
     for (int r = 0; r < kJoinR; ++r) {
-        const int at = (r * kJoinWaves + wave) * 64 + lane;
+        const int at = r * 64 * kJoinWaves + threadIdx.x;
         e[r] = (at < total) ? src[at] : 0ull;
+        key = max(key, (uint32_t)(e[r] >> 32));
     }
-    u64 t = select_from<kJoinR>(e, k, 0);
-    int found = keep_entries<kJoinR>(e, t, best + wave * kMaxTop);
-    if (lane == 0) counts[wave] = found;
+    keys[threadIdx.x] = key;
+    if (threadIdx.x == 0) counter = 0;
     __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kJoinWaves; ++w) key = max(key, keys[w * 64 + lane]);
+    auto count = [&](uint32_t t) { return (int)__popcll(ballot(key >= t)); };
+    uint32_t low = 1u;
+    bool exact;
+    // (of 64 keys for k = 64, the first threshold that all reach is not good enough)
+    if (count(1u) >= k) low = search_threshold(1u, 0xffffffffu, k, k < 64 ? 0 : -1, exact, 12, count);
+    int mine_count = 0;
+#pragma unroll
+    for (int r = 0; r < kJoinR; ++r) mine_count += (uint32_t)(e[r] >> 32) >= low ? 1 : 0;
+    if (mine_count) {
+        int at = atomicAdd(&counter, mine_count);      // (any order: they are ranked in the end)
+#pragma unroll
+        for (int r = 0; r < kJoinR; ++r)
+            if ((uint32_t)(e[r] >> 32) >= low) {
+                if (at < kJoinWaves * 64) best[at] = e[r];
+                ++at;
+            }
+    }
+    __syncthreads();
+    int all = uniform(counter);
+    if (all > kJoinWaves * 64) {
+        __syncthreads();                 // the list is given up
+        const u64 t = select_from<kJoinR>(e, k, 0);
+        const int found = keep_entries<kJoinR>(e, t, best + wave * 64);
+        if (lane >= found) best[wave * 64 + lane] = 0ull;
+        all = kJoinWaves * 64;
+        __syncthreads();
+    }
     if (wave == 1) {
         LseAcc acc;
         acc.init();
@@ -606,10 +629,17 @@ __global__ __launch_bounds__(64 * kJoinWaves) void top_logits_join_kernel(int k,
         if (lane == 0) lse[row] = lse_value(acc, inv_t);
     }
     if (wave != 0) return;
+    int found;
+    auto pick = [&](auto size) {
+        constexpr int R = decltype(size)::value;
+        u64 f[R];
 #pragma unroll
-    for (int r = 0; r < kJoinWaves; ++r) e[r] = (lane < counts[r]) ? best[r * kMaxTop + lane] : 0ull;
-    t = select_from<kJoinR>(e, k, 0);
-    found = keep_entries<kJoinR>(e, t, best);
+        for (int r = 0; r < R; ++r) f[r] = (r * 64 + lane < all) ? best[r * 64 + lane] : 0ull;
+        const u64 t = select_from<R>(f, k, 0, low);
+        found = keep_entries<R>(f, t, best);
+    };
+    if (all <= 384) pick(std::integral_constant<int, 6>());
+    else pick(std::integral_constant<int, kJoinWaves>());
     wave_lds_fence();
     const u64 mine = (lane < found) ? best[lane] : 0ull;
     write_top<T>(mine, found, k, values + row * k, idx + row * k);

@@ -269,6 +269,22 @@ def test_top_logits_ties_orders_and_masks(v, dtype):
     assert int(idx[1].min()) >= -1 and int(idx[1].max()) < v
 
 
+@pytest.mark.parametrize("good", [1, 20, 63, 64, 500])
+def test_top_logits_where_every_piece_of_a_long_row_is_alike(good):
+    """The best of a row in the same few places of every 4096 classes, many of them equal."""
+    v = 245 * 4096
+    at = torch.arange(v, device="cuda")
+    gen = torch.Generator(device="cuda").manual_seed(good)
+    x = torch.full((3, v), -math.inf, device="cuda")
+    x[0, at % 4096 < good] = 1.0
+    x[1] = torch.where(at % 4096 < good, torch.randn(v, device="cuda", generator=gen), torch.tensor(-9.0, device="cuda"))
+    x[2] = torch.where(4095 - at % 4096 < good, at / 4096, -at / 4096.0)
+    for k in (1, 31, 64):
+        for row in range(3):
+            _check_top(x[row:row + 1], k)
+        _check_top(x, k)
+
+
 def test_top_logits_strides_and_shapes():
     x = torch.randn(6, 3001, device="cuda")
     want = top_logits(x[:, 1:2990].contiguous(), 20)
