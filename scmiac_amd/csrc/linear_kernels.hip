@@ -154,9 +154,10 @@ __device__ __forceinline__ void forward_out(float (&v)[V], long long i, long lon
     forward_run<T, V>(v, b, residual != nullptr, added, i * n + j, count, act, y, zk);
 }
 
-// ------------------------------------------------------------------ 64 x 64 tiles, any shape
+// ------------------------------------------------------------------ tiles of 64 x 64, or 128 x 32, any shape
 
-constexpr int kTile = 64, kDepth = 32, kThreads = 256;
+constexpr int kDepth = 32, kThreads = 256;
+constexpr int kTileSize = 4096;      // values of C in either
 
 template <typename T>
 struct Lds {
@@ -171,40 +172,44 @@ struct TileArgs {
     long long rows, cols, depth;   // of C and of the contraction
     long long n;                   // row length of z, dy, y
     int act, splits, lanes;
-    unsigned tiles_i, tiles;       // 64-row tiles of C, and all
+    unsigned tiles_i, tiles;       // tiles of C one below the other, and all
     long long split_len;
     void *out, *keep, *dbias;
     float *part, *part_bias;       // [splits][rows][cols], [splits][rows]
 };
 
-template <typename T>
+template <typename T, int TN>
 struct TileLds {
     union {
         struct {
-            __align__(16) T a[kTile * Lds<T>::LD];
-            __align__(16) T b[kTile * Lds<T>::LD];
+            __align__(16) T a[kTileSize / TN * Lds<T>::LD];
+            __align__(16) T b[TN * Lds<T>::LD];
         };
-        __align__(16) float c[kTile * kTile];
+        __align__(16) float c[kTileSize];
     };
 };
 
-// C leaves through LDS: an accumulator holds one column of four rows a lane, memory wants runs of columns.  A 64 x 64 tile
-// of it lies row by row, every second group of four rows with its halves exchanged, so that the
+// C leaves through LDS: an accumulator holds one column of four rows a lane, memory wants runs of columns.  A tile of TN
+// columns lies row by row, every second group of four rows with its halves (or neighbouring rows) exchanged, so that the
 // two halves of a wave, four rows apart, write to different banks.
-__device__ __forceinline__ int place(int row, int col) { return row * 64 + (col ^ ((row & 4) << 3)); }
-__device__ __forceinline__ void put_quadrant(const f32x16& acc, float* c, int qi, int qj) {
+template <int TN>
+__device__ __forceinline__ int place(int row, int col) {
+    return TN == 64 ? row * 64 + (col ^ ((row & 4) << 3)) : (row ^ ((row >> 2) & 1)) * 32 + col;
+}
+template <int TN>
+__device__ __forceinline__ void put_quadrant(const f32x16& acc, float* c, int i, int j) {
     const int lane = threadIdx.x & 63, half = lane >> 5;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) c[place(qi * 32 + 8 * (r >> 2) + 4 * half + (r & 3), qj * 32 + (lane & 31))] = acc[r];
+    for (int r = 0; r < 16; ++r) c[place<TN>(i + 8 * (r >> 2) + 4 * half + (r & 3), j + (lane & 31))] = acc[r];
 }
-// A 64 x 64 tile from LDS through the epilogue, eight columns at a time, by kT threads: the same columns every time, so
+// A tile from LDS through the epilogue, eight columns at a time, by kT threads: the same columns every time, so
 // that the bias is fetched once, and the residuals of a few rows are fetched before any of them is used.
-template <typename T, int OP, int kT>
+template <typename T, int OP, int kT, int TN>
 __device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long long i0, long long j0, int t) {
-    constexpr int kRuns = (kTile * 8 + kT - 1) / kT, kBatch = kRuns < 4 ? kRuns : 4;
-    const int col = (t & 7) * 8;
+    constexpr int kInRow = TN / 8, kRuns = (kTileSize / 8 + kT - 1) / kT, kBatch = kRuns < 4 ? kRuns : 4;
+    const int col = (t % kInRow) * 8;
     const long long j = j0 + col;
-    if (j >= p.cols || t >= kTile * 8) return;
+    if (j >= p.cols || t >= kTileSize / 8) return;
     const int count = (int)min(8ll, p.cols - j);
     float bias[8] = {};
     if (OP == kForward && p.bias) add_run<T, 8>(bias, static_cast<const T*>(p.bias) + j, count);
@@ -215,16 +220,16 @@ __device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long
         if (residual) {
 #pragma unroll
             for (int u = 0; u < kBatch; ++u) {
-                const long long i = i0 + ((t + (r0 + u) * kT) >> 3);
+                const long long i = i0 + (t + (r0 + u) * kT) / kInRow;
                 take_run<T, 8>(added[u], residual + i * p.ldr + j, i < p.rows ? count : 0);
             }
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-            const int row = (t + (r0 + u) * kT) >> 3;
+            const int row = (t + (r0 + u) * kT) / kInRow;
             const long long i = i0 + row;
             if (i >= p.rows) continue;
-            const f32x4 lo = *reinterpret_cast<const f32x4*>(c + place(row, col)), hi = *reinterpret_cast<const f32x4*>(c + place(row, col + 4));
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(c + place<TN>(row, col)), hi = *reinterpret_cast<const f32x4*>(c + place<TN>(row, col + 4));
             float v[8] = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             if (OP == kForward)
                 forward_run<T, 8>(v, bias, residual != nullptr, added[u], i * p.n + j, count, p.act, static_cast<T*>(p.out),
@@ -236,16 +241,17 @@ __device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long
 }
 
 // Piece `piece` of the work on one product: a tile of C, and within it a split of the contraction.  A group of four waves
-// makes a 64 x 64 tile, each wave a quarter, in steps of 32 along the contraction, fetched one step ahead.  Where the
+// makes a tile, each wave 32 x 32 of it, in steps of 32 along the contraction, fetched one step ahead.  Where the
 // pieces are too few to fill the chip, G groups share one: every G-th step each, added up in their order.
-template <typename T, int OP, int G>
-__device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, TileLds<T>* lds) {
-    constexpr int LD = Lds<T>::LD;
+template <typename T, int OP, int G, int TN>
+__device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, TileLds<T, TN>* lds) {
+    constexpr int LD = Lds<T>::LD, TM = kTileSize / TN;
+    constexpr int kRunsA = TM / 64, kRunB = TN / 8;      // runs of eight a thread fetches of A's step; length of its one of B's
     const int group = G == 1 ? 0 : wave_id() / 4, wave = wave_id() % 4;
     const int t = threadIdx.x % kThreads, lane = t & 63;
     T *as = lds[group].a, *bs = lds[group].b;
     const unsigned split = piece / p.tiles, tile = piece - split * p.tiles, tile_j = tile / p.tiles_i;
-    const long long i0 = (long long)(tile - tile_j * p.tiles_i) * kTile, j0 = (long long)tile_j * kTile;
+    const long long i0 = (long long)(tile - tile_j * p.tiles_i) * TM, j0 = (long long)tile_j * TN;
     const long long c_lo = (long long)split * p.split_len;
     const long long c_hi = min(p.depth, c_lo + p.split_len);
     const T* __restrict__ a = static_cast<const T*>(p.a);
@@ -253,63 +259,69 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
     const T* __restrict__ z = static_cast<const T*>(p.z);
     const T* __restrict__ dy = static_cast<const T*>(p.dy);
 
-    // This thread's eight elements of each operand's step: along the contraction, four threads a row, or
-    // across it, eight threads a column, whichever way they lie next to each other.
+    // This thread's runs of each operand's step: along the contraction, a few threads a row, or
+    // across it, a few threads a column, whichever way its elements lie next to each other.
     constexpr bool kAlongA = OP != kDw, kAlongB = OP == kForward;
-    const int ca = kAlongA ? (t & 3) * 8 : t >> 3, ra = kAlongA ? t >> 2 : (t & 7) * 8;
-    const int cb = kAlongB ? (t & 3) * 8 : t >> 3, rb = kAlongB ? t >> 2 : (t & 7) * 8;
+    constexpr int kInA = kAlongA ? kDepth / 8 : 8, kInB = kAlongB ? kDepth / kRunB : TN / kRunB;
+    const int ca = kAlongA ? (t % kInA) * 8 : t / kInA, ra = kAlongA ? t / kInA : (t % kInA) * 8;
+    const int cb = kAlongB ? (t % kInB) * kRunB : t / kInB, rb = kAlongB ? t / kInB : (t % kInB) * kRunB;
 
-    T va[8], vb[8];
-    float dsum[8] = {};
+    T va[kRunsA][8], vb[kRunB];
+    float dsum[kRunsA][8] = {};
     auto load = [&](long long c0) {
-        {
-            const long long r = i0 + ra, c = c0 + ca;
+#pragma unroll
+        for (int u = 0; u < kRunsA; ++u) {
+            const long long r = i0 + ra + 64 * u, c = c0 + ca;
             const bool there = r < p.rows && c < c_hi;
             const long long count = there ? (kAlongA ? c_hi - c : p.rows - r) : 0;
             if constexpr (OP == kForward) {
-                take_run<T, 8>(va, a + r * p.lda + c, count);
+                take_run<T, 8>(va[u], a + r * p.lda + c, count);
             } else {
                 const long long at = OP == kDx ? r * p.n + c : c * p.n + r;
-                take_run<T, 8>(va, dy + at, count);
+                take_run<T, 8>(va[u], dy + at, count);
                 float g[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) g[e] = to_f32(va[e]);
+                for (int e = 0; e < 8; ++e) g[e] = to_f32(va[u][e]);
                 if (p.act != kActNone) {
                     T vz[8];
                     take_run<T, 8>(vz, z + at, count);
                     slope_values(p.act, g, vz);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) va[e] = from_f32<T>(g[e]);
+                    for (int e = 0; e < 8; ++e) va[u][e] = from_f32<T>(g[e]);
                 }
                 if (OP == kDw) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) dsum[e] += g[e];
+                    for (int e = 0; e < 8; ++e) dsum[u][e] += g[e];
                 }
             }
         }
         {
             const long long r = j0 + rb, c = c0 + cb;
             const long long count = b && r < p.cols && c < c_hi ? (kAlongB ? c_hi - c : p.cols - r) : 0;
-            take_run<T, 8>(vb, b + (kAlongB ? r * p.ldb + c : c * p.ldb + r), count);
+            take_run<T, kRunB>(vb, b + (kAlongB ? r * p.ldb + c : c * p.ldb + r), count);
         }
     };
 
     f32x16 acc = {};
-    const int wr = (wave & 1) * 32 + (lane & 31), wc = (wave >> 1) * 32 + (lane & 31), half = lane >> 5;
+    const int wi = (TN == 64 ? wave & 1 : wave) * 32, wj = TN == 64 ? (wave >> 1) * 32 : 0;     // this wave's part
+    const int wr = wi + (lane & 31), wc = wj + (lane & 31), half = lane >> 5;
     load(c_lo + group * kDepth);
     for (long long c0 = c_lo; c0 < c_hi; c0 += G * kDepth) {
         __syncthreads();
-        if constexpr (kAlongA) {
-            __builtin_memcpy(__builtin_assume_aligned(as + ra * LD + ca, 16), va, sizeof(va));
-        } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) as[(ra + e) * LD + ca] = va[e];
+        for (int u = 0; u < kRunsA; ++u) {
+            if constexpr (kAlongA) {
+                __builtin_memcpy(__builtin_assume_aligned(as + (ra + 64 * u) * LD + ca, 16), va[u], sizeof(va[u]));
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) as[(ra + 64 * u + e) * LD + ca] = va[u][e];
+            }
         }
         if constexpr (kAlongB) {
-            __builtin_memcpy(__builtin_assume_aligned(bs + rb * LD + cb, 16), vb, sizeof(vb));
+            __builtin_memcpy(__builtin_assume_aligned(bs + rb * LD + cb, kRunB * sizeof(T) < 16 ? kRunB * sizeof(T) : 16), vb, sizeof(vb));
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) bs[(rb + e) * LD + cb] = vb[e];
+            for (int e = 0; e < kRunB; ++e) bs[(rb + e) * LD + cb] = vb[e];
         }
         __syncthreads();
         if (c0 + G * kDepth < c_hi) load(c0 + (G + group) * kDepth);
@@ -344,24 +356,26 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
         __syncthreads();
         float* s = lds[group].c;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) s[ca * kTile + ra + e] = dsum[e];
+        for (int u = 0; u < kRunsA; ++u)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) s[ca * TM + ra + 64 * u + e] = dsum[u][e];
         __syncthreads();
-        if (all < kTile && i0 + all < p.rows) {
+        if (all < TM && i0 + all < p.rows) {
             float sum = 0.f;
             for (int g = 0; g < G; ++g)
-                for (int c = 0; c < kDepth; ++c) sum += lds[g].c[c * kTile + all];
+                for (int c = 0; c < kDepth; ++c) sum += lds[g].c[c * TM + all];
             if (p.splits > 1)
                 p.part_bias[(long long)split * p.rows + i0 + all] = sum;
             else
                 static_cast<T*>(p.dbias)[i0 + all] = from_f32<T>(sum);
         }
     }
-    __syncthreads();     // the operands' tiles are read: C's 64 x 64 values take their place
-    put_quadrant(acc, lds[group].c, wave & 1, wave >> 1);
+    __syncthreads();     // the operands' tiles are read: C's values take their place
+    put_quadrant<TN>(acc, lds[group].c, wi, wj);
     __syncthreads();
     float* c = lds[0].c;
     if (G > 1) {
-        for (int e = all * 4; e < kTile * kTile; e += G * kThreads * 4) {
+        for (int e = all * 4; e < kTileSize; e += G * kThreads * 4) {
             f32x4 v = *reinterpret_cast<const f32x4*>(c + e);
 #pragma unroll
             for (int g = 1; g < G; ++g) v += *reinterpret_cast<const f32x4*>(lds[g].c + e);
@@ -370,28 +384,28 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
         __syncthreads();
     }
     if (p.splits > 1) {
-        for (int e = all; e < kTile * kTile; e += G * kThreads) {
-            const long long i = i0 + (e >> 6), j = j0 + (e & 63);
-            if (i < p.rows && j < p.cols) p.part[((long long)split * p.rows + i) * p.cols + j] = c[place(e >> 6, e & 63)];
+        for (int e = all; e < kTileSize; e += G * kThreads) {
+            const long long i = i0 + e / TN, j = j0 + e % TN;
+            if (i < p.rows && j < p.cols) p.part[((long long)split * p.rows + i) * p.cols + j] = c[place<TN>(e / TN, e % TN)];
         }
     } else if (p.out) {
-        tile_out<T, OP, G * kThreads>(p, c, i0, j0, all);
+        tile_out<T, OP, G * kThreads, TN>(p, c, i0, j0, all);
     }
 }
 
-template <typename T, int G>
+template <typename T, int G, int TN>
 __global__ __launch_bounds__(kThreads* G) void linear_tile_forward_kernel(TileArgs p) {
-    __shared__ TileLds<T> lds[G];
-    tile_product<T, kForward, G>(p, blockIdx.x, lds);
+    __shared__ TileLds<T, TN> lds[G];
+    tile_product<T, kForward, G, TN>(p, blockIdx.x, lds);
 }
 // both products of the backward pass in one launch, the first pieces_dx blocks on dx
-template <typename T, int G>
+template <typename T, int G, int TN>
 __global__ __launch_bounds__(kThreads* G) void linear_tile_backward_kernel(TileArgs dx, unsigned pieces_dx, TileArgs dw) {
-    __shared__ TileLds<T> lds[G];
+    __shared__ TileLds<T, TN> lds[G];
     if (blockIdx.x < pieces_dx)
-        tile_product<T, kDx, G>(dx, blockIdx.x, lds);
+        tile_product<T, kDx, G, TN>(dx, blockIdx.x, lds);
     else
-        tile_product<T, kDw, G>(dw, blockIdx.x - pieces_dx, lds);
+        tile_product<T, kDw, G, TN>(dw, blockIdx.x - pieces_dx, lds);
 }
 
 // Joins the splits of the contraction, in their order.
@@ -436,9 +450,9 @@ constexpr unsigned kFewPieces = 256;
 constexpr int kGroups = 4;
 
 // Pieces of the contraction: enough blocks to give every compute unit two, none of them shorter than 256.
-void plan_tiles(long long rows, long long cols, long long depth, int& splits, long long& len) {
+void plan_tiles(long long rows, long long cols, long long depth, int tn, int& splits, long long& len) {
     splits = 1, len = depth;
-    const long long tiles = ceil_div(rows, kTile) * ceil_div(cols, kTile);
+    const long long tiles = ceil_div(rows, kTileSize / tn) * ceil_div(cols, tn);
     if (tiles == 0 || depth == 0) return;
     long long s = 512 / tiles;
     if (s > depth / 256) s = depth / 256;
@@ -446,20 +460,26 @@ void plan_tiles(long long rows, long long cols, long long depth, int& splits, lo
     len = round_up(ceil_div(depth, s), kDepth);
     splits = (int)ceil_div(depth, len);
 }
-size_t tile_bytes(long long rows, long long cols, long long depth) {
+size_t tile_bytes(long long rows, long long cols, long long depth, int tn) {
     int splits;
     long long len;
-    plan_tiles(rows, cols, depth, splits, len);
+    plan_tiles(rows, cols, depth, tn, splits, len);
     return splits > 1 ? sizeof(float) * (size_t)splits * ((size_t)rows * cols + rows) : 0;
 }
 
+// Columns of a tile for C = A B^T.  With at most 32 columns half of a 64 x 64 tile's arithmetic is for nothing, but its tiles
+// are twice as many, which a small A needs more.  Microseconds with 64 and 32 columns:
+// float32 forward 10412 x 2000 -> 30 42.5 / 31.0, 1024 x 2000 -> 30 16.4 / 17.2; backward 4096 x 30 -> 4096 97.7 / 75.5,
+// 2048 x 30 -> 2048 41.1 / 35.7, 1024 x 30 -> 1024 27.5 / 28.5; bfloat16 62.6 / 53.1, 28.3 / 24.9, 20.6 / 21.6.
+inline int tile_width(long long cols, long long size_of_a) { return cols <= 32 && size_of_a >= 2097152 ? 32 : 64; }
+
 // fills in the splits of a product whose partial sums start at ws; returns its number of pieces
-unsigned set_tiles(TileArgs& p, void* ws) {
-    plan_tiles(p.rows, p.cols, p.depth, p.splits, p.split_len);
+unsigned set_tiles(TileArgs& p, int tn, void* ws) {
+    plan_tiles(p.rows, p.cols, p.depth, tn, p.splits, p.split_len);
     p.part = static_cast<float*>(ws);
     p.part_bias = p.part + (size_t)p.splits * p.rows * p.cols;
-    p.tiles_i = (unsigned)ceil_div(p.rows, kTile);
-    p.tiles = (unsigned)(p.tiles_i * ceil_div(p.cols, kTile));
+    p.tiles_i = (unsigned)ceil_div(p.rows, kTileSize / tn);
+    p.tiles = (unsigned)(p.tiles_i * ceil_div(p.cols, tn));
     return p.tiles * (unsigned)p.splits;
 }
 
@@ -915,18 +935,18 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
             }
         return;
     }
-    static_assert(WN % 64 == 0 && WM % 64 == 0 && kWavesAll * kTile * kTile * 4 <= 2 * kBytes, "a 64 x 64 tile of LDS for every wave");
+    static_assert(WN % 64 == 0 && WM % 64 == 0 && kWavesAll * kTileSize * 4 <= 2 * kBytes, "a 64 x 64 tile of LDS for every wave");
     __syncthreads();                             // the operands are read: the room is each wave's own now
-    float* c = reinterpret_cast<float*>(lds) + wave * (kTile * kTile);
+    float* c = reinterpret_cast<float*>(lds) + wave * kTileSize;
 #pragma unroll
     for (int m = 0; m < WM / 64; ++m)
 #pragma unroll
         for (int n = 0; n < WN / 64; ++n) {
             wave_lds_fence();
 #pragma unroll
-            for (int q = 0; q < 4; ++q) put_quadrant(acc[2 * m + (q >> 1)][2 * n + (q & 1)], c, q >> 1, q & 1);
+            for (int q = 0; q < 4; ++q) put_quadrant<64>(acc[2 * m + (q >> 1)][2 * n + (q & 1)], c, (q >> 1) * 32, (q & 1) * 32);
             wave_lds_fence();
-            tile_out<OutT, OP, 64>(p.t, c, i0 + wm + m * 64, j0 + wn + n * 64, lane);
+            tile_out<OutT, OP, 64, 64>(p.t, c, i0 + wm + m * 64, j0 + wn + n * 64, lane);
         }
 }
 
@@ -1204,8 +1224,25 @@ hipError_t backward_large(const LinearArgs& a, const void* z, const void* dy, vo
 
 // scratch of dx in front of that of dw, where neither goes through the large tiles
 size_t backward_dx_bytes(long long m, long long n, long long k, int dtype) {
-    const size_t bytes = has_few_rows_dx(m, n, k) ? few_dx_bytes(m, n, k, dtype == 0 ? 4 : 2) : tile_bytes(m, k, n);
+    const size_t bytes = has_few_rows_dx(m, n, k) ? few_dx_bytes(m, n, k, dtype == 0 ? 4 : 2) : tile_bytes(m, k, n, tile_width(k, m * n));
     return (bytes + 255) & ~(size_t)255;
+}
+
+template <typename T, int TN>
+void run_tiles(TileArgs& p, void* ws, hipStream_t stream) {
+    const unsigned pieces = set_tiles(p, TN, ws);
+    if (pieces <= kFewPieces)
+        linear_tile_forward_kernel<T, kGroups, TN><<<dim3(pieces), kThreads * kGroups, 0, stream>>>(p);
+    else
+        linear_tile_forward_kernel<T, 1, TN><<<dim3(pieces), kThreads, 0, stream>>>(p);
+}
+template <typename T, int TN>
+void run_tiles_backward(const TileArgs& dx, unsigned pieces_dx, const TileArgs& dw, unsigned pieces_dw, hipStream_t stream) {
+    const unsigned pieces = pieces_dx + pieces_dw;
+    if (pieces <= kFewPieces)
+        linear_tile_backward_kernel<T, kGroups, TN><<<dim3(pieces), kThreads * kGroups, 0, stream>>>(dx, pieces_dx, dw);
+    else
+        linear_tile_backward_kernel<T, 1, TN><<<dim3(pieces), kThreads, 0, stream>>>(dx, pieces_dx, dw);
 }
 
 template <typename T>
@@ -1217,11 +1254,10 @@ hipError_t forward_t(const LinearArgs& a, void* y, void* z, void* ws, hipStream_
     p.out = y, p.keep = z;
     if (has_few_rows(a.m, a.n)) return run_few_rows<T>(p, stream);
     if (is_large(a.m, a.n, a.k)) return forward_large<T>(a, p, ws, stream);
-    const unsigned pieces = set_tiles(p, ws);
-    if (pieces <= kFewPieces)
-        linear_tile_forward_kernel<T, kGroups><<<dim3(pieces), kThreads * kGroups, 0, stream>>>(p);
+    if (tile_width(a.n, a.m * a.k) == 32)
+        run_tiles<T, 32>(p, ws, stream);
     else
-        linear_tile_forward_kernel<T, 1><<<dim3(pieces), kThreads, 0, stream>>>(p);
+        run_tiles<T, 64>(p, ws, stream);
     if (p.splits > 1) linear_join_kernel<T, kForward><<<dim3(join_blocks(p.rows * p.cols)), kThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
@@ -1235,24 +1271,25 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
     p.z = z, p.dy = dy, p.n = a.n, p.act = a.act, p.splits = 1;
     TileArgs q = p;
     unsigned pieces_dx = 0, pieces_dw = 0;
+    const int tn = tile_width(a.k, a.m * a.n);      // of both products: A is dz
     if (dx) {
         p.b = a.w, p.ldb = a.ldw, p.rows = a.m, p.cols = a.k, p.depth = a.n, p.out = dx;
         if (has_few_rows_dx(a.m, a.n, a.k)) {
             if (hipError_t e = run_few_rows_dx<T>(p, ws, stream)) return e;
         } else {
-            pieces_dx = set_tiles(p, ws);
+            pieces_dx = set_tiles(p, tn, ws);
         }
     }
     if (dw || dbias) {
         // (for dbias alone there is no product: one column of tiles, and x, which may be NULL, is not read)
         q.b = dw ? a.x : nullptr, q.ldb = a.ldx, q.rows = a.n, q.cols = dw ? a.k : 1, q.depth = a.m, q.out = dw, q.dbias = dbias;
-        pieces_dw = set_tiles(q, ws + backward_dx_bytes(a.m, a.n, a.k, a.dtype));
+        pieces_dw = set_tiles(q, tn, ws + backward_dx_bytes(a.m, a.n, a.k, a.dtype));
     }
     if (pieces_dx + pieces_dw == 0) return hipGetLastError();
-    if (pieces_dx + pieces_dw <= kFewPieces)
-        linear_tile_backward_kernel<T, kGroups><<<dim3(pieces_dx + pieces_dw), kThreads * kGroups, 0, stream>>>(p, pieces_dx, q);
+    if (tn == 32)
+        run_tiles_backward<T, 32>(p, pieces_dx, q, pieces_dw, stream);
     else
-        linear_tile_backward_kernel<T, 1><<<dim3(pieces_dx + pieces_dw), kThreads, 0, stream>>>(p, pieces_dx, q);
+        run_tiles_backward<T, 64>(p, pieces_dx, q, pieces_dw, stream);
     if (pieces_dx == 0) p.splits = 1;      // (its own launches have joined it)
     if (p.splits > 1 || q.splits > 1) {
         const long long ex = p.splits > 1 ? p.rows * p.cols : 0, ew = q.splits > 1 ? q.rows * q.cols : 0;
@@ -1266,8 +1303,9 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
 size_t linear_workspace_bytes(long long m, long long n, long long k, int dtype, int act, int backward) {
     (void)act;
     if (is_large(m, n, k)) return carve_big(m, n, k, dtype, backward).total;
-    if (!backward) return has_few_rows(m, n) ? 0 : tile_bytes(m, n, k);
-    const size_t dw = tile_bytes(n, k, m), bias = tile_bytes(n, 1, m);      // (dbias alone is cut up by itself)
+    if (!backward) return has_few_rows(m, n) ? 0 : tile_bytes(m, n, k, tile_width(n, m * k));
+    const int tn = tile_width(k, m * n);
+    const size_t dw = tile_bytes(n, k, m, tn), bias = tile_bytes(n, 1, m, tn);      // (dbias alone is cut up by itself)
     return backward_dx_bytes(m, n, k, dtype) + (dw > bias ? dw : bias);
 }
 
