@@ -162,7 +162,19 @@ constexpr int kTileSize = 4096;      // values of C in either
 template <typename T>
 struct Lds {
     static constexpr int LD = sizeof(T) == 4 ? kDepth + 4 : kDepth + 8;   // rows start on 16 bytes, four banks apart
+    // Where element c of row r of a step lies.  The 16-byte pieces of every eight rows are exchanged differently: an operand
+    // that lies across the contraction is written a column of every eighth row at a time.
+    static __device__ __forceinline__ int at(int r, int c) { return r * LD + (c ^ (sizeof(T) == 4 ? 4 * ((r >> 3) & 7) : 8 * ((r >> 3) & 3))); }
 };
+
+// V neighbouring elements of a row of a step
+template <typename T, int V>
+__device__ __forceinline__ void put_run(T* lds, int r, int c, const T (&v)[V]) {
+    constexpr int kPiece = V * sizeof(T) < 16 ? V : 16 / sizeof(T);
+#pragma unroll
+    for (int e = 0; e < V; e += kPiece)
+        __builtin_memcpy(__builtin_assume_aligned(lds + Lds<T>::at(r, c + e), kPiece * sizeof(T)), v + e, kPiece * sizeof(T));
+}
 
 struct TileArgs {
     const void *a, *b;             // forward: x, w;  dx: -, w;  dw: -, x
@@ -245,7 +257,7 @@ __device__ __forceinline__ void tile_out(const TileArgs& p, const float* c, long
 // pieces are too few to fill the chip, G groups share one: every G-th step each, added up in their order.
 template <typename T, int OP, int G, int TN>
 __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, TileLds<T, TN>* lds) {
-    constexpr int LD = Lds<T>::LD, TM = kTileSize / TN;
+    constexpr int TM = kTileSize / TN;
     constexpr int kRunsA = TM / 64, kRunB = TN / 8;      // runs of eight a thread fetches of A's step; length of its one of B's
     const int group = G == 1 ? 0 : wave_id() / 4, wave = wave_id() % 4;
     const int t = threadIdx.x % kThreads, lane = t & 63;
@@ -311,17 +323,17 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
 #pragma unroll
         for (int u = 0; u < kRunsA; ++u) {
             if constexpr (kAlongA) {
-                __builtin_memcpy(__builtin_assume_aligned(as + (ra + 64 * u) * LD + ca, 16), va[u], sizeof(va[u]));
+                put_run<T, 8>(as, ra + 64 * u, ca, va[u]);
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e) as[(ra + 64 * u + e) * LD + ca] = va[u][e];
+                for (int e = 0; e < 8; ++e) as[Lds<T>::at(ra + 64 * u + e, ca)] = va[u][e];
             }
         }
         if constexpr (kAlongB) {
-            __builtin_memcpy(__builtin_assume_aligned(bs + rb * LD + cb, kRunB * sizeof(T) < 16 ? kRunB * sizeof(T) : 16), vb, sizeof(vb));
+            put_run<T, kRunB>(bs, rb, cb, vb);
         } else {
 #pragma unroll
-            for (int e = 0; e < kRunB; ++e) bs[(rb + e) * LD + cb] = vb[e];
+            for (int e = 0; e < kRunB; ++e) bs[Lds<T>::at(rb + e, cb)] = vb[e];
         }
         __syncthreads();
         if (c0 + G * kDepth < c_hi) load(c0 + (G + group) * kDepth);
@@ -330,8 +342,8 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
             // gives the same sum of products, and this one reads 16 bytes a lane
 #pragma unroll
             for (int s = 0; s < kDepth / 8; ++s) {
-                const f32x4 fa = *reinterpret_cast<const f32x4*>(&as[wr * LD + s * 8 + half * 4]);
-                const f32x4 fb = *reinterpret_cast<const f32x4*>(&bs[wc * LD + s * 8 + half * 4]);
+                const f32x4 fa = *reinterpret_cast<const f32x4*>(&as[Lds<T>::at(wr, s * 8 + half * 4)]);
+                const f32x4 fb = *reinterpret_cast<const f32x4*>(&bs[Lds<T>::at(wc, s * 8 + half * 4)]);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(fa[q], fb[q], acc, 0, 0, 0);
             }
@@ -339,12 +351,12 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
 #pragma unroll
             for (int s = 0; s < kDepth / 16; ++s) {
                 if constexpr (__is_same(T, bf16)) {
-                    const bf16x8 fa = *reinterpret_cast<const bf16x8*>(&as[wr * LD + s * 16 + half * 8]);
-                    const bf16x8 fb = *reinterpret_cast<const bf16x8*>(&bs[wc * LD + s * 16 + half * 8]);
+                    const bf16x8 fa = *reinterpret_cast<const bf16x8*>(&as[Lds<T>::at(wr, s * 16 + half * 8)]);
+                    const bf16x8 fb = *reinterpret_cast<const bf16x8*>(&bs[Lds<T>::at(wc, s * 16 + half * 8)]);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fa, fb, acc, 0, 0, 0);
                 } else {
-                    const f16x8 fa = *reinterpret_cast<const f16x8*>(&as[wr * LD + s * 16 + half * 8]);
-                    const f16x8 fb = *reinterpret_cast<const f16x8*>(&bs[wc * LD + s * 16 + half * 8]);
+                    const f16x8 fa = *reinterpret_cast<const f16x8*>(&as[Lds<T>::at(wr, s * 16 + half * 8)]);
+                    const f16x8 fb = *reinterpret_cast<const f16x8*>(&bs[Lds<T>::at(wc, s * 16 + half * 8)]);
                     acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(fa, fb, acc, 0, 0, 0);
                 }
             }
