@@ -461,22 +461,61 @@ inline unsigned join_blocks(long long elements) {
 constexpr unsigned kFewPieces = 256;
 constexpr int kGroups = 4;
 
-// Pieces of the contraction: enough blocks to give every compute unit two, none of them shorter than 256.
-void plan_tiles(long long rows, long long cols, long long depth, int tn, int& splits, long long& len) {
-    splits = 1, len = depth;
-    const long long tiles = ceil_div(rows, kTileSize / tn) * ceil_div(cols, tn);
-    if (tiles == 0 || depth == 0) return;
-    long long s = 512 / tiles;
-    if (s > depth / 256) s = depth / 256;
-    if (s < 1) s = 1;
-    len = round_up(ceil_div(depth, s), kDepth);
-    splits = (int)ceil_div(depth, len);
-}
-size_t tile_bytes(long long rows, long long cols, long long depth, int tn) {
+// Pieces of the contraction, of the least expected time: the products of one launch are cut into pieces of about the same
+// number of steps, so many as a piece and the chip then take least for.  With two or more pieces at it, or one of
+// four groups, a compute unit makes a step in about 0.75 us in float32 and 0.25 in the half types, and backward
+// works out the slopes of 64 x 32 pre-activations besides; a join costs 6 us and the partial sums' way.
+// Forward in float32, two blocks to a compute unit wherever the depth allows / this rule: 912 x 3499 -> 1098 170 / 100 us,
+// 1024 x 1024 -> 1024 35 / 29, 33 x 1802 -> 12 15.5 / 10.3; forward and backward with gelu in bfloat16
+// 20 x 3000 -> 1063 39 / 29, 191 x 732 -> 1446 43 / 36, 904 x 108 -> 4686 62 / 61, 2000 x 60 -> 5000 72 / 83.
+struct TilePlan {
     int splits;
     long long len;
-    plan_tiles(rows, cols, depth, tn, splits, len);
-    return splits > 1 ? sizeof(float) * (size_t)splits * ((size_t)rows * cols + rows) : 0;
+};
+struct TileShape {
+    long long rows, cols, depth;
+};
+template <int N>
+void plan_tiles(const TileShape (&of)[N], int tn, int esize, int act, bool backward, TilePlan (&plan)[N]) {
+    static const float slope_us[] = {0.f, 0.05f, 0.6f, 0.4f};
+    const double step = (esize == 4 ? 0.75 : 0.25) + (backward ? slope_us[act] : 0.f);
+    long long tiles[N], steps[N], longest = 1;
+    for (int i = 0; i < N; ++i) {
+        tiles[i] = ceil_div(of[i].rows, kTileSize / tn) * ceil_div(of[i].cols, tn);
+        steps[i] = tiles[i] ? ceil_div(of[i].depth, kDepth) : 0;
+        plan[i] = {1, of[i].depth};
+        if (steps[i] > longest) longest = steps[i];
+    }
+    double least = 1e30;
+    for (long long s = 1; s <= 48 && s <= longest; ++s) {
+        const long long len = ceil_div(longest, s);
+        long long pieces = 0, work = 0;
+        double sums = 0.;
+        for (int i = 0; i < N; ++i) {
+            const long long c = steps[i] > len ? ceil_div(steps[i], len) : 1;
+            pieces += tiles[i] * c, work += tiles[i] * steps[i];
+            if (c > 1) sums += (double)c * of[i].rows * of[i].cols;
+        }
+        double t = s > 1 ? 6.0 + sums * 2e-6 : 0.0;
+        if (pieces <= kFewPieces) {
+            t += step * round_up(len, kGroups);
+        } else if (N == 1) {
+            const long long at_once = ceil_div(pieces, 256);
+            t += step * len * (at_once < 2 ? 2 : at_once);
+        } else {
+            const double alone = len * (2 * step > 1. ? 2 * step : 1.), all = step * (work / 256. + len);
+            t += alone > all ? alone : all;
+        }
+        if (t >= least) continue;
+        least = t;
+        for (int i = 0; i < N; ++i) {
+            plan[i] = {1, of[i].depth};
+            if (steps[i] > len) plan[i] = {(int)ceil_div(steps[i], len), len * kDepth};
+        }
+    }
+}
+size_t part_bytes(const TileShape& of, const TilePlan& plan) {
+    return plan.splits > 1 ? sizeof(float) * (size_t)plan.splits * ((size_t)of.rows * of.cols + of.rows) : 0;
 }
 
 // Columns of a tile for C = A B^T.  With at most 32 columns half of a 64 x 64 tile's arithmetic is for nothing, but its tiles
@@ -486,8 +525,8 @@ size_t tile_bytes(long long rows, long long cols, long long depth, int tn) {
 inline int tile_width(long long cols, long long size_of_a) { return cols <= 32 && size_of_a >= 2097152 ? 32 : 64; }
 
 // fills in the splits of a product whose partial sums start at ws; returns its number of pieces
-unsigned set_tiles(TileArgs& p, int tn, void* ws) {
-    plan_tiles(p.rows, p.cols, p.depth, tn, p.splits, p.split_len);
+unsigned set_tiles(TileArgs& p, int tn, const TilePlan& plan, void* ws) {
+    p.splits = plan.splits, p.split_len = plan.len;
     p.part = static_cast<float*>(ws);
     p.part_bias = p.part + (size_t)p.splits * p.rows * p.cols;
     p.tiles_i = (unsigned)ceil_div(p.rows, kTileSize / tn);
@@ -1073,12 +1112,16 @@ __global__ __launch_bounds__(kThreads) void linear_bias_kernel(const float* __re
     if (w == 0 && c < cols) dbias[c] = from_f32<T>((run[0][lane] + run[1][lane]) + (run[2][lane] + run[3][lane]));
 }
 
-// Whether a layer goes through the large tiles: from 2^29 multiply-adds on, of at least 64 inputs and outputs; below,
+// Whether a layer goes through the large tiles: of at least 64 inputs and outputs, from 2^30 multiply-adds on (three times as many in float32,
+// of which the small tiles' instructions do a quarter of what six products of planes cost the large ones); below,
 // packing the operands and filling a few tiles cost more than the 64 x 64 tiles' slower inner loop.
-bool is_large(long long rows, long long cols, long long depth) {
+// Forward and backward, large / small tiles, in microseconds: bfloat16 1024 x 512 -> 1024 45 / 40, 765 x 2937 -> 252
+// 57 / 44, 2048 x 1024 -> 1024 57 / 64, 1862 x 2848 -> 293 60 / 88; float32 1024 x 1024 -> 1024 124 / 95,
+// 10412 x 2000 -> 128 334 / 246, 912 x 3499 -> 1098 289 / 280 and with silu 294 / 364, 1079 x 465 -> 10272 382 / 412.
+bool is_large(long long rows, long long cols, long long depth, int dtype) {
     if (rows <= kFewRows || cols < 64 || depth < 64) return false;
     if (rows > kMaxLd || cols > kMaxLd || depth > kMaxLd) return false;
-    return (double)rows * (double)cols * (double)depth >= 536870912.0;
+    return (double)rows * (double)cols * (double)depth >= (dtype == 0 ? 3221225472.0 : 1073741824.0);
 }
 
 struct GemmPlan {
@@ -1234,15 +1277,32 @@ hipError_t backward_large(const LinearArgs& a, const void* z, const void* dy, vo
     return hipGetLastError();
 }
 
-// scratch of dx in front of that of dw, where neither goes through the large tiles
-size_t backward_dx_bytes(long long m, long long n, long long k, int dtype) {
-    const size_t bytes = has_few_rows_dx(m, n, k) ? few_dx_bytes(m, n, k, dtype == 0 ? 4 : 2) : tile_bytes(m, k, n, tile_width(k, m * n));
-    return (bytes + 255) & ~(size_t)255;
+// The small tiles' backward pass: the same cuts and scratch, dx's in front of dw's, whichever of its outputs are wanted.
+struct BackwardPlan {
+    int tn;
+    bool few_rows;           // of dx
+    TilePlan dx, dw;
+    size_t dx_bytes, total;
+};
+BackwardPlan plan_backward(long long m, long long n, long long k, int dtype, int act) {
+    BackwardPlan o;
+    const int esize = dtype == 0 ? 4 : 2;
+    o.tn = tile_width(k, m * n);      // (A is dz in both products)
+    o.few_rows = has_few_rows_dx(m, n, k);
+    const TileShape of[2] = {{o.few_rows ? 0 : m, k, n}, {n, k, m}};
+    TilePlan plan[2];
+    plan_tiles(of, o.tn, esize, act, true, plan);
+    o.dx = plan[0], o.dw = plan[1];
+    o.dx_bytes = ((o.few_rows ? few_dx_bytes(m, n, k, esize) : part_bytes(of[0], o.dx)) + 255) & ~(size_t)255;
+    o.total = o.dx_bytes + part_bytes(of[1], o.dw);      // (dbias alone: one column in place of k)
+    return o;
 }
 
 template <typename T, int TN>
 void run_tiles(TileArgs& p, void* ws, hipStream_t stream) {
-    const unsigned pieces = set_tiles(p, TN, ws);
+    TilePlan plan[1];
+    plan_tiles({{p.rows, p.cols, p.depth}}, TN, sizeof(T), p.act, false, plan);
+    const unsigned pieces = set_tiles(p, TN, plan[0], ws);
     if (pieces <= kFewPieces)
         linear_tile_forward_kernel<T, kGroups, TN><<<dim3(pieces), kThreads * kGroups, 0, stream>>>(p);
     else
@@ -1265,7 +1325,7 @@ hipError_t forward_t(const LinearArgs& a, void* y, void* z, void* ws, hipStream_
     p.rows = a.m, p.cols = a.n, p.depth = a.k, p.n = a.n, p.act = a.act;
     p.out = y, p.keep = z;
     if (has_few_rows(a.m, a.n)) return run_few_rows<T>(p, stream);
-    if (is_large(a.m, a.n, a.k)) return forward_large<T>(a, p, ws, stream);
+    if (is_large(a.m, a.n, a.k, a.dtype)) return forward_large<T>(a, p, ws, stream);
     if (tile_width(a.n, a.m * a.k) == 32)
         run_tiles<T, 32>(p, ws, stream);
     else
@@ -1277,28 +1337,28 @@ hipError_t forward_t(const LinearArgs& a, void* y, void* z, void* ws, hipStream_
 template <typename T>
 hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* dx, void* dw, void* dbias, void* ws_,
                       hipStream_t stream) {
-    if (is_large(a.m, a.n, a.k)) return backward_large<T>(a, z, dy, dx, dw, dbias, ws_, stream);
+    if (is_large(a.m, a.n, a.k, a.dtype)) return backward_large<T>(a, z, dy, dx, dw, dbias, ws_, stream);
     char* ws = static_cast<char*>(ws_);
     TileArgs p = {};
     p.z = z, p.dy = dy, p.n = a.n, p.act = a.act, p.splits = 1;
     TileArgs q = p;
     unsigned pieces_dx = 0, pieces_dw = 0;
-    const int tn = tile_width(a.k, a.m * a.n);      // of both products: A is dz
+    const BackwardPlan plan = plan_backward(a.m, a.n, a.k, a.dtype, a.act);
     if (dx) {
         p.b = a.w, p.ldb = a.ldw, p.rows = a.m, p.cols = a.k, p.depth = a.n, p.out = dx;
-        if (has_few_rows_dx(a.m, a.n, a.k)) {
+        if (plan.few_rows) {
             if (hipError_t e = run_few_rows_dx<T>(p, ws, stream)) return e;
         } else {
-            pieces_dx = set_tiles(p, tn, ws);
+            pieces_dx = set_tiles(p, plan.tn, plan.dx, ws);
         }
     }
     if (dw || dbias) {
         // (for dbias alone there is no product: one column of tiles, and x, which may be NULL, is not read)
         q.b = dw ? a.x : nullptr, q.ldb = a.ldx, q.rows = a.n, q.cols = dw ? a.k : 1, q.depth = a.m, q.out = dw, q.dbias = dbias;
-        pieces_dw = set_tiles(q, tn, ws + backward_dx_bytes(a.m, a.n, a.k, a.dtype));
+        pieces_dw = set_tiles(q, plan.tn, plan.dw, ws + plan.dx_bytes);
     }
     if (pieces_dx + pieces_dw == 0) return hipGetLastError();
-    if (tn == 32)
+    if (plan.tn == 32)
         run_tiles_backward<T, 32>(p, pieces_dx, q, pieces_dw, stream);
     else
         run_tiles_backward<T, 64>(p, pieces_dx, q, pieces_dw, stream);
@@ -1313,12 +1373,13 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
 }  // namespace
 
 size_t linear_workspace_bytes(long long m, long long n, long long k, int dtype, int act, int backward) {
-    (void)act;
-    if (is_large(m, n, k)) return carve_big(m, n, k, dtype, backward).total;
-    if (!backward) return has_few_rows(m, n) ? 0 : tile_bytes(m, n, k, tile_width(n, m * k));
-    const int tn = tile_width(k, m * n);
-    const size_t dw = tile_bytes(n, k, m, tn), bias = tile_bytes(n, 1, m, tn);      // (dbias alone is cut up by itself)
-    return backward_dx_bytes(m, n, k, dtype) + (dw > bias ? dw : bias);
+    if (is_large(m, n, k, dtype)) return carve_big(m, n, k, dtype, backward).total;
+    if (backward) return plan_backward(m, n, k, dtype, act).total;
+    if (has_few_rows(m, n)) return 0;
+    TilePlan plan[1];
+    const TileShape of[1] = {{m, n, k}};
+    plan_tiles(of, tile_width(n, m * k), dtype == 0 ? 4 : 2, act, false, plan);
+    return part_bytes(of[0], plan[0]);
 }
 
 hipError_t launch_linear_forward(const LinearArgs& a, void* y, void* z, void* ws, hipStream_t stream) {

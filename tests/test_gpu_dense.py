@@ -121,8 +121,10 @@ def test_activations(act, dtype):
 
 # products large enough for the big tiles: whole tiles, a few rows over, odd widths that need padding
 LARGE = [(1024, 512, 768), (1025, 511, 769), (2100, 320, 1000), (520, 1600, 514), (300, 4100, 1100),
-         # ends of rows and columns within a step of 64 and a tile, read as they lie
-         (1003, 520, 1032), (1032, 1048, 520), (777, 1032, 1096), (2050, 1000, 328)]
+         # ends of rows and columns within a step of 64 and a tile, read as they lie or packed
+         (1003, 520, 1032), (1031, 1048, 1032), (777, 1032, 1352), (2050, 1600, 328), (1032, 1003, 1047),
+         # large in float32, too; few splits and many; tiles of 256 x 256 forward, of dx and of dw
+         (2056, 1048, 2001), (1100, 4100, 960), (9000, 3900, 130), (3390, 400, 3401), (3400, 3391, 400), (400, 3392, 3400)]
 
 
 @pytest.mark.parametrize("dtype", TYPES)
