@@ -670,10 +670,22 @@ __global__ __launch_bounds__(kThreads) void linear_few_rows_dx_kernel(TileArgs p
 }
 
 constexpr long long kMaxFewCols = 1 << 22;   // splits of dx fit a grid's second dimension
-bool has_few_rows(long long m, long long n) { return m >= 1 && m <= kFewRows && n <= kMaxFewCols; }
-// dx goes that way from 2^18 weights on: with fewer, its splits and their join cost more than one launch of tiles for dx
-// and dw together (6 rows, 272 -> 172 in float32: 35 us against 24 for the whole pass).
-bool has_few_rows_dx(long long m, long long n, long long k) { return has_few_rows(m, n) && n * k >= (1 << 18); }
+// Against tiles, which read w no faster but multiply on the matrix cores.  Microseconds, this way / tiles, in bfloat16 and
+// float32:  1 row 4096 -> 16384 24 / 35, 45 / 94, and 50 -> 128 3.2 / 4.4, 3.5 / 6.1;  2 rows 4.2 / 4.4, 4.7 / 6.1;
+// 4 rows 4096 -> 16384 28 / 35, 52 / 94, 4096 -> 4096 14.6 / 14.8, 21 / 30, 500 -> 1000 9.1 / 7.2, 9.1 / 9.2;
+// 8 rows 4096 -> 16384 52 / 35, 71 / 94, 500 -> 1000 16 / 7.3, 16 / 9.5.
+bool has_few_rows(long long m, long long n, long long k, bool float32) {
+    if (m < 1 || m > kFewRows || n > kMaxFewCols) return false;
+    const long long weights = n * k;
+    if (m <= 2) return true;
+    if (m <= 4) return weights >= (float32 ? 1 << 20 : 1 << 24);
+    return float32 && weights >= (1 << 24);
+}
+// dx, its splits and their join in two launches of their own: 1 row with dw, 4096 -> 4096 42 / 45, 59 / 69, 1000 -> 8000
+// 37 / 27, 45 / 37;  8 rows 4096 -> 16384 159 / 150, 239 / 273.
+bool has_few_rows_dx(long long m, long long n, long long k, bool float32) {
+    return m >= 1 && m <= (float32 ? kFewRows : 4) && n <= kMaxFewCols && n * k >= (1 << 24);
+}
 
 void plan_few_dx(long long n, long long k, int esize, int& splits, long long& len) {
     const long long groups = ceil_div(k, 64 * (16 / esize));
@@ -699,7 +711,7 @@ hipError_t run_few_rows(TileArgs p, hipStream_t stream) {
     if (p.rows == 1) linear_few_rows_kernel<T, 1><<<grid, kThreads, 0, stream>>>(p);
     else if (p.rows == 2) linear_few_rows_kernel<T, 2><<<grid, kThreads, 0, stream>>>(p);
     else if (p.rows <= 4) linear_few_rows_kernel<T, 4><<<grid, kThreads, 0, stream>>>(p);
-    else linear_few_rows_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
+    else if constexpr (sizeof(T) == 4) linear_few_rows_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
     return hipGetLastError();
 }
 
@@ -711,7 +723,7 @@ hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
     if (p.rows == 1) linear_few_rows_dx_kernel<T, 1><<<grid, kThreads, 0, stream>>>(p);
     else if (p.rows == 2) linear_few_rows_dx_kernel<T, 2><<<grid, kThreads, 0, stream>>>(p);
     else if (p.rows <= 4) linear_few_rows_dx_kernel<T, 4><<<grid, kThreads, 0, stream>>>(p);
-    else linear_few_rows_dx_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
+    else if constexpr (sizeof(T) == 4) linear_few_rows_dx_kernel<T, 8><<<grid, kThreads, 0, stream>>>(p);
     if (p.splits > 1) {
         linear_join_kernel<T, kDx><<<dim3(join_blocks(p.rows * p.cols)), kThreads, 0, stream>>>(p);
     }
@@ -1132,26 +1144,28 @@ struct GemmPlan {
 };
 GemmPlan plan_gemm(long long rows, long long cols, long long depth, int pairs) {
     GemmPlan g;
-    const long long t256 = ceil_div(rows, 256) * ceil_div(cols, 256);
-    g.wide = t256 >= 192;    // three quarters of the compute units at least
+    g.steps = (int)ceil_div(depth, kBK) * pairs;
+    // By expected time.  A step of one small tile on a compute unit takes 0.68 us, of two at a time 1.13; of a large one,
+    // which has the unit to itself, 2.0 with all units at work and less with fewer.  Where there are few small tiles the
+    // contraction is cut into pieces; joining costs a launch and the partial sums' way to memory and back (4 bytes a value
+    // each way, 4 TB/s).  bfloat16 with large / small tiles, 4096 inputs: 4096 x 4096 130 / 153 us, 3584 x 3584 115 / 134,
+    // 2816 x 2560 113 / 86, 3840 x 4864 (29 large tiles over) 223 / 182; 2048 x 2048 x 2048 in two pieces 41, in one 28.
+    const long long t256 = ceil_div(rows, 256) * ceil_div(cols, 256), t128 = ceil_div(rows, 128) * ceil_div(cols, 128);
+    const long long over = t256 % 256;
+    const double large = g.steps * ((t256 / 256) * 2.0 + (over ? 1.5 + over / 512.0 : 0.0));
+    long long s = 1;
+    double small = 1e30;
+    for (long long c = 1; c <= 32 && (c == 1 || c * 4 <= g.steps); ++c) {
+        const long long blocks = ceil_div(t128 * c, 256);       // on the busiest compute unit
+        const double step = (blocks / 2) * 1.13 + (blocks % 2) * 0.68;
+        const double t = (double)ceil_div(g.steps, c) * step + (c > 1 ? 6.0 + c * (double)rows * cols * 2e-6 : 0.0);
+        if (t < small) small = t, s = c;
+    }
+    g.wide = large < small;
+    if (g.wide) s = 1;
     const int b = g.wide ? 256 : 128;
     g.tiles_i = (unsigned)ceil_div(rows, b);
     g.tiles_j = (unsigned)ceil_div(cols, b);
-    g.steps = (int)ceil_div(depth, kBK) * pairs;
-    const long long tiles = (long long)g.tiles_i * g.tiles_j;
-    // Pieces of the contraction where there are few of the small tiles.  A step of one block on a compute unit takes 0.68 us,
-    // of two at a time 1.13; joining costs a launch and the partial sums' way to memory and back (4 bytes a value
-    // each way, 4 TB/s).  (2048 x 2048 x 2048: 41 us in two pieces, 28 in one.)
-    long long s = 1;
-    if (!g.wide) {
-        double best = 1e30;
-        for (long long c = 1; c <= 32 && c * 4 <= g.steps; ++c) {
-            const long long blocks = ceil_div(tiles * c, 256);       // on the busiest compute unit
-            const double step = (blocks / 2) * 1.13 + (blocks % 2) * 0.68;
-            const double t = (double)ceil_div(g.steps, c) * step + (c > 1 ? 6.0 + c * (double)rows * cols * 2e-6 : 0.0);
-            if (t < best) best = t, s = c;
-        }
-    }
     g.split_len = (int)ceil_div(g.steps, s);
     g.splits = (int)ceil_div(g.steps, g.split_len);
     g.part_bytes = g.splits > 1 ? sizeof(float) * (size_t)g.splits * rows * cols : 0;
@@ -1288,7 +1302,7 @@ BackwardPlan plan_backward(long long m, long long n, long long k, int dtype, int
     BackwardPlan o;
     const int esize = dtype == 0 ? 4 : 2;
     o.tn = tile_width(k, m * n);      // (A is dz in both products)
-    o.few_rows = has_few_rows_dx(m, n, k);
+    o.few_rows = has_few_rows_dx(m, n, k, dtype == 0);
     const TileShape of[2] = {{o.few_rows ? 0 : m, k, n}, {n, k, m}};
     TilePlan plan[2];
     plan_tiles(of, o.tn, esize, act, true, plan);
@@ -1324,7 +1338,7 @@ hipError_t forward_t(const LinearArgs& a, void* y, void* z, void* ws, hipStream_
     p.bias = a.bias, p.residual = a.residual, p.ldr = a.ldr;
     p.rows = a.m, p.cols = a.n, p.depth = a.k, p.n = a.n, p.act = a.act;
     p.out = y, p.keep = z;
-    if (has_few_rows(a.m, a.n)) return run_few_rows<T>(p, stream);
+    if (has_few_rows(a.m, a.n, a.k, sizeof(T) == 4)) return run_few_rows<T>(p, stream);
     if (is_large(a.m, a.n, a.k, a.dtype)) return forward_large<T>(a, p, ws, stream);
     if (tile_width(a.n, a.m * a.k) == 32)
         run_tiles<T, 32>(p, ws, stream);
@@ -1375,7 +1389,7 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
 size_t linear_workspace_bytes(long long m, long long n, long long k, int dtype, int act, int backward) {
     if (is_large(m, n, k, dtype)) return carve_big(m, n, k, dtype, backward).total;
     if (backward) return plan_backward(m, n, k, dtype, act).total;
-    if (has_few_rows(m, n)) return 0;
+    if (has_few_rows(m, n, k, dtype == 0)) return 0;
     TilePlan plan[1];
     const TileShape of[1] = {{m, n, k}};
     plan_tiles(of, tile_width(n, m * k), dtype == 0 ? 4 : 2, act, false, plan);
