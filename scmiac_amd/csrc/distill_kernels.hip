@@ -13,6 +13,8 @@
 // rows), to the four waves of a block, or to several blocks whose results a second kernel joins (few rows).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "train_common.h"
 #include "train_kernels.h"
 
@@ -27,11 +29,17 @@ constexpr int kThreads = 256;
 constexpr int kWaves = kThreads / 64;
 constexpr int kMaxTop = 64;        // one entry per lane of a wave
 constexpr int kGather = 4;         // candidates of a row, in 64s, that are sorted out in one go (>= kWaves)
-constexpr int kShortRow = 1024;    // up to here a wave takes a whole row: a block's four waves would find less than
-                                   // one 16-byte vector per lane each
-// A wave takes a row of up to kShortTopRow classes by itself, too, where there are kManyRows of them (top logits):
-// sorting out a row's candidates is one wave's work, and this keeps all of them at it.
-constexpr int kShortTopRow = 16384, kManyRows = 2048;
+// Up to kShortRow classes a wave takes a whole row: a block's four waves would find less than one 16-byte vector per lane
+// each.  4096 x 1000 float32, k = 8, with a wave a row / four: loss 10.8 / 12.7 us, top logits 12.1 / 11.8 (k = 8 leaves
+// little to sort out); 256 x 2000 7.7 / 7.0 and 9.2 / 8.4.
+constexpr int kShortRow = 1024;
+// So it does with longer rows where there are many.  Top logits: sorting out a row's candidates is one wave's work, and
+// this keeps all of them at it (4096 x 10412 bfloat16, k = 30: 38.6 / 57.0 us).  Loss and gradient, k = 30:
+// 4096 x 2000 bfloat16 26.0 / 29.8, 8192 x 4000 53.2 / 58.0, float32 82.7 / 85.2; but 8192 x 8000 float32 184 / 178,
+// 2048 x 4000 28.4 / 27.4.
+constexpr int kShortTopRow = 16384, kManyTopRows = 2048;
+constexpr int kShortLossRow = 4096, kManyLossRows = 4096;
+inline bool wave_per_row(long long n, long long v) { return v <= kShortRow || (v <= kShortLossRow && n >= kManyLossRows); }
 constexpr int kLoads = 4;          // vectors a lane has in flight
 constexpr int kAhead = 4;          // vectors fetched ahead of the one at work, where the k best are kept
 
@@ -375,7 +383,9 @@ __device__ __forceinline__ uint32_t bound_of_maxima(float max1, float max2, bool
     return search_threshold(1u, 0xffffffffu, k, k / 8, exact, 10, count);
 }
 
-// Block (row group, split).  WPR: waves per row.
+// Block (row group, split).  WPR: waves per row.  Bound by the stream of logits where rows are long, each class costing a compare
+// and an exponential on the way (4096 x 100 000 float16, k = 64: 217 us, 3.8 TB/s), and by the choice among a row's
+// candidates where they are short (4096 x 10412 bfloat16, k = 30: 38 us, 2.2 TB/s).
 template <typename T, int WPR>
 __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restrict__ x, long long ld, long long n, int v,
                                                               int k, float c, float inv_t, int splits, int split_len,
@@ -818,6 +828,7 @@ __global__ __launch_bounds__(kSumThreads) void distill_sum_kernel(const float* _
     }
 }
 
+// Bound by memory: 8192 x 100 000 bfloat16, k = 64, 720 us, 4.5 TB/s read and written (forward 330 us, 5.0 TB/s read).
 // Block (row group, split): the dense part of the split's columns, then the listed classes among them.
 // The dense pass has written tau p g / T there; the second write replaces it with the difference, computed
 // in float32 from x again, so that nothing is lost where p and t nearly cancel.
@@ -892,7 +903,8 @@ __global__ __launch_bounds__(kThreads) void distill_backward_kernel(const T* __r
 
 // Splits of a row: enough blocks for the chip's 256 compute units several times over, none shorter than
 // 4096 columns (16 KiB of float32: below that a block's start and end cost more than its columns), no
-// more than a join can take.
+// more than a join can take.  Top logits of float32 rows, k = 30, with at least 2048 / 4096 / 16384 columns a split:
+// 1 x 100 000 15.9 / 16.8 / 20.2 us, 64 x 30 000 19.5 / 18.6 / 20.4, 64 x 100 000 21.2 / 21.5 / 22.3.
 constexpr long long kMinSplit = 4096;
 constexpr int kMaxSplits = 256;
 void plan_splits(long long n, long long v, int esize, int& splits, long long& len) {
@@ -921,7 +933,7 @@ hipError_t top_logits_t(const void* x, long long ld, long long n, long long v, i
     T* vt = static_cast<T*>(values);
     u64* part = static_cast<u64*>(ws);
     float2* part_ms = reinterpret_cast<float2*>(part + (size_t)n * splits * k);
-    if (v <= kShortRow || (v <= kShortTopRow && n >= kManyRows)) {
+    if (v <= kShortRow || (v <= kShortTopRow && n >= kManyTopRows)) {
         top_logits_kernel<T, 1><<<dim3((unsigned)ceil_div(n, kWaves)), kThreads, 0, stream>>>(xt, ld, n, (int)v, k, c, 1.f / temperature, 1, (int)v, vt, idx,
                                                                                                lse, nullptr, nullptr);
     } else {
@@ -944,7 +956,7 @@ hipError_t distill_forward_t(const DistillArgs& a, int reduction, float* loss, f
     float2* part_ms = static_cast<float2*>(ws);
     float* row_loss = reduction == 0 ? loss : reinterpret_cast<float*>(part_ms + (size_t)a.n * splits);
     if (a.n > 0) {
-        if (a.v <= kShortRow) {
+        if (wave_per_row(a.n, a.v)) {
             distill_forward_kernel<T, 1><<<dim3((unsigned)ceil_div(a.n, kWaves)), kThreads, 0, stream>>>(
                 x, a.ld, a.n, a.v, c, 1, a.v, a.idx, a.top, a.k, a.teacher_lse, ca, a.teacher_temperature, row_loss, stats, nullptr);
         } else {
@@ -969,7 +981,7 @@ hipError_t distill_backward_t(const DistillArgs& a, const float4* stats, const f
     plan_splits(a.n, a.v, sizeof(T), splits, len);
     const T* x = static_cast<const T*>(a.x);
     T* d = static_cast<T*>(dx);
-    if (a.v <= kShortRow)
+    if (wave_per_row(a.n, a.v))
         distill_backward_kernel<T, 1><<<dim3((unsigned)ceil_div(a.n, kWaves)), kThreads, sizeof(int) * kWaves * a.k, stream>>>(
             x, a.ld, a.n, a.v, c, 1.f / a.temperature, 1, a.v, a.idx, a.top, a.k, ca, stats, grad, grad_stride, scale, d, ldd);
     else

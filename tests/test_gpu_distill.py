@@ -92,7 +92,7 @@ def _rand(n, v, k, dtype, seed=0, spread=2.0, pads=True):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,v,k", [(1, 1, 1), (2, 2, 3), (5, 7, 2), (9, 64, 64), (6, 200, 8), (3, 1023, 30), (3, 1024, 30),
-                                   (3, 1025, 30), (2, 4099, 100), (1, 20011, 17), (2, 8192, 1024), (1, 70000, 5)])
+                                   (3, 1025, 30), (2, 4099, 100), (1, 20011, 17), (2, 8192, 1024), (1, 70000, 5), (4099, 1501, 7), (4096, 4096, 3)])
 def test_loss_and_gradient(n, v, k, dtype):
     x, idx, top, gen = _rand(n, v, k, dtype)
     _check(x, idx, top, T=1.0)
@@ -240,7 +240,7 @@ def _check_top(x, k, T=1.0):
 
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("n,v,k", [(1, 1, 1), (3, 5, 8), (7, 64, 64), (300, 200, 8), (5, 1023, 64), (5, 1024, 1), (4, 1025, 64),
-                                   (3, 2049, 30), (2, 10412, 30), (1, 200003, 64), (3, 65537, 7), (1100, 1500, 13)])
+                                   (3, 2049, 30), (2, 10412, 30), (1, 200003, 64), (3, 65537, 7), (1100, 1500, 13), (2049, 3001, 20)])
 def test_top_logits(n, v, k, dtype):
     x = _rand(n, v, 1, dtype, seed=11)[0]
     _check_top(x, k)
