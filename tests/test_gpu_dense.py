@@ -103,7 +103,7 @@ def _check(m, k, n, dtype, act, bias=True, residual=True, seed=0):
 
 SHAPES = [(1, 1, 1), (1, 64, 7), (2, 8, 64), (3, 5, 129), (64, 64, 64), (65, 33, 63), (256, 50, 128), (257, 200, 70),
           (1, 4096, 300), (5, 1000, 1030), (16, 513, 2049), (300, 2000, 17), (2000, 30, 515), (4097, 64, 30),
-          (2049, 31, 1030), (2100, 7, 1001), (2100, 1031, 29), (5000, 421, 32),
+          (2049, 31, 1030), (150001, 30, 29), (13, 100003, 16), (2100, 7, 1001), (2100, 1031, 29), (5000, 421, 32),
           (4, 1030, 1100), (3, 4100, 4099), (7, 4101, 4099), (8, 4096, 4096), (1, 4097, 4099), (2, 4096, 4100)]
 
 
