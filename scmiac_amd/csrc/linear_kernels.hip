@@ -466,11 +466,11 @@ inline bool share_pieces(unsigned pieces, long long longest) { return pieces <= 
 // Pieces of the contraction, of the least expected time: the products of one launch are cut into pieces of about the same
 // number of steps, so many as a piece and the chip then take least for.  With two or more pieces at it, or one of
 // four groups, a compute unit makes a step in about 0.75 us in float32 and 0.25 in the half types, and backward
-// works out the slopes of 64 x 32 pre-activations besides; a join costs 6 us, and for each of a value's sums its
-// fetch and its way to memory and back.
+// works out the slopes of 64 x 32 pre-activations besides (four groups of two products, whose pieces are not of one
+// length, a third more); a join costs 6 us, and for each of a value's sums its fetch and its way to memory and back.
 // Forward in float32, two blocks to a compute unit wherever the depth allows / this rule: 912 x 3499 -> 1098 170 / 100 us,
 // 1024 x 1024 -> 1024 35 / 29, 33 x 1802 -> 12 15.5 / 10.3; forward and backward with gelu in bfloat16
-// 20 x 3000 -> 1063 39 / 29, 191 x 732 -> 1446 43 / 36, 904 x 108 -> 4686 62 / 61, 2000 x 60 -> 5000 72 / 83.
+// 20 x 3000 -> 1063 39 / 29, 191 x 732 -> 1446 43 / 36, 904 x 108 -> 4686 62 / 63, 2000 x 60 -> 5000 72 / 83.
 struct TilePlan {
     int splits;
     long long len;
@@ -501,7 +501,7 @@ void plan_tiles(const TileShape (&of)[N], int tn, int esize, int act, bool backw
         }
         double t = s > 1 ? 6.0 + 0.05 * N * s + sums * 2e-6 : 0.0;
         if (pieces <= kFewPieces) {
-            t += step * round_up(len, kGroups);      // (a piece of up to three steps, by one group: no less)
+            t += (N == 2 ? 1.3 : 1.0) * step * round_up(len, kGroups);      // (a piece of up to three steps, by one group: no less)
         } else if (N == 1) {
             const long long at_once = ceil_div(pieces, 256);
             t += step * len * (at_once < 2 ? 2 : at_once);
