@@ -775,26 +775,7 @@ struct GemmArgs {
     TileArgs t;                      // the epilogue's part
 };
 
-template <typename T16>
-struct Frag;
-template <>
-struct Frag<bf16> {
-    typedef bf16x8 type;
-    static __device__ __forceinline__ f32x16 mfma(type a, type b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
-    }
-};
-template <>
-struct Frag<f16> {
-    typedef f16x8 type;
-    static __device__ __forceinline__ f32x16 mfma(type a, type b, f32x16 c) {
-        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
-    }
-};
-
-__device__ __forceinline__ uint32_t lds_address(const char* lds) {
-    return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
-}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
 __device__ const u32x4 kZeros = {0u, 0u, 0u, 0u};
 
@@ -815,7 +796,7 @@ struct TileOperand {
     static constexpr int kLoads = W / 8 / kWavesAll;                   // of this wave in each step
     static constexpr int kChunks = kTurned ? W / 8 : 8, kRowsPer = 64 / kChunks;
     static constexpr int kBytes = W * kBK * 2;
-    typedef typename Frag<T16>::type frag;
+    static constexpr bool kIsTurned = kTurned;
     const char* base;
     unsigned off[kLoads];
     int at_chunk, at_row;           // (of a lane in each load) its chunk's first element, its row
@@ -862,63 +843,124 @@ struct TileOperand {
             }
         }
     }
-    // where this lane reads from, for 32 rows of C (columns) from `from` on, and the eight steps of the contraction that are
-    // this half wave's of the sixteen from 16 kk on
-    int at[2];
-    __device__ __forceinline__ void init_reads(int from) {
+    // Where this lane reads from, for rows of C (columns) from `from` on, and the eight steps of the contraction that are
+    // this half wave's of the sixteen from 16 kk on: along the contraction 16 bytes of a row for every 32 rows, at(kk) +
+    // 32 rows f; across it two times 8 bytes, four steps apart, at(kk, f & 1) + 128 (f / 2).
+    uint32_t start[2];
+    static constexpr int kStepBytes = 16 * (W * 2), kHalf = 4 * (W * 2), kRows32 = 32 * (kBK * 2);
+    __device__ __forceinline__ void init_reads(int from, const char* lds) {
         const int lane = threadIdx.x & 63, half = lane >> 5;
+        const uint32_t base = (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)lds;
         if constexpr (kTurned) {
             const int s = lane & 15, row = 8 * half + (s >> 2);
 #pragma unroll
             for (int odd = 0; odd < 2; ++odd) {
                 const int chunk = (from / 8 + 4 * odd + 2 * ((lane >> 4) & 1) + ((s & 3) >> 1)) ^ (2 * (s >> 2));
-                at[odd] = row * (W * 2) + chunk * 16 + (s & 1) * 8;
+                start[odd] = base + row * (W * 2) + chunk * 16 + (s & 1) * 8;
             }
         } else {
-            at[0] = (from + (lane & 31)) * (kBK * 2);
-            at[1] = 0;
+            start[0] = base + (from + (lane & 31)) * (kBK * 2) + ((half ^ (lane & 7)) * 16);
+            start[1] = 0;
         }
     }
-    // F times 32 rows of C (columns)
-    template <int F>
-    __device__ __forceinline__ void read(frag (&out)[F], const char* lds, int kk) const {
-        if constexpr (kTurned) {
-            const uint32_t from = lds_address(lds) + kk * 16 * (W * 2);
-            typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-            u32x2 part[2 * F];
-            if constexpr (F == 4) {
-                asm volatile(
-                    "ds_read_b64_tr_b16 %0, %8\n\tds_read_b64_tr_b16 %1, %8 offset:%c10\n\t"
-                    "ds_read_b64_tr_b16 %2, %9\n\tds_read_b64_tr_b16 %3, %9 offset:%c10\n\t"
-                    "ds_read_b64_tr_b16 %4, %8 offset:128\n\tds_read_b64_tr_b16 %5, %8 offset:%c11\n\t"
-                    "ds_read_b64_tr_b16 %6, %9 offset:128\n\tds_read_b64_tr_b16 %7, %9 offset:%c11\n\t"
-                    "s_waitcnt lgkmcnt(0)"
-                    : "=&v"(part[0]), "=&v"(part[1]), "=&v"(part[2]), "=&v"(part[3]), "=&v"(part[4]), "=&v"(part[5]),
-                      "=&v"(part[6]), "=&v"(part[7])
-                    : "v"(from + at[0]), "v"(from + at[1]), "n"(4 * W * 2), "n"(4 * W * 2 + 128)
-                    : "memory");
-            } else {
-                static_assert(F == 2, "32 or 64 columns a lane");
-                asm volatile(
-                    "ds_read_b64_tr_b16 %0, %4\n\tds_read_b64_tr_b16 %1, %4 offset:%c6\n\t"
-                    "ds_read_b64_tr_b16 %2, %5\n\tds_read_b64_tr_b16 %3, %5 offset:%c6\n\t"
-                    "s_waitcnt lgkmcnt(0)"
-                    : "=&v"(part[0]), "=&v"(part[1]), "=&v"(part[2]), "=&v"(part[3])
-                    : "v"(from + at[0]), "v"(from + at[1]), "n"(4 * W * 2)
-                    : "memory");
-            }
-#pragma unroll
-            for (int f = 0; f < F; ++f)
-                out[f] = __builtin_bit_cast(frag, __builtin_shufflevector(part[2 * f], part[2 * f + 1], 0, 1, 2, 3));
-        } else {
-            const int lane = threadIdx.x & 63;
-#pragma unroll
-            for (int f = 0; f < F; ++f)
-                out[f] = *reinterpret_cast<const frag*>(lds + at[0] + (((2 * kk + (lane >> 5)) ^ (lane & 7)) * 16) + f * 32 * (kBK * 2));
-        }
+    __device__ __forceinline__ uint32_t at(int kk, int odd = 0) const {
+        return kTurned ? start[odd] + kk * kStepBytes : start[0] ^ (kk * 32);
     }
 };
 
+// A wave's fragments of sixteen steps of the contraction: 32 rows of C each (columns), eight steps a lane.
+template <int F, bool kTurned>
+struct Fragments {
+    u32x4 whole[F];
+    __device__ __forceinline__ u32x4 get(int f) const { return whole[f]; }
+};
+template <int F>
+struct Fragments<F, true> {
+    u32x2 part[2 * F];
+    __device__ __forceinline__ u32x4 get(int f) const { return __builtin_shufflevector(part[2 * f], part[2 * f + 1], 0, 1, 2, 3); }
+};
+
+// One step of sixteen: C += the products of the fragments x, y, while the next ones are on their way from LDS.  Written
+// out in one block with its wait, since the compiler gathers a step's reads in front of its products.  (The
+// products of a block go to different accumulators, so that none waits for another.)
+#define SCMIAC_MUL(t, i, j) "v_mfma_f32_32x32x16_" t " %[c" #i #j "], %[x" #i "], %[y" #j "], %[c" #i #j "]\n\t"
+#define SCMIAC_ROW(v, f, off) "ds_read_b128 %[" #v #f "], %[" #v "at0] offset:" #off "\n\t"
+#define SCMIAC_TURNED(v, f, odd, off)                                            \
+    "ds_read_b64_tr_b16 %[" #v #f "l], %[" #v "at" #odd "] offset:" #off "\n\t" \
+    "ds_read_b64_tr_b16 %[" #v #f "h], %[" #v "at" #odd "] offset:%c[" #v "h" #off "]\n\t"
+#define SCMIAC_BLOCK_4_2(t, a0, a1, a2, a3, b0, b1)                                                               \
+    "s_nop 1\n\t" SCMIAC_MUL(t, 0, 0) a0 SCMIAC_MUL(t, 0, 1) a1 SCMIAC_MUL(t, 1, 0) a2 SCMIAC_MUL(t, 1, 1) a3      \
+        SCMIAC_MUL(t, 2, 0) b0 SCMIAC_MUL(t, 2, 1) b1 SCMIAC_MUL(t, 3, 0) SCMIAC_MUL(t, 3, 1) "s_waitcnt lgkmcnt(0)"
+#define SCMIAC_BLOCK_2_2(t, a0, a1, b0, b1) \
+    "s_nop 1\n\t" SCMIAC_MUL(t, 0, 0) a0 b0 SCMIAC_MUL(t, 0, 1) a1 b1 SCMIAC_MUL(t, 1, 0) SCMIAC_MUL(t, 1, 1) "s_waitcnt lgkmcnt(0)"
+#define SCMIAC_ROWS_4(v) SCMIAC_ROW(v, 0, 0), SCMIAC_ROW(v, 1, 4096), SCMIAC_ROW(v, 2, 8192), SCMIAC_ROW(v, 3, 12288)
+#define SCMIAC_ROWS_2(v) SCMIAC_ROW(v, 0, 0), SCMIAC_ROW(v, 1, 4096)
+#define SCMIAC_TURNED_4(v) SCMIAC_TURNED(v, 0, 0, 0), SCMIAC_TURNED(v, 1, 1, 0), SCMIAC_TURNED(v, 2, 0, 128), SCMIAC_TURNED(v, 3, 1, 128)
+#define SCMIAC_TURNED_2(v) SCMIAC_TURNED(v, 0, 0, 0), SCMIAC_TURNED(v, 1, 1, 0)
+#define SCMIAC_SUM_2 [c00] "+v"(c[0][0]), [c01] "+v"(c[0][1]), [c10] "+v"(c[1][0]), [c11] "+v"(c[1][1])
+#define SCMIAC_SUM_4 SCMIAC_SUM_2, [c20] "+v"(c[2][0]), [c21] "+v"(c[2][1]), [c30] "+v"(c[3][0]), [c31] "+v"(c[3][1])
+#define SCMIAC_OUT_ROWS_2(v, n) [v##0] "=&v"(n.whole[0]), [v##1] "=&v"(n.whole[1])
+#define SCMIAC_OUT_ROWS_4(v, n) SCMIAC_OUT_ROWS_2(v, n), [v##2] "=&v"(n.whole[2]), [v##3] "=&v"(n.whole[3])
+#define SCMIAC_OUT_TURNED_2(v, n) \
+    [v##0l] "=&v"(n.part[0]), [v##0h] "=&v"(n.part[1]), [v##1l] "=&v"(n.part[2]), [v##1h] "=&v"(n.part[3])
+#define SCMIAC_OUT_TURNED_4(v, n) \
+    SCMIAC_OUT_TURNED_2(v, n), [v##2l] "=&v"(n.part[4]), [v##2h] "=&v"(n.part[5]), [v##3l] "=&v"(n.part[6]), [v##3h] "=&v"(n.part[7])
+#define SCMIAC_AT_ROWS(v, at) [v##at0] "v"(at[0])
+#define SCMIAC_AT_TURNED(v, at, half) [v##at0] "v"(at[0]), [v##at1] "v"(at[1]), [v##h0] "n"(half), [v##h128] "n"(half + 128)
+#define SCMIAC_IN_2 [x0] "v"(x.get(0)), [x1] "v"(x.get(1)), [y0] "v"(y.get(0)), [y1] "v"(y.get(1))
+#define SCMIAC_IN_4 SCMIAC_IN_2, [x2] "v"(x.get(2)), [x3] "v"(x.get(3))
+#define SCMIAC_MULTIPLY(t)                                                                                                        \
+    if constexpr (FA == 4 && !kTurnedA && !kTurnedB)                                                                              \
+        asm volatile(SCMIAC_EXPAND(SCMIAC_BLOCK_4_2, t, SCMIAC_ROWS_4(a), SCMIAC_ROWS_2(b))                                       \
+                     : SCMIAC_SUM_4, SCMIAC_OUT_ROWS_4(a, xn), SCMIAC_OUT_ROWS_2(b, yn)                                           \
+                     : SCMIAC_IN_4, SCMIAC_AT_ROWS(a, at_a), SCMIAC_AT_ROWS(b, at_b)                                              \
+                     : "memory");                                                                                                 \
+    else if constexpr (FA == 4 && !kTurnedA)                                                                                      \
+        asm volatile(SCMIAC_EXPAND(SCMIAC_BLOCK_4_2, t, SCMIAC_ROWS_4(a), SCMIAC_TURNED_2(b))                                     \
+                     : SCMIAC_SUM_4, SCMIAC_OUT_ROWS_4(a, xn), SCMIAC_OUT_TURNED_2(b, yn)                                         \
+                     : SCMIAC_IN_4, SCMIAC_AT_ROWS(a, at_a), SCMIAC_AT_TURNED(b, at_b, kHalfB)                                    \
+                     : "memory");                                                                                                 \
+    else if constexpr (FA == 4)                                                                                                   \
+        asm volatile(SCMIAC_EXPAND(SCMIAC_BLOCK_4_2, t, SCMIAC_TURNED_4(a), SCMIAC_TURNED_2(b))                                   \
+                     : SCMIAC_SUM_4, SCMIAC_OUT_TURNED_4(a, xn), SCMIAC_OUT_TURNED_2(b, yn)                                       \
+                     : SCMIAC_IN_4, SCMIAC_AT_TURNED(a, at_a, kHalfA), SCMIAC_AT_TURNED(b, at_b, kHalfB)                          \
+                     : "memory");                                                                                                 \
+    else if constexpr (!kTurnedA && !kTurnedB)                                                                                    \
+        asm volatile(SCMIAC_EXPAND(SCMIAC_BLOCK_2_2, t, SCMIAC_ROWS_2(a), SCMIAC_ROWS_2(b))                                       \
+                     : SCMIAC_SUM_2, SCMIAC_OUT_ROWS_2(a, xn), SCMIAC_OUT_ROWS_2(b, yn)                                           \
+                     : SCMIAC_IN_2, SCMIAC_AT_ROWS(a, at_a), SCMIAC_AT_ROWS(b, at_b)                                              \
+                     : "memory");                                                                                                 \
+    else if constexpr (!kTurnedA)                                                                                                 \
+        asm volatile(SCMIAC_EXPAND(SCMIAC_BLOCK_2_2, t, SCMIAC_ROWS_2(a), SCMIAC_TURNED_2(b))                                     \
+                     : SCMIAC_SUM_2, SCMIAC_OUT_ROWS_2(a, xn), SCMIAC_OUT_TURNED_2(b, yn)                                         \
+                     : SCMIAC_IN_2, SCMIAC_AT_ROWS(a, at_a), SCMIAC_AT_TURNED(b, at_b, kHalfB)                                    \
+                     : "memory");                                                                                                 \
+    else                                                                                                                          \
+        asm volatile(SCMIAC_EXPAND(SCMIAC_BLOCK_2_2, t, SCMIAC_TURNED_2(a), SCMIAC_TURNED_2(b))                                   \
+                     : SCMIAC_SUM_2, SCMIAC_OUT_TURNED_2(a, xn), SCMIAC_OUT_TURNED_2(b, yn)                                       \
+                     : SCMIAC_IN_2, SCMIAC_AT_TURNED(a, at_a, kHalfA), SCMIAC_AT_TURNED(b, at_b, kHalfB)                          \
+                     : "memory")
+#define SCMIAC_EXPAND(block, ...) block(__VA_ARGS__)
+
+template <typename T16, int FA, int FB, bool kTurnedA, bool kTurnedB, int kHalfA, int kHalfB>
+__device__ __forceinline__ void multiply(f32x16 (&c)[FA][FB], const Fragments<FA, kTurnedA>& x, const Fragments<FB, kTurnedB>& y,
+                                         Fragments<FA, kTurnedA>& xn, Fragments<FB, kTurnedB>& yn, const uint32_t (&at_a)[2],
+                                         const uint32_t (&at_b)[2]) {
+    static_assert((FA == 4 || FA == 2) && FB == 2 && (kTurnedB || !kTurnedA), "the blocks there are");
+    if constexpr (__is_same(T16, bf16)) {
+        SCMIAC_MULTIPLY("bf16");
+    } else {
+        SCMIAC_MULTIPLY("f16");
+    }
+}
+// the last products are done: the compiler does not know of them
+template <int FA, int FB>
+__device__ __forceinline__ void settle(f32x16 (&c)[FA][FB]) {
+    if constexpr (FA == 4)
+        asm volatile("s_nop 15\n\ts_nop 15" : SCMIAC_SUM_4);
+    else
+        asm volatile("s_nop 15\n\ts_nop 15" : SCMIAC_SUM_2);
+}
 template <typename T16, typename OutT, int BM, int BN, int WM, int WN, int OP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel(GemmArgs p) {
     constexpr int kWavesN = BN / WN, kWavesAll = (BM / WM) * kWavesN;
@@ -927,7 +969,6 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
     typedef TileOperand<T16, BN, kWavesAll, OP != kForward> OperandB;
     constexpr int kBytesA = OperandA::kBytes, kBytes = kBytesA + OperandB::kBytes;
     __shared__ __align__(128) char lds[2 * kBytes];
-    typedef typename Frag<T16>::type frag;
     const int lane = threadIdx.x & 63, wave = wave_id();
     const int wm = (wave / kWavesN) * WM, wn = (wave % kWavesN) * WN;
 
@@ -949,8 +990,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
     OperandB b;
     a.init(p.a, i0, p.rows - i0, wave);
     b.init(p.b, j0, p.cols - j0, wave);
-    a.init_reads(wm);
-    b.init_reads(wn);
+    a.init_reads(wm, lds);
+    b.init_reads(wn, lds + kBytesA);
     auto stage = [&](int step, int buf) {
         int kb = step, pa = 0, pb = 0;
         if (p.pairs > 1) {
@@ -968,25 +1009,32 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
 
     f32x16 acc[FA][FB] = {};
     const int half = lane >> 5, l31 = lane & 31;
-    // while one buffer is read, the next step is on its way to the other, which every wave has done with when they meet
-    int buf = 0;
+    Fragments<FA, OperandA::kIsTurned> x, xn;
+    Fragments<FB, OperandB::kIsTurned> y, yn;
+    auto step16 = [&](int kk, int buf) {      // the products of x, y, and the fragments of kk from buffer buf in their place
+        const uint32_t at_a[2] = {a.at(kk) + buf * kBytes, a.at(kk, 1) + buf * kBytes};
+        const uint32_t at_b[2] = {b.at(kk) + buf * kBytes, b.at(kk, 1) + buf * kBytes};
+        multiply<T16, FA, FB, OperandA::kIsTurned, OperandB::kIsTurned, OperandA::kHalf, OperandB::kHalf>(acc, x, y, xn, yn, at_a, at_b);
+        x = xn, y = yn;
+    };
+    x = {}, y = {};                           // (whose products are zeros)
     stage(s_lo, 0);
+    if (s_lo + 1 < s_hi) stage(s_lo + 1, 1);
+    wait_and_meet();
+    step16(0, 0);
+    // While one buffer is read, the next step is on its way to the other.  Before its last sixteen products a wave has the last
+    // of a buffer in hand: when they meet, the buffer can be filled anew, and the other has landed, this wave's share
+    // of it, then everybody's.  (Behind the last step there is no other: what is read then is not used.)
+    int buf = 0;
     for (int step = s_lo; step < s_hi; ++step) {
-        wait_and_meet();     // this step's tiles have landed: this wave's share of them, then everybody's
-        if (step + 1 < s_hi) stage(step + 1, buf ^ 1);
-        const char* from = lds + buf * kBytes;
 #pragma unroll
-        for (int kk = 0; kk < kBK / 16; ++kk) {
-            frag fa[FA], fb[FB];
-            a.read(fa, from, kk);
-            b.read(fb, from + kBytesA, kk);
-#pragma unroll
-            for (int f = 0; f < FA; ++f)
-#pragma unroll
-                for (int g = 0; g < FB; ++g) acc[f][g] = Frag<T16>::mfma(fa[f], fb[g], acc[f][g]);
-        }
+        for (int kk = 1; kk < kBK / 16; ++kk) step16(kk, buf);
+        wait_and_meet();
+        if (step + 2 < s_hi) stage(step + 2, buf);
         buf ^= 1;
+        step16(0, buf);
     }
+    settle(acc);
 
     if (p.splits > 1) {
 #pragma unroll
