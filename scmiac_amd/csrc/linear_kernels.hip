@@ -965,6 +965,7 @@ template <typename T16, typename OutT, int BM, int BN, int WM, int WN, int OP>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel(GemmArgs p) {
     constexpr int kWavesN = BN / WN, kWavesAll = (BM / WM) * kWavesN;
     constexpr int FA = WM / 32, FB = WN / 32;
+    constexpr bool kInParts = BM == 256;
     typedef TileOperand<T16, BM, kWavesAll, OP == kDw> OperandA;
     typedef TileOperand<T16, BN, kWavesAll, OP != kForward> OperandB;
     constexpr int kBytesA = OperandA::kBytes, kBytes = kBytesA + OperandB::kBytes;
@@ -992,7 +993,8 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
     b.init(p.b, j0, p.cols - j0, wave);
     a.init_reads(wm, lds);
     b.init_reads(wn, lds + kBytesA);
-    auto stage = [&](int step, int buf) {
+    // half 0, 1: one operand of a step
+    auto stage = [&](int step, int buf, int half) {
         int kb = step, pa = 0, pb = 0;
         if (p.pairs > 1) {
             const int pair = step / k_blocks;
@@ -1003,8 +1005,10 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
         }
         const bool edge = ragged && kb == k_blocks - 1;
         char* to = lds + buf * kBytes;
-        a.fetch(pa, kb, edge, to, wave);
-        b.fetch(pb, kb, edge, to + kBytesA, wave);
+        if (half == 0)
+            a.fetch(pa, kb, edge, to, wave);
+        else
+            b.fetch(pb, kb, edge, to + kBytesA, wave);
     };
 
     f32x16 acc[FA][FB] = {};
@@ -1018,19 +1022,29 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void linear_gemm_kernel
         x = xn, y = yn;
     };
     x = {}, y = {};                           // (whose products are zeros)
-    stage(s_lo, 0);
-    if (s_lo + 1 < s_hi) stage(s_lo + 1, 1);
+    stage(s_lo, 0, 0), stage(s_lo, 0, 1);
+    if (s_lo + 1 < s_hi) {
+        stage(s_lo + 1, 1, 0);
+        if (!kInParts) stage(s_lo + 1, 1, 1);
+    }
     wait_and_meet();
     step16(0, 0);
-    // While one buffer is read, the next step is on its way to the other.  Before its last sixteen products a wave has the last
-    // of a buffer in hand: when they meet, the buffer can be filled anew, and the other has landed, this wave's share
-    // of it, then everybody's.  (Behind the last step there is no other: what is read then is not used.)
+    // While one buffer is read, the next step is on its way to the other.  In the large tiles an operand at a time, between the
+    // products: all of it at once would hold up the products behind it (8192 x 4096 -> 4096 250 us, in two parts 235; in
+    // four, of which the last has too little time to land, 255).  In the small ones, two blocks of which share a
+    // compute unit, all at once (2048 x 2048 -> 2048 28 us, in two parts 31).  Before its last sixteen products a wave has the last of a
+    // buffer in hand: when they meet, the buffer can be filled anew, and the other has landed, this wave's share of
+    // it, then everybody's.  (Behind the last step there is no other: what is read then is not used.)
     int buf = 0;
     for (int step = s_lo; step < s_hi; ++step) {
+        if (kInParts && step + 1 < s_hi) stage(step + 1, buf ^ 1, 1);
 #pragma unroll
         for (int kk = 1; kk < kBK / 16; ++kk) step16(kk, buf);
         wait_and_meet();
-        if (step + 2 < s_hi) stage(step + 2, buf);
+        if (step + 2 < s_hi) {
+            stage(step + 2, buf, 0);
+            if (!kInParts) stage(step + 2, buf, 1);
+        }
         buf ^= 1;
         step16(0, buf);
     }
