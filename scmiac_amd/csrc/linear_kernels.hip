@@ -746,11 +746,11 @@ hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
 // value e of lane l, four columns each).  The memory pipe writes lane after lane, row after row, and reading one chunk
 // of many rows would hit the same banks every time; so a lane fetches the chunk that belongs there once rows
 // are turned against each other, and the reads look it up.
-// The transposing reads are written out, with their wait: the compiler's form of them waits for all that the memory pipe
-// fetches as well, that is for the next step's tiles.  Forward 8192 x 4096 -> 4096 in bf16 255 us = 1.08 PFLOP/s; with
-// its backward, gelu and residual 850 us, against 890 us with turned copies of the operands.  Without the MFMAs' operand
-// reads the loads alone take 151 us of the 255, without the loads reads and MFMAs 186 us: L2 and LDS share the
-// bound.  Longer pipelines, steps of 32, and tiles of 128 x 128 a wave gave nothing.
+// Bound by the LDS (three operand reads to eight products, and the memory pipe's writes) and the clock, beside the matrix pipe:
+// 8192 x 4096 -> 4096 in bf16 235 us = 1.17 PFLOP/s, its backward pass 471; with gelu and residual 805 together, 890 with
+// turned copies of the operands and the compiler's order of the reads.  Without the loads from memory it takes 202 us
+// (with operands of zeros, at a higher clock, 152 and with the loads 186).  Tiles of 128 x 128 a wave take
+// 247 us, steps of 32 with three on their way 272, a fifth slot for an operand 243.
 //
 // float32 operands come as three bf16 planes whose sum is the value to 2^-25 or better: the product is
 // the six products of planes that matter (the other three are below 2^-24 of the result), run as one
@@ -1190,14 +1190,16 @@ __global__ __launch_bounds__(kThreads) void linear_bias_kernel(const float* __re
     if (w == 0 && c < cols) dbias[c] = from_f32<T>((run[0][lane] + run[1][lane]) + (run[2][lane] + run[3][lane]));
 }
 
-// Whether a layer goes through the large tiles: of at least 64 inputs and outputs, from 2^30 multiply-adds on (three times as many in float32,
-// of which the small tiles' instructions do a quarter of what six products of planes cost the large ones); below,
-// packing the operands and filling a few tiles cost more than the 64 x 64 tiles' slower inner loop.
-// Forward and backward, large / small tiles, in microseconds: bfloat16 1024 x 512 -> 1024 45 / 40, 765 x 2937 -> 252
-// 57 / 44, 2048 x 1024 -> 1024 57 / 64, 1862 x 2848 -> 293 60 / 88; float32 1024 x 1024 -> 1024 124 / 95,
-// 10412 x 2000 -> 128 334 / 246, 912 x 3499 -> 1098 289 / 280 and with silu 294 / 364, 1079 x 465 -> 10272 382 / 412.
+// Whether a layer goes through the large tiles: with at least 64 inputs and outputs, from 2^30 multiply-adds on (in float32,
+// of which the small tiles' instructions do a quarter of what six products of planes cost the large ones, with
+// at least 128 and from three times as many on); below, packing the operands and filling a few tiles cost more than the
+// 64 x 64 tiles' slower inner loop.  Forward and backward, large / small tiles, in microseconds: bfloat16
+// 1024 x 512 -> 1024 45 / 40, 765 x 2937 -> 252 57 / 44, 2048 x 1024 -> 1024 57 / 64, 8192 x 64 -> 8192 153 / 164; float32
+// 1024 x 1024 -> 1024 124 / 81, 10412 x 2000 -> 128 321 / 205, 912 x 3499 -> 1098 270 / 280 and with silu 270 / 364,
+// 16384 x 4096 -> 120 760 / 571 and with gelu 766 / 774, 100 000 x 64 -> 512 664 / 261.
 bool is_large(long long rows, long long cols, long long depth, int dtype) {
-    if (rows <= kFewRows || cols < 64 || depth < 64) return false;
+    const int least = dtype == 0 ? 128 : 64;
+    if (rows <= kFewRows || cols < least || depth < least) return false;
     if (rows > kMaxLd || cols > kMaxLd || depth > kMaxLd) return false;
     return (double)rows * (double)cols * (double)depth >= (dtype == 0 ? 3221225472.0 : 1073741824.0);
 }
@@ -1212,13 +1214,13 @@ GemmPlan plan_gemm(long long rows, long long cols, long long depth, int pairs) {
     GemmPlan g;
     g.steps = (int)ceil_div(depth, kBK) * pairs;
     // By expected time.  A step of one small tile on a compute unit takes 0.68 us, of two at a time 1.13; of a large one,
-    // which has the unit to itself, 2.0 with all units at work and less with fewer.  Where there are few small tiles the
+    // which has the unit to itself, 1.85 with all units at work and less with fewer.  Where there are few small tiles the
     // contraction is cut into pieces; joining costs a launch and the partial sums' way to memory and back (4 bytes a value
-    // each way, 4 TB/s).  bfloat16 with large / small tiles, 4096 inputs: 4096 x 4096 130 / 153 us, 3584 x 3584 115 / 134,
-    // 2816 x 2560 113 / 86, 3840 x 4864 (29 large tiles over) 223 / 182; 2048 x 2048 x 2048 in two pieces 41, in one 28.
+    // each way, 4 TB/s).  bfloat16 with large / small tiles, 4096 inputs: 4096 x 4096 123 / 146 us, 3584 x 3584 107 / 130,
+    // 2816 x 2560 92 / 79, 3840 x 4864 (29 large tiles over) 195 / 176; 2048 x 2048 x 2048 in two pieces 41, in one 28.
     const long long t256 = ceil_div(rows, 256) * ceil_div(cols, 256), t128 = ceil_div(rows, 128) * ceil_div(cols, 128);
     const long long over = t256 % 256;
-    const double large = g.steps * ((t256 / 256) * 2.0 + (over ? 1.5 + over / 512.0 : 0.0));
+    const double large = g.steps * ((t256 / 256) * 1.85 + (over ? 1.35 + over / 512.0 : 0.0));
     long long s = 1;
     double small = 1e30;
     for (long long c = 1; c <= 32 && (c == 1 || c * 4 <= g.steps); ++c) {
