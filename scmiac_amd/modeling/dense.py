@@ -19,7 +19,8 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
     ``x [..., k]``, ``weight [n, k]``, ``bias [n]``, ``residual [..., n]``: all float32, float16 or bfloat16 and on
     one device; the result has their type.  ``activation``: ``"none"``, ``"relu"``, ``"gelu"`` (with the error
     function) or ``"silu"``.  Gradients of all four; not differentiable twice.  ``x``, ``weight`` and ``residual``
-    may be strided; in float32 the product is as exact as float32 sums allow."""
+    may be strided; in float32 the product is as exact as float32 sums allow.  What an infinity or a NaN reaches is not
+    finite; a large float32 layer makes NaN of it where smaller ones may keep the infinity."""
     _hip._cuda_device(x, "x")
     act = _hip.ACTIVATIONS.get(activation)
     if act is None:

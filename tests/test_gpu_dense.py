@@ -282,3 +282,23 @@ def test_half_precision_pre_activations_beyond_the_type():
         dx, dw = torch.autograd.grad(y, [xx, ww], torch.ones_like(y))
         assert not y[0].any() and not y[2].any() and torch.isinf(y[1]).all()
         assert dx.flatten().tolist() == [0.0, 750.0, 0.0, 750.0] and dw.flatten().tolist() == [301.0] * 3
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(40, 96, 70), (2056, 1048, 2001)])
+def test_what_is_not_finite_stays_in_its_row(m, k, n, dtype):
+    x, w, b, _, dy = _make(m, k, n, dtype, seed=11, residual=False)
+    clean = linear_act(x, w, b)
+    for bad in (math.inf, -math.inf, math.nan):
+        spoilt = x.clone()
+        spoilt[m // 2, k - 1] = bad
+        y = linear_act(spoilt, w, b)
+        hit = w[:, k - 1] != 0
+        assert not torch.isfinite(y[m // 2][hit]).any()
+        rest = torch.arange(m, device="cuda") != m // 2
+        assert torch.equal(y[rest], clean[rest])
+        leaf = spoilt.requires_grad_()
+        weight = w.clone().requires_grad_()
+        dx, dw = torch.autograd.grad(linear_act(leaf, weight, b), (leaf, weight), dy)
+        assert torch.isfinite(dx).all() and torch.isfinite(dw[:, :k - 1]).all()
+        assert not torch.isfinite(dw[dy[m // 2] != 0, k - 1]).any()
