@@ -777,7 +777,7 @@ hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
 // of many rows would hit the same banks every time; so a lane fetches the chunk that belongs there once rows
 // are turned against each other, and the reads look it up.
 // Bound by the LDS (three operand reads to eight products, and the memory pipe's writes) and the clock, beside the matrix pipe:
-// 8192 x 4096 -> 4096 in bf16 235 us = 1.17 PFLOP/s, its backward pass 471; with gelu and residual 805 together, 890 with
+// 8192 x 4096 -> 4096 in bf16 235 us = 1.17 PFLOP/s, its backward pass 471; with gelu and residual 783 together, 890 with
 // turned copies of the operands and the compiler's order of the reads.  Without the loads from memory it takes 202 us
 // (with operands of zeros, at a higher clock, 152 and with the loads 186).  Tiles of 128 x 128 a wave take
 // 247 us, steps of 32 with three on their way 272, a fifth slot for an operand 243.
@@ -911,8 +911,10 @@ struct Fragments<F, true> {
 };
 
 // One step of sixteen: C += the products of the fragments x, y, while the next ones are on their way from LDS.  Written
-// out in one block with its wait, since the compiler gathers a step's reads in front of its products.  (The
-// products of a block go to different accumulators, so that none waits for another.)
+// out in one block with its wait, since the compiler gathers a step's reads in front of its products.  The products of a
+// block go to different accumulators, and the next use of one is the same product of the next block, three others
+// and two wait states (s_nop 1, which also keeps a copied fragment's distance) later: accumulating needs no more.  What reads
+// the sums otherwise comes after settle().
 #define SCMIAC_MUL(t, i, j) "v_mfma_f32_32x32x16_" t " %[c" #i #j "], %[x" #i "], %[y" #j "], %[c" #i #j "]\n\t"
 #define SCMIAC_ROW(v, f, off) "ds_read_b128 %[" #v #f "], %[" #v "at0] offset:" #off "\n\t"
 #define SCMIAC_TURNED(v, f, odd, off)                                            \
