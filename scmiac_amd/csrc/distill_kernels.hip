@@ -7,9 +7,10 @@
 //   distill backward dL/dx_j = (tau p_j - sum_{i: idx_i = j} t_i) / T,   p = softmax(x / T)
 //
 // All of it is bound by reading the rows once (and, backward, writing them once): one pass keeps a running
-// maximum m and sum of exponentials s per lane, s = sum exp2((x - m) c) with c = log2(e) / T for v_exp_f32.  The
-// difference comes first: x c alone overflows for the lowest values of float32 and bfloat16, which serve as
-// masks, and near the maximum, where the weight is, it is exact.  A row belongs to one wave (short
+// maximum m and sum of exponentials s per lane, s = sum exp2((x - m) c) with c = log2(e) / T for v_exp_f32.  In the
+// loss the difference comes first (LseAcc): x c alone overflows for the lowest values of float32 and bfloat16, which serve as
+// masks, and near the maximum, where the weight is, it is exact.  top_logits folds it into one multiply-add as long as
+// |x| c is below 2^24 (WaveLse).  A row belongs to one wave (short
 // rows), to the four waves of a block, or to several blocks whose results a second kernel joins (few rows).
 #include <hip/hip_runtime.h>
 
@@ -86,7 +87,9 @@ __device__ __forceinline__ float lse_value(const LseAcc& a, float inv_t) {
 // The same for a wave that has seen a sample of its entries: one reference r for all lanes and no running
 // maximum.  An entry may exceed r by up to 64 in the exponent before it is moved (the sum stays
 // far from overflow), and (x - r) c is one multiply-add with the product r c rounded; what that rounding does to
-// all terms alike is taken out at the end.  Where r c would overflow (masks at the lowest value), the difference comes first.
+// all terms alike, a factor 2^err, is taken out at the end.  From |r| c = 2^24 on (finite masks like -1e9 and below, a
+// type's lowest value, small temperatures) the difference comes first: err, up to half a step of r c, is at most 1/2 below and would
+// soon be an exponent that overflows.
 struct WaveLse {
     float r, rc, err, limit, s;
     int far;
@@ -97,7 +100,7 @@ struct WaveLse {
     __device__ __forceinline__ void refer(float to, float c) {
         s *= fast_exp2((r - to) * c - err);
         r = to;
-        far = uniform((int)!(fabsf(r) * c < 1e37f));
+        far = uniform((int)!(fabsf(r) * c < 16777216.f));
         rc = far ? 0.f : r * c;
         err = far ? 0.f : fmaf(r, c, -rc);
         limit = r + 64.f / c;

@@ -396,3 +396,35 @@ def test_a_teacher_of_vanishing_weight_still_counts():
     assert rows[0] == 0 and rows[1] == 0
     # the mean is over the three rows that have a teacher
     torch.testing.assert_close(topk_distill(x, idx, top, teacher_lse=lse), rows.sum() / 3, rtol=1e-6, atol=0)
+
+
+# ------------------------------------------------------------------ values far from the rest of their row
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(8, 200), (8, 3000), (2049, 3000), (8, 40000)])
+def test_top_logits_of_finite_masks_and_of_large_logits(n, v, dtype):
+    """Rows, starts, ends and whole pieces of rows at finite mask values, and logits as large the other way.
+
+    The log-sum-exp is m / T + log s: 1 / T and the sum rounded, 2^-22 of |m| / T with room, and s off by at most
+    2^-23 for every addition to a lane's part of it, and as much for terms whose exponents are a few hundred at most."""
+    x = _rand(n, v, 1, dtype, seed=13)[0]
+    masks = [-6e4, -3e4, -100.0] if dtype == torch.float16 else [-1e9, -5e9, -1e10, -1e12, -1e30, -1e36]
+    for mask in masks:
+        m = x.clone()
+        m[0] = mask
+        m[1, :3 * v // 4] = mask
+        m[2, v // 4:] = mask
+        m[3, :v // 2] = mask
+        m[3, 0] = mask * 1.05
+        m[4] = -mask
+        m[5, v // 3] = -mask
+        m[6, ::2] = mask
+        m[7, v // 2:] = mask
+        m[7, :v // 2] = mask * 1.05
+        order = torch.sort(m.float(), dim=1, descending=True, stable=True).indices[:, :5]
+        for T in (1e-5, 1e-3, 1.0) if dtype == torch.float16 else (0.1, 1.0, 30.0):
+            values, idx, lse = top_logits(m, 5, T)
+            assert torch.equal(idx.long(), order) and torch.equal(values, m.gather(1, order))
+            wide = m.double() / T
+            bound = 2.0 ** -22 * wide.amax(1).abs() + 2.0 ** -23 * (v / 64 + 300)
+            assert bool(((lse.double() - torch.logsumexp(wide, 1)).abs() <= bound).all()), (mask, T)
