@@ -279,7 +279,7 @@ __device__ __forceinline__ int shrink_list(u64* buf, int cnt, int k, int slack, 
 template <typename T>
 struct WaveList {
     static constexpr int kTrigger = 256;
-    static constexpr int kCap = kTrigger + 64 * 4;             // four elements of every lane add up to 256 entries
+    static constexpr int kCap = kTrigger + 64 * 4;             // a lot of push_careful adds up to 256 entries
     u64* buf;
     int cnt, k;
     float tau;      // k entries of the list are >= tau; all of them came earlier, so a later entry must exceed it
@@ -314,17 +314,20 @@ struct WaveList {
             append(ballot(take), take, f[i], first + i);
         }
     }
-    // The same with room made first; also while everything is taken (`valid` entries of the lane are real).
+    // The same with room made first; also while everything is taken (`valid` entries of the lane are real).  256 entries at a
+    // time, ascending in index from one lot to the next (of the half types' eight a lane, 32 lanes each): tau may move in
+    // between, and leaves out an equal value only if k entries in front of it are kept.
     template <int N>
     __device__ __forceinline__ void push_careful(const float (&f)[N], uint32_t first, int valid) {
+        constexpr int kLots = N / 4;
 #pragma unroll 1
-        for (int h = 0; h < N; h += 4) {
+        for (int h = 0; h < kLots; ++h) {
             room();
+            const bool turn = kLots == 1 || (int)(threadIdx.x & 63) / (64 / kLots) == h;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = (N > 4 && h) ? f[N - 4 + i] : f[i];
-                const bool take = h + i < valid && (open || x > tau);
-                append(ballot(take), take, x, first + h + i);
+            for (int i = 0; i < N; ++i) {
+                const bool take = turn && i < valid && (open || f[i] > tau);
+                append(ballot(take), take, f[i], first + i);
             }
         }
     }

@@ -428,3 +428,19 @@ def test_top_logits_of_finite_masks_and_of_large_logits(n, v, dtype):
             wide = m.double() / T
             bound = 2.0 ** -22 * wide.amax(1).abs() + 2.0 ** -23 * (v / 64 + 300)
             assert bool(((lse.double() - torch.logsumexp(wide, 1)).abs() <= bound).all()), (mask, T)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("n,v", [(6, 1001), (6, 1023), (6, 3001), (2052, 3001), (6, 10411), (6, 40003)])
+def test_top_logits_of_equal_values_in_rows_that_start_anywhere(n, v, dtype):
+    gen = torch.Generator(device="cuda").manual_seed(v)
+    at = torch.arange(v + 1, device="cuda")
+    x = torch.randint(0, 3, (n, v + 1), device="cuda", generator=gen).float()
+    x[0] = 1.0
+    x[1] = torch.where(at % 97 == 5, 2.0, -math.inf)
+    x[2] = -math.inf
+    x[3] = (torch.randn(v + 1, device="cuda", generator=gen) * 2).round()
+    x = x.to(dtype)
+    for rows in (x[:, :v], x[:, 1:], x[:, 1:v], x[:, :v].contiguous()):
+        for k in (1, 16, 33, 64):
+            _check_top(rows, k)
