@@ -59,12 +59,12 @@ struct LseAcc {
     // another sum, of entries up to its maximum om
     __device__ __forceinline__ void join(float om, float os, float c) {
         raise(om, c);
-        if (om != -INFINITY) s += os * fast_exp2((om - r) * c);
+        if (om != -INFINITY) s += om == m ? os : os * fast_exp2((om - r) * c);      // (om may be +inf)
     }
     // all lanes of the wave
     __device__ __forceinline__ void join_wave(float c) {
         const float top = wave_max(m);
-        s = wave_sum((m == -INFINITY) ? s : s * fast_exp2((m - top) * c));   // (a NaN stays)
+        s = wave_sum((m == -INFINITY || m == top) ? s : s * fast_exp2((m - top) * c));   // (a NaN stays)
         m = top;
         r = (top == -INFINITY) ? 0.f : top;
     }
@@ -75,11 +75,11 @@ __device__ __forceinline__ LseAcc join_pairs(const float2* p, int n, float c) {
     a.init();
     for (int i = 0; i < n; ++i) a.m = fmaxf(a.m, p[i].x);
     a.r = (a.m == -INFINITY) ? 0.f : a.m;
-    for (int i = 0; i < n; ++i) a.s += (p[i].x == -INFINITY) ? p[i].y : p[i].y * fast_exp2((p[i].x - a.r) * c);
+    for (int i = 0; i < n; ++i) a.s += (p[i].x == -INFINITY || p[i].x == a.m) ? p[i].y : p[i].y * fast_exp2((p[i].x - a.r) * c);
     return a;
 }
 __device__ __forceinline__ float lse_value(const LseAcc& a, float inv_t) {
-    if (a.m == INFINITY) return a.m;
+    if (a.m == INFINITY && a.s == a.s) return a.m;
     if (a.s == 0.f) return -INFINITY;               // every entry -inf
     return fmaf(a.m == -INFINITY ? 0.f : a.m, inv_t, kLn2 * log2f(a.s));
 }
@@ -114,7 +114,7 @@ struct WaveLse {
             for (int i = 0; i < N; ++i) s += fast_exp2(fmaf(f[i], c, -rc));
         } else {
 #pragma unroll
-            for (int i = 0; i < N; ++i) s += fast_exp2((f[i] - r) * c);
+            for (int i = 0; i < N; ++i) s += f[i] == r ? 1.f : fast_exp2((f[i] - r) * c);      // (r may be +inf)
         }
     }
     __device__ __forceinline__ LseAcc finish() {

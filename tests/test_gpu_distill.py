@@ -444,3 +444,14 @@ def test_top_logits_of_equal_values_in_rows_that_start_anywhere(n, v, dtype):
     for rows in (x[:, :v], x[:, 1:], x[:, 1:v], x[:, :v].contiguous()):
         for k in (1, 16, 33, 64):
             _check_top(rows, k)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [150, 5000, 40000])
+def test_top_logits_of_a_nan_beside_an_infinity(v, dtype):
+    x = _rand(8, v, 1, dtype, seed=3)[0]
+    for row, (i, j) in enumerate([(0, 1), (1, 0), (0, v - 1), (v - 1, 0), (v // 2, v // 2 + 1), (v // 3, 2 * v // 3)]):
+        x[row, i], x[row, j] = math.inf, math.nan
+    x[6, [0, v // 2, v - 1]] = math.inf
+    lse = top_logits(x, 3)[2]
+    assert torch.isnan(lse[:6]).all() and lse[6] == math.inf and torch.isfinite(lse[7])
