@@ -59,7 +59,7 @@ struct LseAcc {
     // another sum, of entries up to its maximum om
     __device__ __forceinline__ void join(float om, float os, float c) {
         raise(om, c);
-        if (om != -INFINITY) s += om == m ? os : os * fast_exp2((om - r) * c);      // (om may be +inf)
+        s += om == m || om == -INFINITY ? os : os * fast_exp2((om - r) * c);      // (om may be +inf; of -inf, os is 0 or NaN)
     }
     // all lanes of the wave
     __device__ __forceinline__ void join_wave(float c) {

@@ -455,3 +455,22 @@ def test_top_logits_of_a_nan_beside_an_infinity(v, dtype):
     x[6, [0, v // 2, v - 1]] = math.inf
     lse = top_logits(x, 3)[2]
     assert torch.isnan(lse[:6]).all() and lse[6] == math.inf and torch.isfinite(lse[7])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [150, 5000, 40000, 420000])
+def test_a_nan_among_masked_classes_is_seen(v, dtype):
+    x = torch.full((4, v), -math.inf, device="cuda", dtype=dtype)
+    x[:, :20] = 1.0
+    x[2, : v // 2 - 1] = 1.0
+    x[2, v // 2 + v // 8:] = 1.0
+    x[0, v - 3] = math.nan
+    x[1] = x[1].flip(0)
+    x[1, 5] = math.nan
+    x[2, v // 2] = math.nan
+    want = [True, True, True, False]
+    lse = top_logits(x, 3)[2]
+    idx = torch.zeros(4, 2, dtype=torch.int32, device="cuda")
+    idx[1] = v - 1
+    loss = topk_distill(x, idx, torch.zeros(4, 2, device="cuda"), reduction="none")
+    assert (torch.isnan(lse).tolist(), torch.isnan(loss).tolist()) == (want, want)
