@@ -413,8 +413,8 @@ SCMIAC_API int scmiac_top_logits(const void *x, int64_t ld, int64_t n, int64_t v
  *     L   = sum_i t_i (log t_i - log softmax(x / T)[idx_i])
  *   idx [n, k] int32, top [n, k] float32, teacher_lse [n] float32 or NULL, x of `dtype`, rows ld apart.
  *   idx -1 is padding, and a weight t_i of 0 contributes nothing.  A class may be listed more than once.  A row
- *   without a teacher (all padding, or all a_i -inf) and a row whose classes are all -inf have L = 0 and no
- *   gradient.  An idx below -1 or from v on, or a listed a_i that is NaN, makes the row's L and gradient NaN.
+ *   without a teacher (all padding, or all a_i -inf), whatever its logits hold, and a row whose classes are all -inf
+ *   have L = 0 and no gradient.  An idx below -1 or from v on, or a listed a_i that is NaN, makes the row's L and gradient NaN.
  * forward: reduction SCMIAC_REDUCE_NONE: loss [n]; _MEAN: loss [1] over the rows that count (those not
  *   described above as L = 0), 0 if there are none; _SUM: loss [1].  row_stats [4 n] and scale [1]
  *   (MEAN, SUM) float32 are what backward reads.

@@ -724,7 +724,7 @@ __device__ __forceinline__ void finish_row(const T* __restrict__ xr, long long v
     if (lane == 0) {
         float value = empty ? 0.f : kLn2 * fmaf(tau, log2f(acc.s), part);
         float share = empty ? -1.f : tau / acc.s;
-        if (bad || acc.s != acc.s) value = share = NAN;
+        if (bad || (!empty && acc.s != acc.s)) value = share = NAN;      // (a row without a teacher may hold anything)
         loss[row] = value;
         stats[row] = make_float4(acc.r, share, ref, log_sum);
     }

@@ -474,3 +474,23 @@ def test_a_nan_among_masked_classes_is_seen(v, dtype):
     idx[1] = v - 1
     loss = topk_distill(x, idx, torch.zeros(4, 2, device="cuda"), reduction="none")
     assert (torch.isnan(lse).tolist(), torch.isnan(loss).tolist()) == (want, want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("v", [64, 1500, 40000])
+def test_rows_without_a_teacher_may_hold_anything(v, dtype):
+    x, idx, top, _ = _rand(8, v, 5, dtype, seed=21, pads=False)
+    idx[[1, 3, 5]] = -1
+    top[6] = -math.inf
+    clean = topk_distill(x[[0, 2, 4, 7]], idx[[0, 2, 4, 7]], top[[0, 2, 4, 7]], reduction="none")
+    x[1], x[3, v // 2], x[5, ::3], x[6, v - 1] = math.nan, math.nan, math.inf, math.nan
+    for reduction in ("none", "sum", "mean"):
+        leaf = x.detach().requires_grad_()
+        loss = topk_distill(leaf, idx, top, reduction=reduction)
+        dx, = torch.autograd.grad(loss.sum(), [leaf])
+        assert not dx[[1, 3, 5, 6]].any() and torch.isfinite(dx).all()
+        if reduction == "none":
+            assert not loss[[1, 3, 5, 6]].any() and torch.equal(loss[[0, 2, 4, 7]], clean)
+        else:      # summed in 64 bits and rounded; the division rounds once more
+            want = float(clean.double().sum()) / (4 if reduction == "mean" else 1)
+            assert abs(loss.item() - want) <= 2.0 ** -23 * abs(want)
