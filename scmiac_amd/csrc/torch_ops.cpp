@@ -7,6 +7,8 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -115,18 +117,24 @@ struct Scratch {
 };
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
-// Stands behind the gradients of a backward pass that was itself recorded (create_graph): they have no derivative.
-struct Final : torch::autograd::Function<Final> {
-    static Tensor forward(AutogradContext*, const Tensor& grad, const Tensor&) { return grad.detach(); }
-    static variable_list backward(AutogradContext*, variable_list) {
-        TORCH_CHECK(false, "this operator is not differentiable twice");
-        return {};
-    }
-};
-void close(variable_list& grads, const Tensor& input) {
-    if (!at::GradMode::is_enabled() || !input.defined() || !input.requires_grad()) return;
+// Gradients of a backward pass that was itself recorded (create_graph) have no derivative: a node that says so stands
+// between them and every input of the pass that requires a gradient, whether or not it was kept for this pass, and
+// the gradient `given` to it.
+void close(variable_list& grads, const Tensor& given) {
+    if (!at::GradMode::is_enabled()) return;
+    torch::autograd::edge_list edges;
+    const std::shared_ptr<torch::autograd::Node> self = torch::autograd::get_current_node();
+    TORCH_CHECK(self, "create_graph needs the autograd engine");
+    for (const torch::autograd::Edge& e : self->next_edges())
+        if (e.is_valid()) edges.push_back(e);
+    if (given.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(given));
+    const std::shared_ptr<torch::autograd::Node> last(
+        new torch::autograd::Error("this operator is not differentiable twice", std::move(edges)), torch::autograd::deleteNode);
     for (Tensor& g : grads)
-        if (g.defined()) g = Final::apply(g, input);
+        if (g.defined()) {
+            g = g.detach();
+            torch::autograd::set_history(g, last);
+        }
 }
 
 // ------------------------------------------------------------------ dense layer
@@ -189,9 +197,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             check(lib.linear_backward(x.data(), x.ld, w.data(), w.ld, in_ptr(saved[2]), in_ptr(dy), m, n, k, code, (int)act,
                                       out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]), ws.data(), ws.bytes, stream_of(dy)));
         }
-        Tensor input = saved[0].defined() && saved[0].requires_grad() ? saved[0] : saved[1];
-        if (!(input.defined() && input.requires_grad())) input = given;
-        close(out, input);
+        close(out, given);
         return out;
     }
 };
@@ -303,7 +309,7 @@ struct TopkDistill : torch::autograd::Function<TopkDistill> {
                                        static_cast<const float*>(in_ptr(scale)), out_ptr(dx), ldd, stream_of(logits)));
             out[0] = dx;
         }
-        close(out, logits);
+        close(out, grad);
         return out;
     }
 };

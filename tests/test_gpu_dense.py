@@ -302,3 +302,21 @@ def test_what_is_not_finite_stays_in_its_row(m, k, n, dtype):
         dx, dw = torch.autograd.grad(linear_act(leaf, weight, b), (leaf, weight), dy)
         assert torch.isfinite(dx).all() and torch.isfinite(dw[:, :k - 1]).all()
         assert not torch.isfinite(dw[dy[m // 2] != 0, k - 1]).any()
+
+
+@pytest.mark.parametrize("trained", ["w", "b", "wb", "x", "xw", "xwb"])
+def test_second_derivatives_are_refused_whatever_is_trained(trained):
+    t = {"x": torch.randn(6, 5, device="cuda"), "w": torch.randn(4, 5, device="cuda"), "b": torch.randn(4, device="cuda")}
+    leaves = [t[name].requires_grad_() for name in trained]
+    for act in ACTS:
+        y = linear_act(t["x"], t["w"], t["b"], activation=act)
+        grads = torch.autograd.grad(y, leaves, torch.ones_like(y), create_graph=True)
+        for g, same in zip(grads, torch.autograd.grad(linear_act(t["x"], t["w"], t["b"], activation=act), leaves, torch.ones_like(y))):
+            assert torch.equal(g, same)
+        for g in grads:      # a penalty on a gradient, beside a term that has a derivative of its own
+            for leaf in leaves:
+                with pytest.raises(RuntimeError, match="differentiable twice"):
+                    torch.autograd.grad(g.square().sum() + leaf.sum(), leaf, retain_graph=True)
+    # a recorded pass is no harm where no second derivative is asked for
+    y = linear_act(t["x"], t["w"], t["b"], activation="gelu")
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(y.sum(), leaves, create_graph=True))

@@ -494,3 +494,13 @@ def test_rows_without_a_teacher_may_hold_anything(v, dtype):
         else:      # summed in 64 bits and rounded; the division rounds once more
             want = float(clean.double().sum()) / (4 if reduction == "mean" else 1)
             assert abs(loss.item() - want) <= 2.0 ** -23 * abs(want)
+
+
+def test_second_derivatives_of_the_loss_are_refused():
+    x, idx, top, _ = _rand(4, 30, 3, torch.float32, seed=2)
+    leaf = x.detach().requires_grad_()
+    up = torch.ones(4, device="cuda", requires_grad=True)
+    g, = torch.autograd.grad(topk_distill(leaf, idx, top, reduction="none"), [leaf], up, create_graph=True)
+    for t in (leaf, up):
+        with pytest.raises(RuntimeError, match="differentiable twice"):
+            torch.autograd.grad(g.sum() + t.sum(), t, retain_graph=True)
