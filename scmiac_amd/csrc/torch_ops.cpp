@@ -178,9 +178,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
                    need_b = needed(ctx->saved_data["bias"].toInt());
         const Tensor& given = grads[0];
         variable_list out(5);
-        if (needed(ctx->saved_data["residual"].toInt())) out[3] = given;
-        if (!(need_x || need_w || need_b)) return out;
-        {
+        if (need_x || need_w || need_b) {
             const at::NoGradGuard no_grad;
             const c10::DeviceGuard guard(given.device());
             const int64_t act = ctx->saved_data["act"].toInt(), k = ctx->saved_data["k"].toInt();
@@ -198,6 +196,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
                                       out_ptr(out[0]), out_ptr(out[1]), out_ptr(out[2]), ws.data(), ws.bytes, stream_of(dy)));
         }
         close(out, given);
+        if (needed(ctx->saved_data["residual"].toInt())) out[3] = given;      // (itself, with whatever derivatives it has)
         return out;
     }
 };

@@ -320,3 +320,18 @@ def test_second_derivatives_are_refused_whatever_is_trained(trained):
     # a recorded pass is no harm where no second derivative is asked for
     y = linear_act(t["x"], t["w"], t["b"], activation="gelu")
     assert all(torch.isfinite(g).all() for g in torch.autograd.grad(y.sum(), leaves, create_graph=True))
+
+
+def test_the_gradient_of_the_residual_keeps_its_derivatives():
+    x, w, dy = (torch.randn(*s, device="cuda", requires_grad=True) for s in ((6, 5), (4, 5), (6, 4)))
+    res = torch.randn(6, 4, device="cuda", requires_grad=True)
+    y = linear_act(x, w, None, res, "gelu")
+    dx, dres = torch.autograd.grad(y, [x, res], dy, create_graph=True)
+    assert torch.equal(dres, dy)
+    g, = torch.autograd.grad((dres * 3).sum(), dy, retain_graph=True)      # dres is dy: a derivative of 1
+    assert torch.equal(g, torch.full_like(dy, 3.0))
+    with pytest.raises(RuntimeError, match="differentiable twice"):
+        torch.autograd.grad(dx.sum(), dy)
+    y = linear_act(x.detach(), w.detach(), None, res)
+    dres, = torch.autograd.grad(y, res, dy, create_graph=True)
+    assert torch.equal(torch.autograd.grad((dres * 2).sum(), dy)[0], torch.full_like(dy, 2.0))
