@@ -90,6 +90,11 @@ const Tensor& on_gpu(const OptTensor& t, const char* what, const Tensor& beside)
     return v;
 }
 
+// An input with a tangent (torch.autograd.forward_ad) would lose it.
+void no_tangent(const OptTensor& t, const char* what) {
+    TORCH_CHECK_NOT_IMPLEMENTED(!torch::autograd::isFwGradDefined(t), what, " has a tangent: this operator has no forward-mode derivative");
+}
+
 // a 2-D tensor whose columns lie next to each other, and its row stride
 struct Rows {
     Tensor t;
@@ -209,6 +214,7 @@ Tensor linear_act(const OptTensor& x_, const OptTensor& w_, const OptTensor& bia
     dtype_code(x, "x");
     const Tensor bias = bias_.has_value() ? on_gpu(bias_, "bias", x) : Tensor();
     const Tensor residual = residual_.has_value() ? on_gpu(residual_, "residual", x) : Tensor();
+    no_tangent(x_, "x"), no_tangent(w_, "weight"), no_tangent(bias_, "bias"), no_tangent(residual_, "residual");
     TORCH_CHECK_TYPE(w.scalar_type() == x.scalar_type(), "weight is ", w.scalar_type(), ", x is ", x.scalar_type());
     TORCH_CHECK_TYPE(!bias.defined() || bias.scalar_type() == x.scalar_type(), "bias is ", bias.scalar_type(), ", x is ", x.scalar_type());
     TORCH_CHECK_TYPE(!residual.defined() || residual.scalar_type() == x.scalar_type(), "residual is ", residual.scalar_type(), ", x is ",
@@ -321,6 +327,7 @@ Tensor topk_distill(const OptTensor& logits_, const OptTensor& idx_, const OptTe
     const at::IntArrayRef rows = logits.sizes().slice(0, logits.dim() - 1);
     Tensor idx = on_gpu(idx_, "teacher_idx", logits), top = on_gpu(top_, "teacher_logits", logits),
            lse = lse_.has_value() ? on_gpu(lse_, "teacher_lse", logits) : Tensor();
+    no_tangent(logits_, "logits"), no_tangent(top_, "teacher_logits"), no_tangent(lse_, "teacher_lse");
     TORCH_CHECK_TYPE(at::isIntegralType(idx.scalar_type(), false), "teacher_idx must hold whole numbers, not ", idx.scalar_type());
     TORCH_CHECK_TYPE(at::isFloatingType(top.scalar_type()), "teacher_logits must not be ", top.scalar_type());
     TORCH_CHECK_TYPE(!lse.defined() || at::isFloatingType(lse.scalar_type()), "teacher_lse must not be ", lse.scalar_type());

@@ -4,6 +4,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from scmiac_amd import _hip
 from scmiac_amd.modeling import LinearAct, NeighborDistillLoss, linear_act, top_logits, topk_distill
@@ -126,3 +127,24 @@ def test_python_refusals_of_device_tensors():
         g, = torch.autograd.grad(out(leaf), [leaf], create_graph=True)
         with pytest.raises(RuntimeError):
             torch.autograd.grad(g.sum(), [leaf])
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivatives_are_refused():
+    x, w, b, r = (torch.randn(*s, device="cuda") for s in ((6, 5), (4, 5), (4,), (6, 4)))
+    idx, top = torch.zeros(6, 2, dtype=torch.int32, device="cuda"), torch.zeros(6, 2, device="cuda")
+    lse = torch.zeros(6, device="cuda")
+    with forward_ad.dual_level():
+        def dual(t):
+            return forward_ad.make_dual(t, torch.ones_like(t))
+
+        for call in (lambda: linear_act(dual(x), w, b, r), lambda: linear_act(x, dual(w), b, r), lambda: linear_act(x, w, dual(b), r),
+                     lambda: linear_act(x, w, b, dual(r)), lambda: topk_distill(dual(x), idx, top),
+                     lambda: topk_distill(x, idx, dual(top)), lambda: topk_distill(x, idx, top, 1.0, dual(lse)),
+                     lambda: NeighborDistillLoss()(dual(x), w, idx, top)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(NotImplementedError, match="forward-mode"):
+                    call()
+        values, _, _ = top_logits(dual(x), 2)                       # a teacher is a constant
+        assert forward_ad.unpack_dual(values).tangent is None
+        linear_act(x, w, b, r), topk_distill(x, idx, top)           # without tangents as ever
