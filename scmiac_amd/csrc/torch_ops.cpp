@@ -5,10 +5,12 @@
 // ctypes call cost more than the kernels.  The library is bound by path at import (bind), so that this module and
 // the ctypes binding use the same one.
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <optional>
@@ -88,6 +90,13 @@ const Tensor& on_gpu(const OptTensor& t, const char* what, const Tensor& beside)
     const Tensor& v = on_gpu(t, what);
     TORCH_CHECK_VALUE(v.device() == beside.device(), what, " is on ", v.device(), ", not on ", beside.device());
     return v;
+}
+
+// A recorder of torch's operators would see the outputs made and never what fills them.
+void no_recorder() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                "this operator cannot be traced (torch.jit.trace, torch.export, make_fx)");
 }
 
 // An input with a tangent (torch.autograd.forward_ad) would lose it.
@@ -209,6 +218,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
 OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 Tensor linear_act(const OptTensor& x_, const OptTensor& w_, const OptTensor& bias_, const OptTensor& residual_, int64_t act) {
+    no_recorder();
     const Tensor& x = on_gpu(x_, "x");
     const Tensor& w = on_gpu(w_, "weight", x);
     dtype_code(x, "x");
@@ -239,6 +249,7 @@ Tensor linear_act(const OptTensor& x_, const OptTensor& w_, const OptTensor& bia
 // ------------------------------------------------------------------ top logits
 
 std::tuple<Tensor, Tensor, Tensor> top_logits(const OptTensor& logits_, int64_t k, double temperature) {
+    no_recorder();
     const Tensor logits = on_gpu(logits_, "logits").detach();
     const int code = dtype_code(logits, "logits");
     TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits need at least one class");
@@ -321,6 +332,7 @@ struct TopkDistill : torch::autograd::Function<TopkDistill> {
 
 Tensor topk_distill(const OptTensor& logits_, const OptTensor& idx_, const OptTensor& top_, const OptTensor& lse_, double temperature,
                     double own_temperature, int64_t reduction) {
+    no_recorder();
     const Tensor& logits = on_gpu(logits_, "logits");
     dtype_code(logits, "logits");
     TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits need at least one class");

@@ -5,6 +5,7 @@ import ctypes
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 from scmiac_amd import _hip
 from scmiac_amd.modeling import LinearAct, NeighborDistillLoss, linear_act, top_logits, topk_distill
@@ -148,3 +149,16 @@ def test_forward_mode_derivatives_are_refused():
         values, _, _ = top_logits(dual(x), 2)                       # a teacher is a constant
         assert forward_ad.unpack_dual(values).tangent is None
         linear_act(x, w, b, r), topk_distill(x, idx, top)           # without tangents as ever
+
+
+@pytest.mark.gpu
+def test_tracing_is_refused():
+    x, w = torch.randn(6, 5, device="cuda"), torch.randn(4, 5, device="cuda")
+    idx, top = torch.zeros(6, 2, dtype=torch.int32, device="cuda"), torch.zeros(6, 2, device="cuda")
+    for call in (lambda t: linear_act(t, w), lambda t: top_logits(t, 2), lambda t: topk_distill(t, idx, top)):
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(call, (x,))
+        for mode in ("real", "fake"):
+            with pytest.raises(RuntimeError, match="cannot be traced"):
+                make_fx(call, tracing_mode=mode)(x)
+        call(x)
