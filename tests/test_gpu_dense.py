@@ -335,3 +335,18 @@ def test_the_gradient_of_the_residual_keeps_its_derivatives():
     y = linear_act(x.detach(), w.detach(), None, res)
     dres, = torch.autograd.grad(y, res, dy, create_graph=True)
     assert torch.equal(torch.autograd.grad((dres * 2).sum(), dy)[0], torch.full_like(dy, 2.0))
+
+
+def test_float32_gelu_keeps_its_digits_where_it_is_small():
+    """z = x * 1 is exact here.  P(z) = erfc(a) / 2, a = -z / sqrt(2) off by two roundings of 2^-24, moves by 2 a^2 <= 64 times
+    as much, 2^-17, and erfc by a few 2^-24 of its own: 2^-16 of gelu in all.  In the slope, P + z phi, the exponent z^2 / 2
+    (46 as a power of two) carries four roundings, 2^-17 of phi, and the two terms of opposite sign add up to 1.3 times
+    the sum at most: 2^-15."""
+    z = torch.linspace(-8, -3, 501, device="cuda").reshape(-1, 1).requires_grad_()
+    y = linear_act(z, torch.ones(1, 1, device="cuda"), activation="gelu")
+    slope, = torch.autograd.grad(y, z, torch.ones_like(y))
+    d = z.detach().double()
+    p = torch.special.erfc(-d / math.sqrt(2)) / 2
+    want = p + d * torch.exp(-d * d / 2) / math.sqrt(2 * math.pi)
+    assert bool(((y.detach().double() - d * p).abs() <= 2.0 ** -16 * (d * p).abs()).all())
+    assert bool(((slope.double() - want).abs() <= 2.0 ** -15 * want.abs()).all())
