@@ -80,14 +80,17 @@ int dtype_code(const Tensor& t, const char* what) {
     }
 }
 
+// The kernels read memory as it is: a negation that a view has pending (imag of a conjugate) is carried out first.
+Tensor as_stored(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 // The kernels take device pointers: a host pointer handed to them is a memory fault, not an exception.
-const Tensor& on_gpu(const OptTensor& t, const char* what) {
+Tensor on_gpu(const OptTensor& t, const char* what) {
     TORCH_CHECK_VALUE(t.has_value() && t->defined() && t->is_cuda(), what, " must be a tensor on a GPU device (got ",
                       t.has_value() && t->defined() ? t->device().str() : std::string("none"), "); there is no CPU path");
-    return *t;
+    return as_stored(*t);
 }
-const Tensor& on_gpu(const OptTensor& t, const char* what, const Tensor& beside) {
-    const Tensor& v = on_gpu(t, what);
+Tensor on_gpu(const OptTensor& t, const char* what, const Tensor& beside) {
+    const Tensor v = on_gpu(t, what);
     TORCH_CHECK_VALUE(v.device() == beside.device(), what, " is on ", v.device(), ", not on ", beside.device());
     return v;
 }
@@ -197,7 +200,7 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
             const c10::DeviceGuard guard(given.device());
             const int64_t act = ctx->saved_data["act"].toInt(), k = ctx->saved_data["k"].toInt();
             const Rows x(need_w ? saved[0] : Tensor()), w(need_x ? saved[1] : Tensor());
-            const Tensor dy = given.contiguous();
+            const Tensor dy = as_stored(given).contiguous();
             const int64_t m = dy.size(0), n = dy.size(1);
             const int code = dtype_code(dy, "the gradient");
             Scratch ws;
@@ -219,8 +222,8 @@ OptTensor given(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor
 
 Tensor linear_act(const OptTensor& x_, const OptTensor& w_, const OptTensor& bias_, const OptTensor& residual_, int64_t act) {
     no_recorder();
-    const Tensor& x = on_gpu(x_, "x");
-    const Tensor& w = on_gpu(w_, "weight", x);
+    const Tensor x = on_gpu(x_, "x");
+    const Tensor w = on_gpu(w_, "weight", x);
     dtype_code(x, "x");
     const Tensor bias = bias_.has_value() ? on_gpu(bias_, "bias", x) : Tensor();
     const Tensor residual = residual_.has_value() ? on_gpu(residual_, "residual", x) : Tensor();
@@ -307,7 +310,8 @@ struct TopkDistill : torch::autograd::Function<TopkDistill> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const variable_list saved = ctx->get_saved_variables();
-        const Tensor &logits = saved[0], &idx = saved[1], &top = saved[2], &stats = saved[3], &scale = saved[4], &grad = grads[0];
+        const Tensor &logits = saved[0], &idx = saved[1], &top = saved[2], &stats = saved[3], &scale = saved[4];
+        const Tensor grad = as_stored(grads[0]);
         variable_list out(7);
         {
             const at::NoGradGuard no_grad;
@@ -333,7 +337,7 @@ struct TopkDistill : torch::autograd::Function<TopkDistill> {
 Tensor topk_distill(const OptTensor& logits_, const OptTensor& idx_, const OptTensor& top_, const OptTensor& lse_, double temperature,
                     double own_temperature, int64_t reduction) {
     no_recorder();
-    const Tensor& logits = on_gpu(logits_, "logits");
+    const Tensor logits = on_gpu(logits_, "logits");
     dtype_code(logits, "logits");
     TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "logits need at least one class");
     const at::IntArrayRef rows = logits.sizes().slice(0, logits.dim() - 1);

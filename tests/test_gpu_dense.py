@@ -350,3 +350,22 @@ def test_float32_gelu_keeps_its_digits_where_it_is_small():
     want = p + d * torch.exp(-d * d / 2) / math.sqrt(2 * math.pi)
     assert bool(((y.detach().double() - d * p).abs() <= 2.0 ** -16 * (d * p).abs()).all())
     assert bool(((slope.double() - want).abs() <= 2.0 ** -15 * want.abs()).all())
+
+
+def test_views_with_a_pending_negation():
+    neg = torch._neg_view
+    x, w, b, res, dy = _make(70, 40, 90, torch.float32)
+    for i in range(4):
+        args, want = [x, w, b, res], [x, w, b, res]
+        args[i], want[i] = neg(args[i]), -want[i]
+        assert torch.equal(linear_act(*args, "silu"), linear_act(*want, "silu")), i
+    # as they come about: the imaginary part of a conjugate
+    z = torch.randn(70, 1, dtype=torch.complex64, device="cuda").conj().imag
+    assert z.is_neg() and torch.equal(linear_act(z, w[:, :1]), linear_act(z.clone(), w[:, :1]))
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    grads = [torch.autograd.grad(linear_act(*leaves, activation="silu"), leaves, g) for g in (neg(dy), -dy)]
+    assert all(torch.equal(p, q) for p, q in zip(*grads))
+    leaf = x.clone().requires_grad_()
+    through, = torch.autograd.grad(linear_act(neg(leaf), w), leaf, dy)
+    straight = (-x).requires_grad_()
+    assert torch.equal(through, -torch.autograd.grad(linear_act(straight, w), straight, dy)[0])

@@ -504,3 +504,18 @@ def test_second_derivatives_of_the_loss_are_refused():
     for t in (leaf, up):
         with pytest.raises(RuntimeError, match="differentiable twice"):
             torch.autograd.grad(g.sum() + t.sum(), t, retain_graph=True)
+
+
+def test_views_with_a_pending_negation():
+    neg = torch._neg_view
+    x, idx, top, gen = _rand(6, 200, 4, torch.float32, seed=7)
+    lse = torch.rand(6, device="cuda", generator=gen) + 4
+    assert all(torch.equal(p, q) for p, q in zip(top_logits(neg(x), 5), top_logits(-x, 5)))
+    for i in range(3):
+        args, want = [x, top, lse], [x, top, lse]
+        args[i], want[i] = neg(args[i]), -want[i]
+        got, other = (topk_distill(t[0], idx, t[1], 1.0, t[2], reduction="none") for t in (args, want))
+        assert torch.equal(got, other), i
+    leaf = x.clone().requires_grad_()
+    grads = [torch.autograd.grad(topk_distill(leaf, idx, top, reduction="none"), leaf, g)[0] for g in (neg(lse), -lse)]
+    assert torch.equal(*grads)
