@@ -356,8 +356,11 @@ Tensor topk_distill(const OptTensor& logits_, const OptTensor& idx_, const OptTe
     TORCH_CHECK_VALUE(k >= 1 && k <= SCMIAC_DISTILL_MAX_K, "k=", k, " outside 1..", SCMIAC_DISTILL_MAX_K);
     TORCH_CHECK_VALUE(!lse.defined() || lse.sizes() == rows, "teacher_lse needs shape ", rows, ", not ", lse.sizes());
     const c10::DeviceGuard guard(logits.device());
-    if (idx.scalar_type() != at::kInt) idx = idx.scalar_type() == at::kLong ? idx.clamp(-2, 2147483647).to(at::kInt) : idx.to(at::kInt);
-    idx = idx.reshape({-1, k}).contiguous();          // (of 64-bit numbers, what is no class stays none)
+    // of numbers that 32 bits do not hold, what is no class stays none (unsigned ones from 2^63 on are negative in 64 bits)
+    if (idx.scalar_type() == at::kUInt64) idx = idx.to(at::kLong), idx = idx.masked_fill(idx.lt(0), 2147483647);
+    if (idx.scalar_type() == at::kUInt32) idx = idx.to(at::kLong);
+    if (idx.scalar_type() == at::kLong) idx = idx.clamp(-2, 2147483647);
+    idx = idx.to(at::kInt).reshape({-1, k}).contiguous();
     top = top.reshape({-1, k}).to(at::kFloat).contiguous();
     if (lse.defined()) lse = lse.reshape({-1}).to(at::kFloat).contiguous();
     const Tensor x = logits.dim() == 2 ? logits : logits.reshape({-1, logits.size(-1)});

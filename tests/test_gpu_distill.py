@@ -519,3 +519,18 @@ def test_views_with_a_pending_negation():
     leaf = x.clone().requires_grad_()
     grads = [torch.autograd.grad(topk_distill(leaf, idx, top, reduction="none"), leaf, g)[0] for g in (neg(lse), -lse)]
     assert torch.equal(*grads)
+
+
+def test_indices_of_every_type():
+    x, idx, top, _ = _rand(4, 100, 3, torch.float32, seed=2, pads=False)
+    want = topk_distill(x, idx, top, reduction="none")
+    for dtype in (torch.int8, torch.uint8, torch.int16, torch.uint16, torch.uint32, torch.int64, torch.uint64):
+        assert torch.equal(topk_distill(x, idx.to(dtype), top, reduction="none"), want), dtype
+    for dtype, bad in ((torch.uint32, 2 ** 32 - 1), (torch.uint32, 2 ** 31 + 5), (torch.uint64, 2 ** 64 - 1), (torch.uint64, 2 ** 32 + 5),
+                       (torch.uint64, 2 ** 63), (torch.int64, 2 ** 32 + 5), (torch.int64, -2 ** 32 - 1), (torch.int8, -2)):
+        rows = idx.tolist()
+        rows[1][2] = bad                                    # (unsigned, there is no -1 that could be padding)
+        table = torch.tensor(rows, dtype=dtype).cuda()
+        loss = topk_distill(x, table, top, reduction="none")
+        assert torch.isnan(loss).tolist() == [False, True, False, False], (dtype, bad)
+        assert torch.equal(loss[[0, 2, 3]], want[[0, 2, 3]])
