@@ -394,7 +394,7 @@ SCMIAC_API int scmiac_linear_backward(const void *x, int64_t ldx, const void *w,
 /*
  * The k largest entries of each row, by (value descending, index ascending), and the row's
  * log-sum-exp: a teacher's side of scmiac_distill_forward.  No counterpart in the reference.
- *   x [n, v] of `dtype`, rows ld elements apart; 1 <= k <= SCMIAC_TOP_MAX_K; temperature > 0
+ *   x [n, v] of `dtype`, rows ld elements apart; 1 <= k <= SCMIAC_TOP_MAX_K; 2^-126 <= temperature < inf
  *   values [n, k] of `dtype`, idx [n, k] int32: past the end of a row of fewer than k classes -inf and -1
  *   (the padding of the k-NN tables).  lse [n] float32 = log sum_j exp(x_j / temperature).
  * A row that holds a NaN has lse NaN; its entries are then unspecified (indices stay within the row).
@@ -420,7 +420,7 @@ SCMIAC_API int scmiac_top_logits(const void *x, int64_t ld, int64_t n, int64_t v
  *   (MEAN, SUM) float32 are what backward reads.
  * backward: dx [n, v] of `dtype` (rows ldd apart): d L / d x, times grad[i * grad_stride] (float32, device) and
  *   *scale (or 1 where scale is NULL).  Deterministic.
- *   1 <= k <= SCMIAC_DISTILL_MAX_K, 1 <= v < 2^31, 0 <= n < 2^24.
+ *   1 <= k <= SCMIAC_DISTILL_MAX_K, 1 <= v < 2^31, 0 <= n < 2^24, 2^-126 <= temperatures < inf.
  */
 #define SCMIAC_DISTILL_MAX_K 1024
 #define SCMIAC_REDUCE_NONE 0

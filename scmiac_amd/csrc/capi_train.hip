@@ -1,4 +1,5 @@
 // extern "C" boundary of the training-side kernels (declared in include/scmiac_hip.h).
+#include <float.h>
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdarg.h>
@@ -27,7 +28,8 @@ __attribute__((format(printf, 2, 3))) int fail(int code, const char* fmt, ...) {
 int done(hipError_t e, const char* what) {
     return e == hipSuccess ? SCMIAC_OK : fail(SCMIAC_ERR_HIP, "%s: %s", what, hipGetErrorString(e));
 }
-bool positive(float v) { return v > 0.f && v < INFINITY; }
+// (of a denormal one neither 1 / v nor log2(e) / v need be finite)
+bool is_temperature(float v) { return v >= FLT_MIN && v < INFINITY; }
 
 int check_dtype(int dtype) {
     if (dtype < SCMIAC_F32 || dtype > SCMIAC_BF16) return fail(SCMIAC_ERR_ARG, "dtype=%d is none of SCMIAC_F32/F16/BF16", dtype);
@@ -67,8 +69,8 @@ int check_top(int64_t n, int64_t v, int k, int dtype) {
 int check_distill(int64_t ld, int64_t n, int64_t v, int dtype, int k, float temperature, float teacher_temperature) {
     if (int rc = check_rows(ld, n, v, dtype)) return rc;
     if (k < 1 || k > SCMIAC_DISTILL_MAX_K) return fail(SCMIAC_ERR_ARG, "k=%d outside 1..%d", k, SCMIAC_DISTILL_MAX_K);
-    if (!positive(temperature) || !positive(teacher_temperature))
-        return fail(SCMIAC_ERR_ARG, "temperatures must be positive and finite");
+    if (!is_temperature(temperature) || !is_temperature(teacher_temperature))
+        return fail(SCMIAC_ERR_ARG, "temperatures must be positive, finite and at least 2^-126");
     return SCMIAC_OK;
 }
 
@@ -120,7 +122,7 @@ int scmiac_top_logits(const void* x, int64_t ld, int64_t n, int64_t v, int dtype
                       int32_t* idx, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
     if (int rc = check_top(n, v, k, dtype)) return rc;
     if (ld < 0) return fail(SCMIAC_ERR_ARG, "negative row stride");
-    if (!positive(temperature)) return fail(SCMIAC_ERR_ARG, "temperature must be positive and finite");
+    if (!is_temperature(temperature)) return fail(SCMIAC_ERR_ARG, "temperature must be positive, finite and at least 2^-126");
     if (n == 0) return SCMIAC_OK;
     if (!x || !values || !idx || !lse) return fail(SCMIAC_ERR_ARG, "NULL device pointer");
     if (int rc = check_workspace(workspace, workspace_bytes, top_logits_workspace_bytes(n, v, k, dtype))) return rc;

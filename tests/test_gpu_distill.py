@@ -534,3 +534,19 @@ def test_indices_of_every_type():
         loss = topk_distill(x, table, top, reduction="none")
         assert torch.isnan(loss).tolist() == [False, True, False, False], (dtype, bad)
         assert torch.equal(loss[[0, 2, 3]], want[[0, 2, 3]])
+
+
+def test_extreme_temperatures():
+    """At the ends of the range: one class has all the weight, or all have the same."""
+    x = torch.tensor([[3.0, -1.0, 2.0, 0.5], [0.0, 0.0, -7.0, -7.5]], device="cuda")
+    idx = torch.tensor([[2, 0], [1, 3]], dtype=torch.int32, device="cuda")
+    top = torch.zeros(2, 2, device="cuda")
+    _, order, lse = top_logits(x, 2, 2.0 ** -126)
+    assert order.tolist() == [[0, 2], [0, 1]] and lse.tolist()[0] == 3 * 2.0 ** 126      # (below 2^128: a float32)
+    assert abs(lse.tolist()[1] - math.log(2.0)) <= 2.0 ** -22
+    lse = top_logits(x, 2, 3e38)[2]
+    assert bool(((lse - math.log(4.0)).abs() <= 2.0 ** -22).all())
+    leaf = x.clone().requires_grad_()
+    loss = topk_distill(leaf, idx, top, 3e38, reduction="none")      # two of four equal classes: log 4 - log 2
+    assert bool(((loss.detach() - math.log(2.0)).abs() <= 2.0 ** -20).all())
+    assert torch.isfinite(torch.autograd.grad(loss.sum(), leaf)[0]).all()

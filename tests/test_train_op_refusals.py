@@ -162,3 +162,14 @@ def test_tracing_is_refused():
             with pytest.raises(RuntimeError, match="cannot be traced"):
                 make_fx(call, tracing_mode=mode)(x)
         call(x)
+
+
+def test_denormal_temperatures_are_refused(lib):
+    """log2(e) / T is an infinity for them, and 0 times it would be NaN."""
+    p = 4096       # never read
+    for bad in (1e-39, 4e-39, 1.1e-38, 1e-45):
+        assert lib.scmiac_top_logits(p, 10, 1, 10, F32, 4, bad, p, p, p, None, 0, None) == 1
+        assert lib.scmiac_distill_forward(p, 10, 1, 10, F32, p, p, 4, None, bad, 1.0, 0, p, p, None, p, 999, None) == 1
+        assert lib.scmiac_distill_forward(p, 10, 1, 10, F32, p, p, 4, None, 1.0, bad, 0, p, p, None, p, 999, None) == 1
+        assert "temperature" in _error(lib)
+        assert lib.scmiac_distill_backward(p, 10, 1, 10, F32, p, p, 4, bad, 1.0, p, p, 0, None, p, 10, None) == 1
