@@ -81,7 +81,7 @@ class NeighborDistillLoss(nn.Module):
         bias = None
         if self.metric == "cosine":
             z, z_ref = nn.functional.normalize(z, dim=-1), nn.functional.normalize(z_ref, dim=-1)
-        else:  # the softmax over the references does not see |z|^2
-            bias = -0.5 * (z_ref * z_ref).sum(-1)
+        else:  # the softmax over the references does not see |z|^2 (float16 has no squares from 256 on: their sum is float32)
+            bias = (-0.5 * z_ref.float().square().sum(-1)).to(z_ref.dtype)
         return topk_distill(linear_act(z, z_ref, bias), teacher_idx, teacher_logits, self.temperature, teacher_lse,
                             self.teacher_temperature, self.reduction)

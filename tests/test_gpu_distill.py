@@ -550,3 +550,20 @@ def test_extreme_temperatures():
     loss = topk_distill(leaf, idx, top, 3e38, reduction="none")      # two of four equal classes: log 4 - log 2
     assert bool(((loss.detach() - math.log(2.0)).abs() <= 2.0 ** -20).all())
     assert torch.isfinite(torch.autograd.grad(loss.sum(), leaf)[0]).all()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_euclidean_neighbors_of_large_embeddings(dtype):
+    """A component of 300: its square is no float16, the score of -45 000 is one.  Bias and score are each rounded, by at most
+    half a step of 2^15 .. 2^16 (16, 128, 2^-9), and the loss divides by the temperature."""
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    z, ref = (torch.randn(n, 8, device="cuda", generator=gen).to(dtype).requires_grad_() for n in (5, 7))
+    with torch.no_grad():
+        ref[3, 2] = 300.0
+    idx = torch.full((5, 1), 3, dtype=torch.int32, device="cuda")
+    loss = NeighborDistillLoss(64.0, 1.0, "euclidean", "none")(z, ref, idx, torch.zeros(5, 1, device="cuda"))
+    a, b = z.detach().double(), ref.detach().double()
+    want = -torch.log_softmax((a @ b.t() - 0.5 * (b * b).sum(1)) / 64.0, 1)[:, 3]
+    step = {torch.float16: 16.0, torch.bfloat16: 128.0, torch.float32: 2.0 ** -9}[dtype]
+    assert bool(((loss.detach().double() - want).abs() <= 2 * step / 64 + 2.0 ** -8).all()), (loss, want)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(loss.sum(), [z, ref]))
