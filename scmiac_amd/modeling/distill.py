@@ -8,6 +8,7 @@ neighbours a teacher's table lists instead of one positive per row.
 """
 from __future__ import annotations
 
+import torch
 import torch.nn as nn
 
 from .. import _hip
@@ -60,6 +61,13 @@ class TopKDistillLoss(nn.Module):
                             self.reduction)
 
 
+def _unit(z):
+    """Rows of length 1, worked out in float32.  Rows of zeros stay zeros: in float16 1e-12, what they are divided by
+    in float32, would be 0, and their gradients too large; it is the smallest normal number there."""
+    eps = max(1e-12, torch.finfo(z.dtype).smallest_normal)
+    return nn.functional.normalize(z.float(), dim=-1, eps=eps).to(z.dtype)
+
+
 class NeighborDistillLoss(nn.Module):
     """Soft-neighbour loss of embeddings: ``loss(z, z_ref, teacher_idx, teacher_logits)`` compares the softmax of the
     similarities of ``z [n, d]`` to all of ``z_ref [m, d]`` with the neighbours the table ``teacher_idx [n, k]`` lists
@@ -80,7 +88,7 @@ class NeighborDistillLoss(nn.Module):
     def forward(self, z, z_ref, teacher_idx, teacher_logits, teacher_lse=None):
         bias = None
         if self.metric == "cosine":
-            z, z_ref = nn.functional.normalize(z, dim=-1), nn.functional.normalize(z_ref, dim=-1)
+            z, z_ref = _unit(z), _unit(z_ref)
         else:  # the softmax over the references does not see |z|^2 (float16 has no squares from 256 on: their sum is float32)
             bias = (-0.5 * z_ref.float().square().sum(-1)).to(z_ref.dtype)
         return topk_distill(linear_act(z, z_ref, bias), teacher_idx, teacher_logits, self.temperature, teacher_lse,

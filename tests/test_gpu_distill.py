@@ -567,3 +567,23 @@ def test_euclidean_neighbors_of_large_embeddings(dtype):
     step = {torch.float16: 16.0, torch.bfloat16: 128.0, torch.float32: 2.0 ** -9}[dtype]
     assert bool(((loss.detach().double() - want).abs() <= 2 * step / 64 + 2.0 ** -8).all()), (loss, want)
     assert all(torch.isfinite(g).all() for g in torch.autograd.grad(loss.sum(), [z, ref]))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_cosine_neighbors_with_rows_of_zeros(dtype):
+    """A row of zeros has similarity 0 to everything: its own loss is log 9, and it is one class like any other.
+
+    The other scores are products of two unit vectors of 16 components, each component and the product rounded to
+    the type: 2^-8 (bfloat16) of at most 1 three times, over the temperature; the loss takes two of them."""
+    gen = torch.Generator(device="cuda").manual_seed(6)
+    z, ref = (torch.randn(n, 16, device="cuda", generator=gen).to(dtype).requires_grad_() for n in (4, 9))
+    with torch.no_grad():
+        z[1], ref[2] = 0.0, 0.0
+    idx = torch.tensor([[2], [5], [0], [8]], dtype=torch.int32, device="cuda")
+    loss = NeighborDistillLoss(0.5, 1.0, "cosine", "none")(z, ref, idx, torch.zeros(4, 1, device="cuda"))
+    a, b = (torch.nn.functional.normalize(t.detach().double(), dim=1) for t in (z, ref))
+    want = -torch.log_softmax(a @ b.t() / 0.5, 1).gather(1, idx.long())[:, 0]
+    assert abs(float(want[1]) - math.log(9.0)) < 1e-12
+    u = torch.finfo(dtype).eps / 2
+    assert bool(((loss.detach().double() - want).abs() <= 12 * u + 2.0 ** -18).all()), (loss, want)
+    assert all(torch.isfinite(g).all() for g in torch.autograd.grad(loss.sum(), [z, ref]))
