@@ -493,7 +493,7 @@ inline unsigned join_blocks(long long elements) {
 // 1024 x 480 -> 1024 25.5 / 17.3 us, 256 x 128 -> 30 (four steps) 6.9 / 6.3; but 256 x 50 -> 128 (two) 5.1 / 6.5.
 constexpr unsigned kFewPieces = 256;
 constexpr int kGroups = 4;
-inline bool share_pieces(unsigned pieces, long long longest) { return pieces <= kFewPieces && longest > 3 * kDepth; }
+inline bool share_pieces(long long pieces, long long longest) { return pieces <= kFewPieces && longest > 3 * kDepth; }
 
 // Pieces of the contraction, of the least expected time: the products of one launch are cut into pieces of about the same
 // number of steps, so many as a piece and the chip then take least for.  With two or more pieces at it, or one of
@@ -1393,10 +1393,12 @@ hipError_t backward_large(const LinearArgs& a, const void* z, const void* dy, vo
     return hipGetLastError();
 }
 
-// The small tiles' backward pass: the same cuts and scratch, dx's in front of dw's, whichever of its outputs are wanted.
+// The small tiles' backward pass: the same cuts, groups of waves and scratch, dx's in front of dw's, whichever of its outputs
+// are wanted, so that a gradient is the same number beside others and alone.
 struct BackwardPlan {
     int tn;
     bool few_rows;           // of dx
+    bool share;
     TilePlan dx, dw;
     size_t dx_bytes, total;
 };
@@ -1409,6 +1411,13 @@ BackwardPlan plan_backward(long long m, long long n, long long k, int dtype, int
     TilePlan plan[2];
     plan_tiles(of, o.tn, esize, act, true, plan);
     o.dx = plan[0], o.dw = plan[1];
+    long long pieces = 0, longest = 0;
+    for (int i = 0; i < 2; ++i) {
+        if (of[i].rows == 0) continue;
+        pieces += ceil_div(of[i].rows, kTileSize / o.tn) * ceil_div(of[i].cols, o.tn) * plan[i].splits;
+        if (plan[i].len > longest) longest = plan[i].len;
+    }
+    o.share = share_pieces(pieces, longest);
     o.dx_bytes = ((o.few_rows ? few_dx_bytes(m, n, k, esize) : part_bytes(of[0], o.dx)) + 255) & ~(size_t)255;
     o.total = o.dx_bytes + part_bytes(of[1], o.dw);      // (dbias alone: one column in place of k)
     return o;
@@ -1425,10 +1434,9 @@ void run_tiles(TileArgs& p, void* ws, hipStream_t stream) {
         linear_tile_forward_kernel<T, 1, TN><<<dim3(pieces), kThreads, 0, stream>>>(p);
 }
 template <typename T, int TN>
-void run_tiles_backward(const TileArgs& dx, unsigned pieces_dx, const TileArgs& dw, unsigned pieces_dw, hipStream_t stream) {
+void run_tiles_backward(const TileArgs& dx, unsigned pieces_dx, const TileArgs& dw, unsigned pieces_dw, bool share, hipStream_t stream) {
     const unsigned pieces = pieces_dx + pieces_dw;
-    const long long longest_dx = pieces_dx ? dx.split_len : 0, longest_dw = pieces_dw ? dw.split_len : 0;
-    if (share_pieces(pieces, longest_dx > longest_dw ? longest_dx : longest_dw))
+    if (share)
         linear_tile_backward_kernel<T, kGroups, TN><<<dim3(pieces), kThreads * kGroups, 0, stream>>>(dx, pieces_dx, dw);
     else
         linear_tile_backward_kernel<T, 1, TN><<<dim3(pieces), kThreads, 0, stream>>>(dx, pieces_dx, dw);
@@ -1476,9 +1484,9 @@ hipError_t backward_t(const LinearArgs& a, const void* z, const void* dy, void* 
     }
     if (pieces_dx + pieces_dw == 0) return hipGetLastError();
     if (plan.tn == 32)
-        run_tiles_backward<T, 32>(p, pieces_dx, q, pieces_dw, stream);
+        run_tiles_backward<T, 32>(p, pieces_dx, q, pieces_dw, plan.share, stream);
     else
-        run_tiles_backward<T, 64>(p, pieces_dx, q, pieces_dw, stream);
+        run_tiles_backward<T, 64>(p, pieces_dx, q, pieces_dw, plan.share, stream);
     if (pieces_dx == 0) p.splits = 1;      // (its own launches have joined it)
     if (p.splits > 1 || q.splits > 1) {
         const long long ex = p.splits > 1 ? p.rows * p.cols : 0, ew = q.splits > 1 ? q.rows * q.cols : 0;
