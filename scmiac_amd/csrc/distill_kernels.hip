@@ -322,11 +322,12 @@ struct WaveList {
         constexpr int kLots = N / 4;
 #pragma unroll 1
         for (int h = 0; h < kLots; ++h) {
+            const int mine = kLots == 1 || (int)(threadIdx.x & 63) / (64 / kLots) == h ? valid : 0;
+            if (!any_lane(mine > 0)) continue;       // (single elements are the first lanes')
             room();
-            const bool turn = kLots == 1 || (int)(threadIdx.x & 63) / (64 / kLots) == h;
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-                const bool take = turn && i < valid && (open || f[i] > tau);
+                const bool take = i < mine && (open || f[i] > tau);
                 append(ballot(take), take, f[i], first + i);
             }
         }
