@@ -483,7 +483,7 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
                     const float vm = unpack<T>(ahead[u], f);
                     ahead[u] = fetch(at + (kAhead + u) * step);
                     sum.add(f, vm, c);
-                    if (any_lane(vm > list.tau)) list.push(f, (uint32_t)(body + (at + u * step + lane) * N));
+                    if (any_lane(vm > list.tau)) list.push(f, (uint32_t)body + (uint32_t)(at + u * step + lane) * N);
                     __builtin_amdgcn_sched_barrier(0);      // one vector's floats in registers at a time
                 }
                 if (!list.open && list.cnt <= WaveList<T>::kCap) {
@@ -499,11 +499,11 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
             const bool single = to > from;
             for (int u = 0; u < (single ? 1 : kAhead); ++u) {
                 float f[N];
-                int first;
+                uint32_t first;      // (of lanes behind the end it may pass 31 bits)
                 int valid;
                 if (single) {
-                    first = from + lane;
-                    valid = first < to ? 1 : 0;
+                    first = (uint32_t)from + lane;
+                    valid = lane < to - from ? 1 : 0;
                     f[0] = valid ? to_f32(xr[first]) : none;
 #pragma unroll
                     for (int i = 1; i < N; ++i) f[i] = none;
@@ -512,9 +512,9 @@ __global__ __launch_bounds__(kThreads) void top_logits_kernel(const T* __restric
                     const Vec16<T> v = fetch(at + u * step);
                     unpack<T>(v, f);
                     valid = at + u * step + lane < nv ? N : 0;
-                    first = body + (at + u * step + lane) * N;
+                    first = (uint32_t)body + (uint32_t)(at + u * step + lane) * N;
                 }
-                list.push_careful(f, (uint32_t)first, valid);
+                list.push_careful(f, first, valid);
             }
             if (!single) at += kAhead * step;
         }

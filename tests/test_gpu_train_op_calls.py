@@ -233,3 +233,30 @@ def test_two_graphs_of_a_training_step_replayed_in_turn():
             eager = step()
             assert all(torch.equal(p, q) for p, q in zip(out, eager)), turn
         torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("start", [0, 1])
+def test_rows_of_as_many_classes_as_there_may_be(start):
+    """2^31 - 1 classes: positions of lanes behind the end of the row pass 31 bits."""
+    v = 2 ** 31 - 1 - start
+    x = torch.full((1, 2 ** 31 - 1), -2.0, dtype=torch.bfloat16, device="cuda")[:, start:]
+    at = [v - 1, 0, 12345, v // 2, v - 2, v - 6, v - 9, 2 ** 30 + 1]
+    for rank, j in enumerate(at):
+        x[0, j] = 30.0 - 2 * rank
+    values, idx, lse = top_logits(x, 10)
+    assert idx[0, :8].tolist() == at and values[0, :8].tolist() == [30.0 - 2 * r for r in range(8)]
+    assert idx[0, 8:].tolist() == [1, 2] and values[0, 8:].tolist() == [-2.0, -2.0]
+    want = math.log(sum(math.exp(30.0 - 2 * r) for r in range(8)) + (v - 8) * math.exp(-2.0))
+    # 2^31 equal terms: a lane adds up 2^31 / 2^16 of them, each addition off by up to 2^-24 of the sum
+    assert abs(float(lse) - want) < 2.0 ** -9
+    table = torch.tensor([[v - 1, 0, v, v // 2]], device="cuda")
+    assert torch.isnan(topk_distill(x, table, torch.zeros(1, 4, device="cuda"), reduction="none")).all()      # v is no class
+    table[0, 2] = v - 2
+    leaf = x.requires_grad_()
+    loss = topk_distill(leaf, table, torch.zeros(1, 4, device="cuda"), reduction="none")
+    dx, = torch.autograd.grad(loss, leaf, torch.ones(1, device="cuda"))
+    scores = [30.0, 28.0, 22.0, 24.0]
+    assert abs(loss.item() - (want - sum(scores) / 4 - math.log(4.0))) < 2.0 ** -9
+    for j, s in zip(table[0].tolist(), scores):
+        p = math.exp(s - want)
+        assert abs(float(dx[0, j]) - (p - 0.25)) <= 2.0 ** -8 * abs(p - 0.25) + 2.0 ** -9
