@@ -371,8 +371,9 @@ SCMIAC_API int scmiac_ntxent2_backward(const float *zi, const float *zj, int64_t
  *     z = x w^T + bias,   y = act(z) + residual
  *   x [m, k] (rows ldx elements apart), w [n, k] (ldw), bias [n] or NULL, residual [m, n] (ldr) or NULL;
  *   y [m, n] out; z [m, n] out: the pre-activation as backward reads it, or NULL.  All of one `dtype`;
- *   sums in float32 (float32 products are exact to float32's own rounding; an infinity among float32 inputs
- *   may come out as NaN).  m >= 0; n, k >= 1.
+ *   sums in float32 (float32 products are exact to float32's own rounding; in a large layer an infinity among float32
+ *   inputs may come out as NaN, and a value below 2^-108 is taken with an error of up to 2^-134).  m >= 0; n, k >= 1.
+ *   The outputs of these functions may not overlap their inputs.
  * backward: dy [m, n]; z as forward left it (may be NULL for SCMIAC_ACT_NONE);
  *   dx [m, k], dw [n, k], dbias [n] out, each may be NULL.  The gradient of `residual` is dy itself.
  *   Sums over rows are taken in an order that depends on the shape alone: results repeat bit for bit.

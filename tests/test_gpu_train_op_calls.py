@@ -260,3 +260,25 @@ def test_rows_of_as_many_classes_as_there_may_be(start):
     for j, s in zip(table[0].tolist(), scores):
         p = math.exp(s - want)
         assert abs(float(dx[0, j]) - (p - 0.25)) <= 2.0 ** -8 * abs(p - 0.25) + 2.0 ** -9
+
+
+@pytest.mark.parametrize("dtype,scale", [(torch.float16, 1e-6), (torch.bfloat16, 1e-39), (torch.float32, 1e-30), (torch.float32, 1e-36),
+                                         (torch.float32, 1e-39)])
+@pytest.mark.parametrize("m,k,n", [(2056, 1048, 2000), (300, 200, 70), (1, 4096, 4097), (4, 4096, 4104)])
+def test_small_and_denormal_inputs_count(m, k, n, dtype, scale):
+    """x and dy of numbers at or below the type's smallest normal one, w large: nothing is taken for zero.  In the large layer a
+    float32 value is three bfloat16 planes, which end at 2^-133: off by half of that where its own digits go further."""
+    g = torch.Generator(device="cuda").manual_seed(m)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g, dtype=torch.float64)  # noqa: E731
+    x, dy = ((r(*s) * scale).to(dtype) for s in ((m, k), (m, n)))
+    w = (r(n, k) * (1000.0 if dtype == torch.float16 else 1e12)).to(dtype)
+    leaf = x.requires_grad_()
+    y = linear_act(leaf, w)
+    dx, = torch.autograd.grad(y, leaf, dy)
+    u, tiny = torch.finfo(dtype).eps / 2, torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    large = dtype == torch.float32 and m > 1000
+    for got, a, b in ((y.detach(), x.detach().double(), w.double().t().contiguous()), (dx, dy.double(), w.double())):
+        want, size = a @ b, a.abs() @ b.abs()
+        bound = u * want.abs() + tiny + a.shape[1] * 2.0 ** -23 * size + (2.0 ** -134 * b.abs().sum(0) if large else 0)
+        assert bool(((got.double() - want).abs() <= bound).all())
+        assert bool((got != 0)[want.abs() > 4 * bound].all())
