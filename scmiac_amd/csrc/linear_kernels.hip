@@ -330,6 +330,8 @@ __device__ __forceinline__ void tile_product(const TileArgs& p, unsigned piece, 
                     T vz[8];
                     take_run<T, 8>(vz, z + at, count);
                     slope_values(p.act, g, vz);
+                    // (dz as the matrix instructions take it: in the half types one rounding more, which makes the errors of
+                    // dx and dw 1.45 times those of their own rounding; a second plane of dz would double both products)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) va[u][e] = from_f32<T>(g[e]);
                 }
@@ -710,6 +712,8 @@ constexpr long long kMaxFewCols = 1 << 22;   // splits of dx fit a grid's second
 // float32:  1 row 4096 -> 16384 24 / 35, 45 / 94, and 50 -> 128 3.2 / 4.4, 3.5 / 6.1;  2 rows 4.2 / 4.4, 4.7 / 6.1;
 // 4 rows 4096 -> 16384 28 / 35, 52 / 94, 4096 -> 4096 14.6 / 14.8, 21 / 30, 500 -> 1000 9.1 / 7.2, 9.1 / 9.2;
 // 8 rows 4096 -> 16384 52 / 35, 71 / 94, 500 -> 1000 16 / 7.3, 16 / 9.5.
+// (Blocks are as many as outputs allow, 16 to 128 each: for one or two rows of very many inputs and few outputs that is too few.
+// 1 row 100 000 -> 16 53 / 18, 146 / 25; 20 000 -> 200 14.8 / 11.3, 17.4 / 17.1; 4096 -> 16 5.5 / 7.3 in bfloat16.)
 bool has_few_rows(long long m, long long n, long long k, bool float32) {
     if (m < 1 || m > kFewRows || n > kMaxFewCols) return false;
     const long long weights = n * k;
@@ -784,7 +788,8 @@ hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
 // (with operands of zeros, at a higher clock, 152 and with the loads 186).  Tiles of 128 x 128 a wave take
 // 247 us, steps of 32 with three on their way 272, a fifth slot for an operand 243.
 //
-// float32 operands come as three bf16 planes whose sum is the value to 2^-25 or better: the product is
+// float32 operands come as three bf16 planes whose sum is the value to 2^-25 or better (to 2^-134 below 2^-108, where the planes'
+// numbers end; an infinity makes NaN of the other planes' zeros): the product is
 // the six products of planes that matter (the other three are below 2^-24 of the result), run as one
 // contraction six times as long.  Six passes at the bf16 rate are 2.6 times as fast as float32 MFMA.
 
@@ -1148,7 +1153,7 @@ __device__ __forceinline__ void split_planes(float v, typename Plane<T>::type (&
         o[1] = m;
         o[2] = static_cast<bf16>(r1 - static_cast<float>(m));
     } else {
-        o[0] = from_f32<T>(v);
+        o[0] = from_f32<T>(v);      // (of dz the one rounding more that the small tiles make, too)
     }
 }
 template <typename T, bool kSlope>

@@ -17,10 +17,15 @@ def linear_act(x, weight, bias=None, residual=None, activation="none"):
     """``act(x @ weight.T + bias) + residual`` on the GPU.
 
     ``x [..., k]``, ``weight [n, k]``, ``bias [n]``, ``residual [..., n]``: all float32, float16 or bfloat16 and on
-    one device; the result has their type.  ``activation``: ``"none"``, ``"relu"``, ``"gelu"`` (with the error
-    function) or ``"silu"``.  Gradients of all four; not differentiable twice.  ``x``, ``weight`` and ``residual``
-    may be strided; in float32 the product is as exact as float32 sums allow.  What an infinity or a NaN reaches is not
-    finite; a large float32 layer makes NaN of it where smaller ones may keep the infinity."""
+    one device (``torch.autocast`` casts none of them); the result has their type.  ``activation``: ``"none"``, ``"relu"``,
+    ``"gelu"`` (with the error function) or ``"silu"``.  ``x``, ``weight`` and ``residual`` may be strided; in float32 the product
+    is as exact as float32 sums allow.  What an infinity or a NaN reaches is not finite; a large float32 layer makes NaN
+    of an infinity where smaller ones may keep it.
+
+    Gradients of all four, each the same number beside others and alone.  In the half types backward reads the
+    pre-activation and the gradient of it rounded to the type, as a layer of separate operations does.  Refused with an error:
+    second derivatives, forward-mode derivatives, tracing (``torch.jit.trace``, ``torch.export``; ``torch.compile`` runs it
+    as it is between its graphs)."""
     _hip._cuda_device(x, "x")
     act = _hip.ACTIVATIONS.get(activation)
     if act is None:

@@ -20,7 +20,8 @@ def top_logits(logits, k, temperature=1.0):
 
     Returns ``(values [..., k], idx [..., k] int32, lse [...] float32)``; ``values`` has the logits' type,
     ``lse`` is ``log sum exp(logits / temperature)`` over the whole row.  Rows of fewer than ``k`` classes are padded
-    with ``-inf`` and -1.  No gradient flows: a teacher is a constant."""
+    with ``-inf`` and -1; of a row with a NaN ``lse`` is NaN and the entries are unspecified.  No derivative flows: a teacher is a
+    constant.  Cannot be traced."""
     _hip._cuda_device(logits, "logits")
     return _hip.torch_ops().top_logits(logits, int(k), temperature)
 
@@ -36,9 +37,10 @@ def topk_distill(logits, teacher_idx, teacher_logits, temperature=1.0, teacher_l
     ``logits [..., v]`` float32, float16 or bfloat16, rows may be strided; ``teacher_idx [..., k]`` (k at most 1024)
     whole numbers, -1 for padding, a class may be listed twice; ``teacher_logits [..., k]``; ``teacher_temperature``
     defaults to ``temperature``.  ``reduction``: ``"none"``, ``"sum"`` or ``"mean"`` over the rows that have a teacher: rows
-    of padding only, of teacher logits that are all ``-inf`` and of student logits that are all ``-inf`` have loss and
-    gradient 0 and are left out.  An index that is no class makes its row's loss and gradient NaN (nothing waits for the GPU
-    to raise).  Gradients for ``logits`` alone: the teacher has to be detached."""
+    of padding only or of teacher logits that are all ``-inf``, whatever the student's logits hold, and rows of student logits that
+    are all ``-inf`` have loss and gradient 0 and are left out.  An index that is no class makes its row's loss and gradient NaN (nothing waits for the GPU
+    to raise).  Gradients for ``logits`` alone: the teacher has to be detached.  Second and forward-mode derivatives and tracing
+    are refused."""
     _hip._cuda_device(logits, "logits")
     number = _hip.REDUCTIONS.get(reduction)
     if number is None:
