@@ -20,24 +20,41 @@ using namespace train;
 enum { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 enum { kForward = 0, kDx = 1, kDw = 2 };
 
-constexpr float kSqrtHalf = 0.70710678118654752440f;
 constexpr float kInvSqrt2Pi = 0.39894228040143267794f;
 
 __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * z)); }      // (good to a step of float32)
 
-// The normal distribution function P(z), and e = exp(-z^2 / 2).  In float32 by the complementary error function: 1 + erf
-// cancels where P is small (at z = -5 it is off by 4 %; this keeps 16 bits down to -8, and costs 112 for 101 us at
-// 2000 x 60 -> 5000, forward and backward).  For the half types P(-a) = e t q(t), t = 1 / (1 + 0.27 a),
-// where q is a polynomial fitted to a relative error of 1.8e-6 (least squares, the weights raised where the error is largest):
-// a hundredth of their rounding, and half the instructions of the error function (2000 x 60 -> 5000 in bfloat16, forward and
-// backward, 85 -> 66 us).
+// The normal distribution function P(z), and e = exp(-z^2 / 2).  P(-a) = e t q(t), t = 1 / (1 + s a), where q is a polynomial
+// fitted to it (least squares of the relative error, the weights raised where that is largest).
+// Half types: one for all a, off by 1.8e-6 relative, a hundredth of their rounding, at half the instructions of the error function
+// (2000 x 60 -> 5000 in bfloat16, forward and backward, 85 -> 66 us).
+// float32: from a = 1 on, off by 8e-8; below 1/2 + z r(z^2), off by 4e-8, where e t q(t) would lose two bits.  P then has a relative error of
+// 1.4e-7 for positive z, 1e-6 down to -3 and 4e-6 to -9, the last from the exponent's rounding.  (1 + erf cancels there: at z = -5 it
+// is off by 4 %.  The complementary error function is as good as this and costs 885 for 740 us at 16384 x 4096 -> 120, forward
+// and backward, where backward works out a slope 64 times.)
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
     e = fast_exp2(-0.5f * kLog2e * z * z);
+    const float a = fabsf(z);
     if constexpr (sizeof(T) == 4) {
-        return 0.5f * erfcf(-z * kSqrtHalf);
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.25f, a, 1.f)), zz = z * z;
+        float q = -0.045124784111976624f;
+        q = fmaf(q, t, 0.1043723002076149f);
+        q = fmaf(q, t, -0.01647164486348629f);
+        q = fmaf(q, t, 0.08863063901662827f);
+        q = fmaf(q, t, 0.07475871592760086f);
+        q = fmaf(q, t, 0.09441080689430237f);
+        q = fmaf(q, t, 0.09966612607240677f);
+        q = fmaf(q, t, 0.09973771125078201f);
+        q *= e * t;
+        float r = 9.423524170415476e-05f;
+        r = fmaf(r, zz, -0.001169353723526001f);
+        r = fmaf(r, zz, 0.009967196732759476f);
+        r = fmaf(r, zz, -0.06648958474397659f);
+        r = fmaf(r, zz, 0.3989422619342804f);
+        return a < 1.f ? fmaf(r, z, 0.5f) : z > 0.f ? 1.f - q : q;
     } else {
-        const float t = __builtin_amdgcn_rcpf(fmaf(0.27f, fabsf(z), 1.f));
+        const float t = __builtin_amdgcn_rcpf(fmaf(0.27f, a, 1.f));
         float q = -0.06008049888899402f;
         q = fmaf(q, t, 0.15620462423136175f);
         q = fmaf(q, t, -0.021565300509812337f);
@@ -504,7 +521,8 @@ inline bool share_pieces(long long pieces, long long longest) { return pieces <=
 // length, a third more); a join costs 6 us, and for each of a value's sums its fetch and its way to memory and back.
 // Forward in float32, two blocks to a compute unit wherever the depth allows / this rule: 912 x 3499 -> 1098 170 / 100 us,
 // 1024 x 1024 -> 1024 35 / 29, 33 x 1802 -> 12 15.5 / 10.3; forward and backward with gelu
-// 20 x 3000 -> 1063 48 / 37, 191 x 732 -> 1446 53 / 46, 904 x 108 -> 4686 90 / 88, 2000 x 60 -> 5000 105 / 106.
+// 20 x 3000 -> 1063 48 / 37, 191 x 732 -> 1446 53 / 46, 904 x 108 -> 4686 90 / 88, 2000 x 60 -> 5000 105 / 106
+// (gelu by the error function; this rule now 77 and 92).
 struct TilePlan {
     int splits;
     long long len;
@@ -783,8 +801,8 @@ hipError_t run_few_rows_dx(TileArgs p, void* ws, hipStream_t stream) {
 // of many rows would hit the same banks every time; so a lane fetches the chunk that belongs there once rows
 // are turned against each other, and the reads look it up.
 // Bound by the LDS (three operand reads to eight products, and the memory pipe's writes) and the clock, beside the matrix pipe:
-// 8192 x 4096 -> 4096 in bf16 235 us = 1.17 PFLOP/s, its backward pass 471; with gelu and residual 783 together, 890 with
-// turned copies of the operands and the compiler's order of the reads.  Without the loads from memory it takes 202 us
+// 8192 x 4096 -> 4096 in bf16 235 us = 1.17 PFLOP/s, its backward pass 471; with gelu and residual 783 to 809 together on several
+// cards, 890 with turned copies of the operands and the compiler's order of the reads.  Without the loads from memory it takes 202 us
 // (with operands of zeros, at a higher clock, 152 and with the loads 186).  Tiles of 128 x 128 a wave take
 // 247 us, steps of 32 with three on their way 272, a fifth slot for an operand 243.
 //
@@ -1235,7 +1253,7 @@ __global__ __launch_bounds__(kThreads) void linear_bias_kernel(const float* __re
 // 64 x 64 tiles' slower inner loop.  Forward and backward, large / small tiles, in microseconds: bfloat16
 // 1024 x 512 -> 1024 45 / 40, 765 x 2937 -> 252 57 / 44, 2048 x 1024 -> 1024 57 / 64, 8192 x 64 -> 8192 153 / 164; float32
 // 1024 x 1024 -> 1024 124 / 81, 10412 x 2000 -> 128 321 / 205, 912 x 3499 -> 1098 270 / 280 and with silu 270 / 364,
-// 16384 x 4096 -> 120 760 / 571 and with gelu 766 / 774, 100 000 x 64 -> 512 664 / 261.
+// 16384 x 4096 -> 120 760 / 571 and with gelu by the error function 766 / 774 (small now 681), 100 000 x 64 -> 512 664 / 261.
 bool is_large(long long rows, long long cols, long long depth, int dtype) {
     const int least = dtype == 0 ? 128 : 64;
     if (rows <= kFewRows || cols < least || depth < least) return false;

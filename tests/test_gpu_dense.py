@@ -338,10 +338,9 @@ def test_the_gradient_of_the_residual_keeps_its_derivatives():
 
 
 def test_float32_gelu_keeps_its_digits_where_it_is_small():
-    """z = x * 1 is exact here.  P(z) = erfc(a) / 2, a = -z / sqrt(2) off by two roundings of 2^-24, moves by 2 a^2 <= 64 times
-    as much, 2^-17, and erfc by a few 2^-24 of its own: 2^-16 of gelu in all.  In the slope, P + z phi, the exponent z^2 / 2
-    (46 as a power of two) carries four roundings, 2^-17 of phi, and the two terms of opposite sign add up to 1.3 times
-    the sum at most: 2^-15."""
+    """z = x * 1 is exact here.  P(z) = exp(-z^2 / 2) times a smooth factor: the exponent (46 as a power of two at z = -8)
+    carries three roundings, 46 x 0.7 x 3 x 2^-24 < 2^-17, the factor less than 2^-20: 2^-16 of gelu in all.  In the slope, P + z phi,
+    the two terms of opposite sign add up to 1.3 times the sum at most: 2^-15."""
     z = torch.linspace(-8, -3, 501, device="cuda").reshape(-1, 1).requires_grad_()
     y = linear_act(z, torch.ones(1, 1, device="cuda"), activation="gelu")
     slope, = torch.autograd.grad(y, z, torch.ones_like(y))
@@ -369,3 +368,18 @@ def test_views_with_a_pending_negation():
     through, = torch.autograd.grad(linear_act(neg(leaf), w), leaf, dy)
     straight = (-x).requires_grad_()
     assert torch.equal(through, -torch.autograd.grad(linear_act(straight, w), straight, dy)[0])
+
+
+def test_float32_gelu_over_its_range():
+    """From -1 on P(z) is 1/2 + z r(z^2), or 1 - q with q < 0.16: fits of 4e-8 and 8e-8 and a few roundings of 2^-24, of at least
+    0.159 at z = -1, so 2^-21 of gelu in all; of the slope, whose terms are at most 1.13, 2^-21."""
+    z = torch.cat([torch.linspace(-1, 9, 4001), torch.tensor([0.0, -0.0, 1e-30, -1e-30, 1e-6, -1e-6, 40.0, 1e30])]).reshape(-1, 1).cuda()
+    z.requires_grad_()
+    y = linear_act(z, torch.ones(1, 1, device="cuda"), activation="gelu")
+    slope, = torch.autograd.grad(y, z, torch.ones_like(y))
+    d = z.detach().double()
+    p = torch.special.erfc(-d / math.sqrt(2)) / 2
+    assert bool(((y.detach().double() - d * p).abs() <= 2.0 ** -21 * (d * p).abs()).all())
+    want = p + d * torch.exp(-d * d / 2) / math.sqrt(2 * math.pi)
+    assert bool(((slope.double() - want).abs() <= 2.0 ** -21).all())
+    assert linear_act(torch.full((1, 1), math.inf, device="cuda"), torch.ones(1, 1, device="cuda"), activation="gelu").item() == math.inf
