@@ -26,12 +26,12 @@ __device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf
 
 // The normal distribution function P(z), and e = exp(-z^2 / 2).  P(-a) = e t q(t), t = 1 / (1 + s a), where q is a polynomial
 // fitted to it (least squares of the relative error, the weights raised where that is largest).
-// Half types: one for all a, off by 1.8e-6 relative, a hundredth of their rounding, at half the instructions of the error function
-// (2000 x 60 -> 5000 in bfloat16, forward and backward, 85 -> 66 us).
-// float32: from a = 1 on, off by 8e-8; below 1/2 + z r(z^2), off by 4e-8, where e t q(t) would lose two bits.  P then has a relative error of
-// 1.4e-7 for positive z, 1e-6 down to -3 and 4e-6 to -9, the last from the exponent's rounding.  (1 + erf cancels there: at z = -5 it
-// is off by 4 %.  The complementary error function is as good as this and costs 885 for 740 us at 16384 x 4096 -> 120, forward
-// and backward, where backward works out a slope 64 times.)
+// Half types: one for all a, off by 1.8e-6 relative, a hundredth of their rounding, at half the instructions of the error
+// function (2000 x 60 -> 5000 in bfloat16, forward and backward, 85 -> 66 us).
+// float32: from a = 1 on, off by 8e-8; below it 1/2 + z r(z^2), off by 4e-8, where e t q(t) would lose two bits.  P then has a
+// relative error of 1.4e-7 for positive z, 1e-6 down to -3 and 4e-6 down to -9, the last from the exponent's rounding.  (1 + erf
+// cancels there: at z = -5 it is off by 4 %.  The complementary error function is as good as this and costs 885 us for 681 at
+// 16384 x 4096 -> 120, forward and backward, where backward works out a slope 64 times; with erf 740.)
 template <typename T>
 __device__ __forceinline__ float normal_cdf(float z, float& e) {
     e = fast_exp2(-0.5f * kLog2e * z * z);

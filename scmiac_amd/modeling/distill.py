@@ -37,10 +37,10 @@ def topk_distill(logits, teacher_idx, teacher_logits, temperature=1.0, teacher_l
     ``logits [..., v]`` float32, float16 or bfloat16, rows may be strided; ``teacher_idx [..., k]`` (k at most 1024)
     whole numbers, -1 for padding, a class may be listed twice; ``teacher_logits [..., k]``; ``teacher_temperature``
     defaults to ``temperature``.  ``reduction``: ``"none"``, ``"sum"`` or ``"mean"`` over the rows that have a teacher: rows
-    of padding only or of teacher logits that are all ``-inf``, whatever the student's logits hold, and rows of student logits that
-    are all ``-inf`` have loss and gradient 0 and are left out.  An index that is no class makes its row's loss and gradient NaN (nothing waits for the GPU
-    to raise).  Gradients for ``logits`` alone: the teacher has to be detached.  Second and forward-mode derivatives and tracing
-    are refused."""
+    of padding only or of teacher logits that are all ``-inf``, whatever the student's logits hold, and rows of student
+    logits that are all ``-inf`` have loss and gradient 0 and are left out.  An index that is no class makes its row's loss
+    and gradient NaN (nothing waits for the GPU to raise).  Gradients for ``logits`` alone: the teacher has to be detached.
+    Second derivatives, forward-mode derivatives and tracing are refused."""
     _hip._cuda_device(logits, "logits")
     number = _hip.REDUCTIONS.get(reduction)
     if number is None:
